@@ -90,6 +90,70 @@ int check_input(const char* fn, const char* name, const void* p, int dtype, int6
   return VC_OK;
 }
 
+// Shapes of the cache and window attention entries: 16-bit types, shared
+// heads, lengths of zero allowed.
+int check_serving(const char* fn, int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
+  if (dtype != VC_DTYPE_F16 && dtype != VC_DTYPE_BF16) {
+    set_last_error("%s: dtype must be VC_DTYPE_F16 or VC_DTYPE_BF16", fn);
+    return VC_ERR_ARG;
+  }
+  if (B < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv || Hq > 4096 || B > (1 << 20) || B * Hq > 65535) {
+    set_last_error("%s: need B, Hkv >= 1, Hq a multiple of Hkv and B*Hq <= 65535 (got B %lld, Hq %lld, Hkv %lld)", fn,
+                   (long long)B, (long long)Hq, (long long)Hkv);
+    return VC_ERR_ARG;
+  }
+  if (D != 64 && D != 128) {
+    set_last_error("%s: head dim must be 64 or 128 (got %lld)", fn, (long long)D);
+    return VC_ERR_ARG;
+  }
+  return VC_OK;
+}
+
+int check_tokens(const char* fn, const char* name, int64_t n) {
+  if (n < 0 || n > (int64_t(1) << 31) - 65536) {
+    set_last_error("%s: %s must be in [0, 2^31 - 65536] (got %lld)", fn, name, (long long)n);
+    return VC_ERR_ARG;
+  }
+  return VC_OK;
+}
+
+int check_cache(const char* fn, const void* pool, int64_t pages, int64_t page_size, const int32_t* table,
+                int64_t width) {
+  if (!pool || (reinterpret_cast<uintptr_t>(pool) & 127u)) {
+    set_last_error("%s: pool must be a non-null 128-byte aligned pointer", fn);
+    return VC_ERR_ARG;
+  }
+  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1))) {
+    set_last_error("%s: page_size must be 16, 32, 64, 128 or 256 (got %lld)", fn, (long long)page_size);
+    return VC_ERR_ARG;
+  }
+  if (pages < 1 || pages > INT32_MAX || width < 0 || width > INT32_MAX / page_size || (width > 0 && !table)) {
+    set_last_error("%s: need 1 <= pages < 2^31, 0 <= table_width * page_size < 2^31 and a page table", fn);
+    return VC_ERR_ARG;
+  }
+  return VC_OK;
+}
+
+int check_visibility(const char* fn, int64_t window, int64_t sinks, float sm_scale) {
+  if (window < 0 || sinks < 0 || window > INT32_MAX || sinks > INT32_MAX) {
+    set_last_error("%s: window (0 = none) and sinks must be in [0, 2^31)", fn);
+    return VC_ERR_ARG;
+  }
+  if (!(sm_scale > 0.f) || !(sm_scale <= 3.4028234663852886e38f)) {
+    set_last_error("%s: sm_scale must be positive and finite", fn);
+    return VC_ERR_ARG;
+  }
+  return VC_OK;
+}
+
+int check_workspace(const char* fn, const void* workspace, int64_t have, int64_t need) {
+  if (need > 0 && (!workspace || have < need || !aligned16(workspace))) {
+    set_last_error("%s: workspace needs %lld bytes (16-byte aligned)", fn, (long long)need);
+    return VC_ERR_WORKSPACE;
+  }
+  return VC_OK;
+}
+
 int finish(const char* fn, int rc) {
   if (rc == VC_ERR_LAUNCH) {
     const cudaError_t e = cudaGetLastError();
@@ -165,14 +229,16 @@ int vc_error_read(int device, uint32_t* code, int clear) {
     set_last_error("vc_error_read: bad device %d", device);
     return VC_ERR_ARG;
   }
-  uint32_t words[6] = {0, 0, 0, 0, 0, 0};
+  uint32_t words[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   cudaError_t e = attention_error_word(&words[0], clear != 0);
   if (e == cudaSuccess) e = read_tu_error_word(&words[5], clear != 0);   // this file: the wait self-test
   if (e == cudaSuccess) e = prep_qk_error_word(&words[1], clear != 0);
   if (e == cudaSuccess) e = prep_v_error_word(&words[2], clear != 0);
   if (e == cudaSuccess) e = prep_hadamard_error_word(&words[3], clear != 0);
   if (e == cudaSuccess) e = tensor_peak_error_word(&words[4], clear != 0);
-  *code = words[0] | words[1] | words[2] | words[3] | words[4] | words[5];
+  if (e == cudaSuccess) e = kv4_cache_error_word(&words[6], clear != 0);
+  if (e == cudaSuccess) e = window_attention_error_word(&words[7], clear != 0);
+  *code = words[0] | words[1] | words[2] | words[3] | words[4] | words[5] | words[6] | words[7];
   cudaSetDevice(prev);
   if (e != cudaSuccess) {
     set_last_error("vc_error_read: %s", cudaGetErrorString(e));
@@ -437,6 +503,154 @@ int vc_attention_fwd_e4m3qk(const uint8_t* q8, const float* qs, const uint8_t* k
              block_values ? 1 : 0, vs_per_block ? 1 : 0, sm_scale, unit_begin, unit_end, 1, k_quant_block,
              expcast == 3 ? 1 : 0};
   return finish(fn, attention_fwd(a, static_cast<cudaStream_t>(stream)));
+}
+
+int vc_kv4_append(const void* k, const void* v, const void* q, void* q_out, int dtype, int64_t B, int64_t Hq,
+                  int64_t Hkv, int64_t S, int64_t D, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s,
+                  int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_s, int64_t q_stride_b, int64_t q_stride_h,
+                  int64_t q_stride_s, int64_t qo_stride_b, int64_t qo_stride_h, int64_t qo_stride_s, const float* cos,
+                  const float* sin, int64_t rot_rows, int64_t rot_dim, int interleaved, const int32_t* positions,
+                  const int32_t* lengths, const int32_t* counts, uint8_t* pool, int64_t pages, int64_t page_size,
+                  const int32_t* page_table, int64_t table_width, void* stream) {
+  const char* fn = "vc_kv4_append";
+  if (int rc = check_serving(fn, dtype, B, q ? Hq : Hkv, Hkv, D)) return rc;
+  if (int rc = check_tokens(fn, "S", S)) return rc;
+  if (int rc = check_cache(fn, pool, pages, page_size, page_table, table_width)) return rc;
+  if (S == 0) return VC_OK;
+  if (int rc = check_input(fn, "k", k, dtype, k_stride_b, k_stride_h, k_stride_s)) return rc;
+  if (int rc = check_input(fn, "v", v, dtype, v_stride_b, v_stride_h, v_stride_s)) return rc;
+  if (q) {
+    if (int rc = check_input(fn, "q", q, dtype, q_stride_b, q_stride_h, q_stride_s)) return rc;
+    if (int rc = check_input(fn, "q_out", q_out, dtype, qo_stride_b, qo_stride_h, qo_stride_s)) return rc;
+  }
+  if (rot_dim < 0 || rot_dim > D || rot_dim % 16 || (rot_dim > 0 && (!cos || !sin || rot_rows < 1))) {
+    set_last_error("%s: rot_dim must be a multiple of 16 in [0, D] with cos and sin of at least one row", fn);
+    return VC_ERR_ARG;
+  }
+  if (!lengths) {
+    set_last_error("%s: lengths is required", fn);
+    return VC_ERR_ARG;
+  }
+  if (B * S > (int64_t(1) << 36) / ((q ? Hq : 0) + 2 * Hkv)) {
+    set_last_error("%s: B*S*(Hq + 2*Hkv) must be at most 2^36", fn);
+    return VC_ERR_ARG;
+  }
+  if (int rc = check_device()) return rc;
+  Kv4AppendArgs a{{pool, page_table, B, Hkv, pages, table_width, page_size}, k, v, q, q_out, dtype, Hq, S, D, k_stride_b,
+                  k_stride_h, k_stride_s, v_stride_b, v_stride_h, v_stride_s, q_stride_b, q_stride_h, q_stride_s,
+                  qo_stride_b, qo_stride_h, qo_stride_s, cos, sin, rot_rows, rot_dim, interleaved ? 1 : 0, positions,
+                  lengths, counts};
+  return finish(fn, kv4_append(a, static_cast<cudaStream_t>(stream)));
+}
+
+int vc_kv4_read(const uint8_t* pool, int64_t pages, int64_t page_size, const int32_t* page_table, int64_t table_width,
+                const int32_t* start, int64_t B, int64_t Hkv, int64_t N, int64_t D, void* k, void* v, int dtype,
+                int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s, int64_t v_stride_b, int64_t v_stride_h,
+                int64_t v_stride_s, void* stream) {
+  const char* fn = "vc_kv4_read";
+  if (int rc = check_serving(fn, dtype == VC_DTYPE_F32 ? int(VC_DTYPE_BF16) : dtype, B, Hkv, Hkv, D)) return rc;
+  if (int rc = check_tokens(fn, "N", N)) return rc;
+  if (int rc = check_cache(fn, pool, pages, page_size, page_table, table_width)) return rc;
+  if (N == 0) return VC_OK;
+  if (int rc = check_input(fn, "k", k, dtype, k_stride_b, k_stride_h, k_stride_s)) return rc;
+  if (int rc = check_input(fn, "v", v, dtype, v_stride_b, v_stride_h, v_stride_s)) return rc;
+  if (B * Hkv * N > (int64_t(1) << 35)) {
+    set_last_error("%s: B*Hkv*N must be at most 2^35", fn);
+    return VC_ERR_ARG;
+  }
+  if (int rc = check_device()) return rc;
+  Kv4ReadArgs a{{const_cast<uint8_t*>(pool), page_table, B, Hkv, pages, table_width, page_size}, k, v, dtype, N, D,
+                k_stride_b, k_stride_h, k_stride_s, v_stride_b, v_stride_h, v_stride_s, start};
+  return finish(fn, kv4_read(a, static_cast<cudaStream_t>(stream)));
+}
+
+int64_t vc_kv4_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D, int causal,
+                                         int64_t window, int64_t sinks, int64_t page_size, int64_t table_width,
+                                         int64_t max_length) {
+  if (B < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv || Sq < 1) return 0;
+  Kv4AttnArgs a{};
+  a.cache.B = B;
+  a.cache.Hkv = Hkv;
+  a.cache.page_size = page_size;
+  a.cache.width = table_width;
+  a.Hq = Hq;
+  a.Sq = Sq;
+  a.D = D;
+  a.causal = causal ? 1 : 0;
+  a.window = window;
+  a.sinks = sinks;
+  a.max_length = max_length;
+  return kv4_attention_workspace(a);
+}
+
+int vc_kv4_attention_fwd(const void* q, int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D,
+                         int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s, const uint8_t* pool,
+                         int64_t pages, int64_t page_size, const int32_t* page_table, int64_t table_width,
+                         const int32_t* lengths, const int32_t* q_lengths, int causal, int64_t window, int64_t sinks,
+                         int64_t max_length, float sm_scale, void* out, int64_t out_stride_b, int64_t out_stride_h,
+                         int64_t out_stride_s, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* fn = "vc_kv4_attention_fwd";
+  if (int rc = check_serving(fn, dtype, B, Hq, Hkv, D)) return rc;
+  if (int rc = check_tokens(fn, "Sq", Sq)) return rc;
+  if (int rc = check_tokens(fn, "max_length", max_length)) return rc;
+  if (int rc = check_cache(fn, pool, pages, page_size, page_table, table_width)) return rc;
+  if (int rc = check_visibility(fn, window, sinks, sm_scale)) return rc;
+  if (Sq == 0) return VC_OK;
+  if (int rc = check_input(fn, "q", q, dtype, q_stride_b, q_stride_h, q_stride_s)) return rc;
+  if (int rc = check_input(fn, "out", out, dtype, out_stride_b, out_stride_h, out_stride_s)) return rc;
+  if (!lengths) {
+    set_last_error("%s: lengths is required", fn);
+    return VC_ERR_ARG;
+  }
+  Kv4AttnArgs a{{const_cast<uint8_t*>(pool), page_table, B, Hkv, pages, table_width, page_size}, q, out, dtype, Hq, Sq,
+                D, q_stride_b, q_stride_h, q_stride_s, out_stride_b, out_stride_h, out_stride_s, lengths, q_lengths,
+                causal ? 1 : 0, window, sinks, max_length, sm_scale, workspace, workspace_bytes};
+  if (int rc = check_workspace(fn, workspace, workspace_bytes, kv4_attention_workspace(a))) return rc;
+  if (int rc = check_device()) return rc;
+  return finish(fn, kv4_attention(a, static_cast<cudaStream_t>(stream)));
+}
+
+int64_t vc_window_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D,
+                                            int causal, int64_t window, int64_t sinks) {
+  if (B < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv || Sq < 1 || Sk < 1) return 0;
+  WindowAttnArgs a{};
+  a.B = B;
+  a.Hq = Hq;
+  a.Hkv = Hkv;
+  a.Sq = Sq;
+  a.Sk = Sk;
+  a.D = D;
+  a.causal = causal ? 1 : 0;
+  a.window = window;
+  a.sinks = sinks;
+  return window_attention_workspace(a);
+}
+
+int vc_window_attention_fwd(const void* q, const void* k, const void* v, int dtype, int64_t B, int64_t Hq,
+                            int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D, int64_t q_stride_b, int64_t q_stride_h,
+                            int64_t q_stride_s, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s,
+                            int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_s, const int32_t* kv_lengths,
+                            int causal, int64_t window, int64_t sinks, float sm_scale, void* out, int64_t out_stride_b,
+                            int64_t out_stride_h, int64_t out_stride_s, void* workspace, int64_t workspace_bytes,
+                            void* stream) {
+  const char* fn = "vc_window_attention_fwd";
+  if (int rc = check_serving(fn, dtype, B, Hq, Hkv, D)) return rc;
+  if (int rc = check_tokens(fn, "Sq", Sq)) return rc;
+  if (int rc = check_tokens(fn, "Sk", Sk)) return rc;
+  if (int rc = check_visibility(fn, window, sinks, sm_scale)) return rc;
+  if (Sq == 0) return VC_OK;
+  if (int rc = check_input(fn, "q", q, dtype, q_stride_b, q_stride_h, q_stride_s)) return rc;
+  if (int rc = check_input(fn, "out", out, dtype, out_stride_b, out_stride_h, out_stride_s)) return rc;
+  if (Sk > 0) {
+    if (int rc = check_input(fn, "k", k, dtype, k_stride_b, k_stride_h, k_stride_s)) return rc;
+    if (int rc = check_input(fn, "v", v, dtype, v_stride_b, v_stride_h, v_stride_s)) return rc;
+  }
+  WindowAttnArgs a{q, k, v, out, dtype, B, Hq, Hkv, Sq, Sk, D, q_stride_b, q_stride_h, q_stride_s, k_stride_b,
+                   k_stride_h, k_stride_s, v_stride_b, v_stride_h, v_stride_s, out_stride_b, out_stride_h, out_stride_s,
+                   kv_lengths, causal ? 1 : 0, window, sinks, sm_scale, workspace, workspace_bytes};
+  if (int rc = check_workspace(fn, workspace, workspace_bytes, Sk > 0 ? window_attention_workspace(a) : 0)) return rc;
+  if (int rc = check_device()) return rc;
+  return finish(fn, window_attention(a, static_cast<cudaStream_t>(stream)));
 }
 
 int vc_tensor_peak(int kind, int n, int64_t iters, int ctas, int a_tmem, int issuers, unsigned long long* stamps,

@@ -112,6 +112,68 @@ cudaError_t prep_qk_error_word(uint32_t* code, bool clear);
 cudaError_t prep_v_error_word(uint32_t* code, bool clear);
 int attention_resources(int head_dim, int64_t* out4);
 
+// Paged 4-bit K/V cache (kv4.cuh has the record layout).
+struct Kv4CacheArgs {
+  uint8_t* pool;
+  const int32_t* table;   // [B, width] page of each page_size tokens
+  int64_t B, Hkv, pages, width, page_size;
+};
+struct Kv4AppendArgs {
+  Kv4CacheArgs cache;
+  const void *k, *v, *q;   // q optional
+  void* q_out;
+  int dtype;
+  int64_t Hq, S, D;
+  int64_t ksb, ksh, kss, vsb, vsh, vss, qsb, qsh, qss, osb, osh, oss;
+  const float *cos, *sin;  // [rot_rows, rot_dim / 2]; rot_dim 0: no rotation
+  int64_t rot_rows, rot_dim;
+  int interleaved;
+  const int32_t *positions, *lengths, *counts;   // positions [B,S] and counts [B] optional
+};
+int kv4_append(const Kv4AppendArgs& a, cudaStream_t st);
+struct Kv4ReadArgs {
+  Kv4CacheArgs cache;
+  void *k, *v;
+  int dtype;
+  int64_t N, D;
+  int64_t ksb, ksh, kss, vsb, vsh, vss;
+  const int32_t* start;   // [B] optional
+};
+int kv4_read(const Kv4ReadArgs& a, cudaStream_t st);
+cudaError_t kv4_cache_error_word(uint32_t* code, bool clear);
+struct Kv4AttnArgs {
+  Kv4CacheArgs cache;
+  const void* q;
+  void* out;
+  int dtype;
+  int64_t Hq, Sq, D;
+  int64_t qsb, qsh, qss, osb, osh, oss;
+  const int32_t *lengths, *q_lengths;   // q_lengths optional
+  int causal;
+  int64_t window, sinks, max_length;
+  float sm_scale;
+  void* workspace;
+  int64_t workspace_bytes;
+};
+int64_t kv4_attention_workspace(const Kv4AttnArgs& a);
+int kv4_attention(const Kv4AttnArgs& a, cudaStream_t st);
+struct WindowAttnArgs {
+  const void *q, *k, *v;
+  void* out;
+  int dtype;
+  int64_t B, Hq, Hkv, Sq, Sk, D;
+  int64_t qsb, qsh, qss, ksb, ksh, kss, vsb, vsh, vss, osb, osh, oss;
+  const int32_t* kv_lengths;   // [B] optional
+  int causal;
+  int64_t window, sinks;
+  float sm_scale;
+  void* workspace;
+  int64_t workspace_bytes;
+};
+int64_t window_attention_workspace(const WindowAttnArgs& a);
+int window_attention(const WindowAttnArgs& a, cudaStream_t st);
+cudaError_t window_attention_error_word(uint32_t* code, bool clear);
+
 int expcast_codes(const float* x, uint8_t* y, int64_t n, cudaStream_t st);
 
 // Tensor-core throughput measurement (tensor_peak.cu): ``ctas`` CTAs, each

@@ -1,0 +1,60 @@
+// The paged 4-bit K/V cache ("kv4"): record layout and addressing.
+//
+// pool: uint8 [pages, Hkv, page_size / 16, 18 * D].  A record holds 16 tokens
+// of one head:
+//   [0, 8D)      K codes, token t at t * D/2; channel 2i in the low four bits
+//   [8D, 16D)    V codes, likewise
+//   [16D, 17D)   K (scale, minimum) bfloat16 pairs, token t, group g at (t * D/64 + g) * 4
+//   [17D, 18D)   V (scale, minimum) pairs, likewise
+// and a value is scale * code + minimum.  A record is contiguous (2304 bytes
+// at D = 128, 1152 at D = 64; both multiples of 128), so one bulk copy brings
+// 16 tokens of K and V with their scales whatever the page size, and a page of
+// one head is contiguous too.  4.5 bits a value.
+#pragma once
+#include "common.cuh"
+#include "kernels.h"
+
+namespace vcb {
+
+constexpr int kKv4Block = 16;    // tokens of a record
+constexpr int kKv4Group = 64;    // channels that share a scale and a minimum
+
+template <int D>
+struct Kv4Rec {
+  static constexpr int kK = 0, kV = 8 * D, kKp = 16 * D, kVp = 17 * D, kBytes = 18 * D;
+  static constexpr int kCodeRow = D / 2;            // bytes of a token's codes
+  static constexpr int kParRow = D / kKv4Group * 4; // bytes of a token's (scale, minimum) pairs
+};
+
+// Page table of one call.  An entry outside [0, pages), or a token past the
+// table's width, has no record: the caller skips it and raises kErrBadIndex.
+struct Kv4Pages {
+  uint8_t* pool;
+  const int32_t* table;     // [B, width]
+  int64_t width, pages, heads;
+  int page_size, page_shift;   // page_size = 1 << page_shift, at least 16
+
+  // Byte offset of the record that holds tokens 16*blk .. 16*blk+15 of
+  // sequence b and head h, or -1.
+  template <int D>
+  __device__ __forceinline__ int64_t record(int64_t b, int64_t h, int64_t blk) const {
+    const int shift = page_shift - 4;
+    const int64_t slot = blk >> shift;
+    if (slot >= width) return -1;
+    const int32_t page = __ldg(table + b * width + slot);
+    if (page < 0 || page >= pages) return -1;
+    const int64_t in_page = blk & ((int64_t(1) << shift) - 1);
+    return (((int64_t(page) * heads + h) << shift) + in_page) * Kv4Rec<D>::kBytes;
+  }
+};
+
+inline Kv4Pages kv4_pages(const Kv4CacheArgs& c) {
+  Kv4Pages g{c.pool, c.table, c.width, c.pages, c.Hkv, static_cast<int>(c.page_size), 0};
+  while ((int64_t(1) << g.page_shift) < c.page_size) ++g.page_shift;
+  return g;
+}
+
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
+}  // namespace vcb

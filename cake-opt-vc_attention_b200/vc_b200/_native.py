@@ -43,6 +43,15 @@ SIGNATURES = {
                                 _i32, _i32, _i32, _f, _i64, _i64, _p]),
     "vc_attention_fwd_e4m3qk": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                        _i64, _i32, _i32, _i32, _i64, _f, _i64, _i64, _p]),
+    "vc_kv4_append": (_i32, [_p, _p, _p, _p, _i32] + [_i64] * 17 + [_p, _p, _i64, _i64, _i32, _p, _p, _p, _p, _i64,
+                                                                    _i64, _p, _i64, _p]),
+    "vc_kv4_read": (_i32, [_p, _i64, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _i32] + [_i64] * 6 + [_p]),
+    "vc_kv4_attention_workspace_bytes": (_i64, [_i64] * 5 + [_i32] + [_i64] * 5),
+    "vc_kv4_attention_fwd": (_i32, [_p, _i32] + [_i64] * 8 + [_p, _i64, _i64, _p, _i64, _p, _p, _i32, _i64, _i64,
+                                                              _i64, _f, _p, _i64, _i64, _i64, _p, _i64, _p]),
+    "vc_window_attention_workspace_bytes": (_i64, [_i64] * 6 + [_i32, _i64, _i64]),
+    "vc_window_attention_fwd": (_i32, [_p, _p, _p, _i32] + [_i64] * 15 + [_p, _i32, _i64, _i64, _f, _p, _i64, _i64,
+                                                                          _i64, _p, _i64, _p]),
     "vc_kernel_resources": (_i32, [_i32, C.POINTER(C.c_int64)]),
     "vc_attention_plan": (_i32, [C.c_int64, C.c_int64, C.c_int64, _i32, C.POINTER(C.c_int64)]),
     "vc_tensor_peak": (_i32, [_i32, _i32, _i64, _i32, _i32, _i32, _p, _p]),

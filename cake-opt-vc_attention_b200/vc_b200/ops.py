@@ -266,6 +266,310 @@ def attention_fwd(q8, qs, k8, ks, v8, vs, means, *, out_dtype=torch.bfloat16, sm
     return out
 
 
+# ---------------------------------------------------------------------------
+# Paged 4-bit K/V cache and window attention (inference only).
+# ---------------------------------------------------------------------------
+KV4_RECORD_TOKENS = 16
+_LAYOUTS = ("HND", "NHD")
+
+
+def _aligned(x: torch.Tensor) -> torch.Tensor:
+    """``_rowmajor`` for any strides: an axis of one element may have any
+    stride, a broadcast token axis is copied."""
+    es = x.element_size()
+    st = x.stride()
+    if st[3] == 1 and x.data_ptr() % 16 == 0 and (st[2] > 0 or x.shape[2] < 2) and \
+            all(n < 2 or (s * es) % 16 == 0 for s, n in zip(st[:3], x.shape[:3])):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(x: torch.Tensor) -> tuple:
+    """(b, h, s) strides in elements; those of one-element axes, which address nothing, as one row."""
+    d = x.shape[3]
+    st = x.stride()
+    return tuple(s if n > 1 else d for s, n in zip(st[:3], x.shape[:3]))
+
+
+def _serving(name, layout, dtype, device, *tensors):
+    """Layout, type and device checks shared by the cache and window ops; the
+    tensors (None allowed) as aligned [B,H,S,D] views."""
+    if layout not in _LAYOUTS:
+        raise ValueError(f"{name}: tensor_layout must be HND or NHD")
+    out = []
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is None:
+            out.append(None)
+            continue
+        if t.dtype is not dtype or t.device != device:
+            raise ValueError(f"{name}: tensors must share one dtype and device, got {t.dtype} on {t.device} "
+                             f"and {dtype} on {device}")
+        if t.dim() != 4:
+            raise ValueError(f"{name}: expected four-dimensional tensors, got shape {tuple(t.shape)}")
+        if grad and t.requires_grad:
+            raise ValueError(f"{name} has no backward pass; detach its inputs or call it under torch.no_grad()")
+        out.append(_aligned(t if layout == "HND" else t.transpose(1, 2)))
+    if device.type != "cuda":
+        raise ValueError(f"{name}: tensors must be on a CUDA device (no CPU fallback)")
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"{name}: FP16 or BF16 tensors required, got {dtype}")
+    return out
+
+
+def _ints(name, what, t, shape, device):
+    """An int32 contiguous device tensor of ``shape`` (None passes through)."""
+    if t is None:
+        return None
+    if tuple(t.shape) != shape or t.dtype not in (torch.int32, torch.int64) or t.device != device:
+        raise ValueError(f"{name}: {what} must be an integer tensor of shape {shape} on {device}, got "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    return (t if t.dtype is torch.int32 else t.to(torch.int32)).contiguous()
+
+
+def _cache(name, pool, page_table, device):
+    """(kv heads, head dim, page size, batch) of a pool and its page table."""
+    if pool.dtype is not torch.uint8 or pool.dim() != 4 or not pool.is_contiguous() or pool.shape[3] not in (1152, 2304):
+        raise ValueError(f"{name}: pool must be a contiguous uint8 tensor [pages, kv_heads, page_size/16, 18*head_dim], "
+                         f"got {tuple(pool.shape)} {pool.dtype}")
+    if pool.device != device or page_table.device != device:
+        raise ValueError(f"{name}: pool and page_table must be on {device}")
+    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous():
+        raise ValueError(f"{name}: page_table must be a contiguous int32 tensor [batch, pages per sequence]")
+    return pool.shape[1], pool.shape[3] // 18, pool.shape[2] * KV4_RECORD_TOKENS, page_table.shape[0]
+
+
+def _empty_like_layout(B, H, S, D, layout, dtype, device):
+    """A fresh contiguous tensor in ``layout`` and its [B,H,S,D] view."""
+    if layout == "HND":
+        t = torch.empty((B, H, S, D), dtype=dtype, device=device)
+        return t, t
+    t = torch.empty((B, S, H, D), dtype=dtype, device=device)
+    return t, t.transpose(1, 2)
+
+
+def _call(what, device, fn, *args):
+    """One library call with ``device`` current and its current stream as the last argument."""
+    if torch.cuda.current_device() == device.index:
+        N.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+        return
+    with torch.cuda.device(device):
+        N.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+
+
+def kv4_pool(pages: int, kv_heads: int, head_dim: int, page_size: int = 64, *, device=None) -> torch.Tensor:
+    """Zeroed pages of the 4-bit K/V cache: uint8 [pages, kv_heads,
+    page_size/16, 18*head_dim] (4.5 bits a value, see ``kv4_append``)."""
+    if head_dim not in (64, 128):
+        raise ValueError("kv4_pool: head_dim must be 64 or 128")
+    if page_size not in (16, 32, 64, 128, 256):
+        raise ValueError("kv4_pool: page_size must be 16, 32, 64, 128 or 256")
+    if pages < 1 or kv_heads < 1:
+        raise ValueError("kv4_pool: pages and kv_heads must be positive")
+    return torch.zeros((pages, kv_heads, page_size // KV4_RECORD_TOKENS, 18 * head_dim), dtype=torch.uint8,
+                       device="cuda" if device is None else device)
+
+
+def kv4_append(pool: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+               *, q: torch.Tensor | None = None, cos: torch.Tensor | None = None, sin: torch.Tensor | None = None,
+               positions: torch.Tensor | None = None, counts: torch.Tensor | None = None, interleaved: bool = False,
+               tensor_layout: str = "HND") -> torch.Tensor | None:
+    """Write new tokens to the paged 4-bit cache, rotated by their position.
+
+    ``k``/``v`` [B,Hkv,S,D] (``tensor_layout`` HND) or [B,S,Hkv,D] (NHD);
+    tokens ``t < min(S, counts[b])`` (all S without ``counts``) of sequence b
+    go to index ``lengths[b] + t`` (``lengths`` is what the cache holds before
+    the call and is not changed).  With ``cos``/``sin`` (FP32 [rows, R/2], R a
+    multiple of 16 up to D) the first R channels of ``k``, and of ``q`` when
+    given, are rotated by row ``positions[b,t]`` (default: the token's index)
+    in pairs (i, i + R/2), or (2i, 2i + 1) if ``interleaved``; ``v`` is not.
+    K and V are quantised to 4 bits with a BF16 scale and minimum per token,
+    head and 64 channels.  Returns the rotated ``q`` (a new tensor, same layout
+    and type), or None.
+
+    Page ids, indices and positions are checked on the device: a token whose
+    index has no page is not written and bit 0x80 of ``error_word`` is set.
+    """
+    name = "kv4_append"
+    dev, dt = k.device, k.dtype
+    kk, vv, qq = _serving(name, tensor_layout, dt, dev, k, v, q)
+    H, D, page, B = _cache(name, pool, page_table, dev)
+    S = kk.shape[2]
+    if kk.shape != (B, H, S, D) or vv.shape != kk.shape:
+        raise ValueError(f"{name}: k and v must be [{B},{H},S,{D}] as the cache and page table say, got "
+                         f"{tuple(kk.shape)} and {tuple(vv.shape)}")
+    Hq, out, oo = 0, None, None
+    if qq is not None:
+        Hq = qq.shape[1]
+        if qq.shape != (B, Hq, S, D) or Hq < 1 or Hq % H:
+            raise ValueError(f"{name}: q must be [{B}, a multiple of {H}, {S}, {D}], got {tuple(qq.shape)}")
+        out, oo = _empty_like_layout(B, Hq, S, D, tensor_layout, dt, dev)
+    rows = rot = 0
+    if (cos is None) != (sin is None):
+        raise ValueError(f"{name}: cos and sin come together")
+    if cos is not None:
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32 \
+                or cos.device != dev or sin.device != dev:
+            raise ValueError(f"{name}: cos and sin must be FP32 [positions, R/2] on {dev}")
+        rows, rot = cos.shape[0], 2 * cos.shape[1]
+        if rot % 16 or rot > D or rows < 1 or rot < 16:
+            raise ValueError(f"{name}: cos/sin must have at least one row and R/2 columns with R a multiple of 16, at "
+                             f"most {D}")
+        cos, sin = cos.contiguous(), sin.contiguous()
+    lengths = _ints(name, "lengths", lengths, (B,), dev)
+    positions = _ints(name, "positions", positions, (B, S), dev)
+    counts = _ints(name, "counts", counts, (B,), dev)
+    if S == 0:
+        return out
+    ks, vs = _strides(kk), _strides(vv)
+    qs, os_ = (_strides(qq), _strides(oo)) if qq is not None else (ks, ks)
+    _call(name, dev, N.load().vc_kv4_append, kk.data_ptr(), vv.data_ptr(), _p(qq), _p(oo), _DT[dt], B, Hq, H, S, D,
+          ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], qs[0], qs[1], qs[2], os_[0], os_[1], os_[2], _p(cos), _p(sin), rows,
+          rot, int(interleaved), _p(positions), lengths.data_ptr(), _p(counts), pool.data_ptr(), pool.shape[0], page,
+          page_table.data_ptr(), page_table.shape[1])
+    return out
+
+
+def kv4_read(pool: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor | None, count: int, *,
+             dtype: torch.dtype = torch.bfloat16, tensor_layout: str = "HND") -> tuple[torch.Tensor, torch.Tensor]:
+    """The values that the 4-bit cache holds for tokens ``start[b]`` (default
+    0) to ``start[b] + count - 1`` of every sequence: (K, V) in ``dtype``
+    (FP16, BF16 or FP32), [B,Hkv,count,D] or [B,count,Hkv,D] for NHD."""
+    name = "kv4_read"
+    if tensor_layout not in _LAYOUTS:
+        raise ValueError(f"{name}: tensor_layout must be HND or NHD")
+    if dtype not in _DT:
+        raise ValueError(f"{name}: dtype must be FP16, BF16 or FP32")
+    _require_cuda(name, pool, page_table, start)
+    dev = pool.device
+    H, D, page, B = _cache(name, pool, page_table, dev)
+    count = int(count)
+    if count < 0:
+        raise ValueError(f"{name}: count must not be negative")
+    start = _ints(name, "start", start, (B,), dev)
+    k, kk = _empty_like_layout(B, H, count, D, tensor_layout, dtype, dev)
+    v, vv = _empty_like_layout(B, H, count, D, tensor_layout, dtype, dev)
+    if count and B:
+        ks, vs = _strides(kk), _strides(vv)
+        _call(name, dev, N.load().vc_kv4_read, pool.data_ptr(), pool.shape[0], page, page_table.data_ptr(),
+              page_table.shape[1], _p(start), B, H, count, D, kk.data_ptr(), vv.data_ptr(), _DT[dtype], ks[0], ks[1],
+              ks[2], vs[0], vs[1], vs[2])
+    return k, v
+
+
+def _visibility(name, window, sinks, causal, sm_scale, D):
+    if window is not None and (isinstance(window, bool) or not isinstance(window, int) or window < 1):
+        raise ValueError(f"{name}: window must be None or a positive integer")
+    if isinstance(sinks, bool) or not isinstance(sinks, int) or sinks < 0:
+        raise ValueError(f"{name}: sinks must be a non-negative integer")
+    if not isinstance(causal, bool):
+        raise ValueError(f"{name}: causal must be a bool")
+    scale = D ** -0.5 if sm_scale is None else float(sm_scale)
+    if not (0 < scale <= 3.4028234663852886e38):
+        raise ValueError(f"{name}: sm_scale must be positive and finite")
+    most = 2 ** 31 - 1   # no sequence is longer
+    return min(window or 0, most), min(sinks, most), scale
+
+
+def kv4_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, *,
+                  q_lengths: torch.Tensor | None = None, causal: bool = True, window: int | None = None, sinks: int = 0,
+                  sm_scale: float | None = None, max_length: int | None = None, tensor_layout: str = "HND",
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the newest tokens of each sequence over the 4-bit cache.
+
+    ``q`` [B,Hq,Sq,D] (HND) or [B,Sq,Hq,D] (NHD), FP16 or BF16; query head h
+    reads K/V head ``h // (Hq // Hkv)``.  ``lengths`` [B]: cached tokens of each
+    sequence, of which the last ``q_lengths[b]`` (default Sq) are the queries.
+    The query at position i sees cached token j iff j < lengths[b],
+    (``causal`` implies j <= i) and (no ``window``, or j > i - window, or
+    j < ``sinks``).  Rows that see nothing, and rows past ``q_lengths[b]``, are
+    zeros.  ``max_length`` (an upper bound of ``lengths``; default the page
+    table's width) only steers how long sequences are split.  Returns a new
+    tensor like ``q``, or ``out``.
+    """
+    name = "kv4_attention"
+    dev, dt = q.device, q.dtype
+    qq, oo = _serving(name, tensor_layout, dt, dev, q, None)
+    H, D, page, B = _cache(name, pool, page_table, dev)
+    Hq, Sq = qq.shape[1], qq.shape[2]
+    if qq.shape != (B, Hq, Sq, D) or Hq < 1 or Hq % H:
+        raise ValueError(f"{name}: q must be [{B}, a multiple of {H}, Sq, {D}] as the cache and page table say, got "
+                         f"{tuple(qq.shape)}")
+    window, sinks, scale = _visibility(name, window, sinks, causal, sm_scale, D)
+    lengths = _ints(name, "lengths", lengths, (B,), dev)
+    q_lengths = _ints(name, "q_lengths", q_lengths, (B,), dev)
+    width = page_table.shape[1]
+    most = width * page if max_length is None else int(max_length)
+    if most < 0:
+        raise ValueError(f"{name}: max_length must not be negative")
+    most = min(most, width * page)
+    out, oo, copy = _output(name, out, q, tensor_layout, B, Hq, Sq, D)
+    if Sq == 0:
+        return out
+    lib = N.load()
+    wsb = lib.vc_kv4_attention_workspace_bytes(B, Hq, H, Sq, D, causal, window, sinks, page, width, most)
+    ws = _workspace(wsb, dev) if wsb else None
+    qs, os_ = _strides(qq), _strides(oo)
+    _call(name, dev, lib.vc_kv4_attention_fwd, qq.data_ptr(), _DT[dt], B, Hq, H, Sq, D, qs[0], qs[1], qs[2],
+          pool.data_ptr(), pool.shape[0], page, page_table.data_ptr(), width, lengths.data_ptr(), _p(q_lengths), causal,
+          window, sinks, most, scale, oo.data_ptr(), os_[0], os_[1], os_[2], _p(ws), wsb)
+    if copy is not None:
+        copy.copy_(oo)
+    return out
+
+
+def _output(name, out, q, layout, B, H, S, D):
+    """(out, aligned [B,H,S,D] view that the library writes, view to copy it to or None)."""
+    if out is None:
+        out, oo = _empty_like_layout(B, H, S, D, layout, q.dtype, q.device)
+        return out, oo, None
+    if out.shape != q.shape or out.dtype is not q.dtype or out.device != q.device:
+        raise ValueError(f"{name}: out must have q's shape, dtype and device")
+    view = out if layout == "HND" else out.transpose(1, 2)
+    oo = _aligned(view)
+    return out, oo, (None if oo is view else view)
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int | None = None, sinks: int = 0,
+                     causal: bool = True, kv_lengths: torch.Tensor | None = None, sm_scale: float | None = None,
+                     tensor_layout: str = "HND", out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention with a sliding window and a few first tokens that stay visible.
+
+    ``q`` [B,Hq,Sq,D], ``k``/``v`` [B,Hkv,Sk,D] (HND; NHD swaps the middle
+    axes), one FP16 or BF16 type, D 64 or 128; query head h reads K/V head
+    ``h // (Hq // Hkv)``.  Query t is at position i = Sk - Sq + t and sees key j
+    iff j < ``kv_lengths[b]`` (default Sk), (``causal`` implies j <= i) and (no
+    ``window``, or j > i - window, or j < ``sinks``).  Rows that see nothing are
+    zeros; keys and values at and past ``kv_lengths[b]`` are not used, whatever
+    they hold.  Returns a new tensor like ``q``, or ``out``.
+    """
+    name = "window_attention"
+    dev, dt = q.device, q.dtype
+    qq, kk, vv = _serving(name, tensor_layout, dt, dev, q, k, v)
+    B, Hq, Sq, D = qq.shape
+    H, Sk = kk.shape[1], kk.shape[2]
+    if D not in (64, 128):
+        raise ValueError(f"{name}: head dim must be 64 or 128, got {D}")
+    if kk.shape != (B, H, Sk, D) or vv.shape != kk.shape or B < 1 or H < 1 or Hq < 1 or Hq % H:
+        raise ValueError(f"{name}: k and v must share one shape with q's batch and head dim and a head count that divides "
+                         f"q's, got q {tuple(qq.shape)}, k {tuple(kk.shape)}, v {tuple(vv.shape)}")
+    window, sinks, scale = _visibility(name, window, sinks, causal, sm_scale, D)
+    kv_lengths = _ints(name, "kv_lengths", kv_lengths, (B,), dev)
+    out, oo, copy = _output(name, out, q, tensor_layout, B, Hq, Sq, D)
+    if Sq == 0:
+        return out
+    lib = N.load()
+    wsb = lib.vc_window_attention_workspace_bytes(B, Hq, H, Sq, Sk, D, causal, window, sinks)
+    ws = _workspace(wsb, dev) if wsb else None
+    qs, ks, vs, os_ = _strides(qq), _strides(kk), _strides(vv), _strides(oo)
+    _call(name, dev, lib.vc_window_attention_fwd, qq.data_ptr(), kk.data_ptr(), vv.data_ptr(), _DT[dt], B, Hq, H, Sq, Sk,
+          D, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], _p(kv_lengths), causal, window, sinks, scale,
+          oo.data_ptr(), os_[0], os_[1], os_[2], _p(ws), wsb)
+    if copy is not None:
+        copy.copy_(oo)
+    return out
+
+
 def attention_plan(qtiles: int, unit_range: tuple[int, int], sms: int) -> dict:
     """How ``attention_fwd`` spreads a unit range over its ExpCast kernels
     (channel-scaled V, the default kernel choice), from the library's own rule

@@ -22,6 +22,11 @@
  *   vs          fp32  [B, H, D] (channel) or [B, H, ceil(Sk/128), D] (block)
  *   means       fp16  [B, H, ceil(Sk/128), D] (V smoothing only)
  *   perm        int64 [B, H, Sk] token permutation (V grouping), or NULL
+ *   pool        uint8 [pages, Hkv, page_size/16, 18*D]: the paged 4-bit K/V
+ *               cache (vc_kv4_*)
+ *   page_table  int32 [B, table_width]: the page that holds tokens
+ *               [i*page_size, (i+1)*page_size) of a sequence; entries past a
+ *               sequence's end are never read
  */
 #ifndef VC_B200_H
 #define VC_B200_H
@@ -55,7 +60,7 @@ const char* vc_last_error(void);
  * optionally clears it.  Bits: 0x01-0x10 a bounded wait gave up (TMA, MMA,
  * softmax, correction, producer), 0x20 tensor-memory allocation, 0x40 a bad
  * kernel argument, 0x80 a permutation entry outside [0, S) (that row was read
- * as zeros), 0x100 the wait of vc_selftest_wait_timeout gave up (as intended).
+ * as zeros) or a page table entry, length or position out of range (vc_kv4_*), 0x100 the wait of vc_selftest_wait_timeout gave up (as intended).
  * Replaces: no reference counterpart (the reference spins without bound,
  * third_party/sageattention_local/csrc/vc/vc_sm90.cu:114-128). */
 int vc_error_read(int device, uint32_t* code, int clear);
@@ -198,6 +203,77 @@ int vc_attention_fwd_e4m3qk(const uint8_t* q8, const float* qs, const uint8_t* k
                             int64_t out_stride_h, int64_t out_stride_s, int expcast, int block_values,
                             int vs_per_block, int64_t k_quant_block, float sm_scale, int64_t unit_begin,
                             int64_t unit_end, void* stream);
+
+/* Paged 4-bit K/V cache.  Token j of a sequence sits in page
+ * page_table[b][j / page_size]; a page holds, for each K/V head, page_size/16
+ * records of 18*D bytes with 16 tokens each:
+ *   [0, 8D) K codes (token t at t*D/2, channel 2i in the low four bits),
+ *   [8D, 16D) V codes, [16D, 17D) K (scale, minimum) pairs of bfloat16 (token
+ *   t, 64-channel group g at (t*D/64 + g)*4), [17D, 18D) V pairs.
+ * value = scale * code + minimum.  page_size is 16, 32, 64, 128 or 256, D 64
+ * or 128.  A page table entry outside [0, pages) for a token that a call has
+ * to write or read, or a length past the table's width, sets bit 0x80 of the
+ * device error word; that token is not written, reads as zeros, and is not
+ * attended to.  No counterpart in the reference, which keeps no cache.
+ *
+ * vc_kv4_append: tokens t < min(S, counts[b]) (counts NULL: S) of sequence b
+ * go to index lengths[b] + t.  K, and Q where q is given (written to q_out for
+ * every t < S), are rotated first when rot_dim > 0: row p of cos and sin [rot_rows,
+ * rot_dim/2], p = positions[b*S + t] (NULL: lengths[b] + t; outside
+ * [0, rot_rows): bit 0x80 and row 0), pairs (i, i + rot_dim/2), or
+ * (2i, 2i + 1) when interleaved, of the first rot_dim channels (a multiple of
+ * 16, at most D):  y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin.  Each group of
+ * 64 channels is then quantised: scale = bf16((max - min)/15), minimum =
+ * bf16(min), code = clamp(rint((x - minimum) * (1/scale)), 0, 15).  A group
+ * with a NaN or an infinity reads back as NaN.  dtype F16 or BF16. */
+int vc_kv4_append(const void* k, const void* v, const void* q, void* q_out, int dtype, int64_t B, int64_t Hq,
+                  int64_t Hkv, int64_t S, int64_t D, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s,
+                  int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_s, int64_t q_stride_b, int64_t q_stride_h,
+                  int64_t q_stride_s, int64_t qo_stride_b, int64_t qo_stride_h, int64_t qo_stride_s, const float* cos,
+                  const float* sin, int64_t rot_rows, int64_t rot_dim, int interleaved, const int32_t* positions,
+                  const int32_t* lengths, const int32_t* counts, uint8_t* pool, int64_t pages, int64_t page_size,
+                  const int32_t* page_table, int64_t table_width, void* stream);
+
+/* The values of tokens start[b] .. start[b] + N - 1 (start NULL: 0) of every
+ * sequence into k and v [B,Hkv,N,D] (through strides, dtype F16, BF16 or F32). */
+int vc_kv4_read(const uint8_t* pool, int64_t pages, int64_t page_size, const int32_t* page_table, int64_t table_width,
+                const int32_t* start, int64_t B, int64_t Hkv, int64_t N, int64_t D, void* k, void* v, int dtype,
+                int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s, int64_t v_stride_b, int64_t v_stride_h,
+                int64_t v_stride_s, void* stream);
+
+/* Attention of the last tokens of each sequence over the 4-bit cache.
+ * q [B,Hq,Sq,D], out alike; query head h reads K/V head h / (Hq/Hkv).  The
+ * sequence has lengths[b] cached tokens, of which the last q_lengths[b] (NULL:
+ * Sq) are the queries: query t is at position i = lengths[b] - q_lengths[b] + t
+ * and sees key j iff j < lengths[b], (not causal or j <= i) and (window = 0 or
+ * j > i - window or j < sinks).  Rows that see nothing, and rows t >=
+ * q_lengths[b], are zeros.  max_length (at least every length; 0: the table's
+ * width) only sizes the split of long sequences and the workspace. */
+int64_t vc_kv4_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D, int causal,
+                                         int64_t window, int64_t sinks, int64_t page_size, int64_t table_width,
+                                         int64_t max_length);
+int vc_kv4_attention_fwd(const void* q, int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D,
+                         int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s, const uint8_t* pool,
+                         int64_t pages, int64_t page_size, const int32_t* page_table, int64_t table_width,
+                         const int32_t* lengths, const int32_t* q_lengths, int causal, int64_t window, int64_t sinks,
+                         int64_t max_length, float sm_scale, void* out, int64_t out_stride_b, int64_t out_stride_h,
+                         int64_t out_stride_s, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Attention over 16-bit K/V with a sliding window and sinks.  q [B,Hq,Sq,D],
+ * k and v [B,Hkv,Sk,D], dtype F16 or BF16 for all.  Query t is at position
+ * i = Sk - Sq + t; visibility as above with kv_lengths[b] (NULL: Sk; clamped to
+ * [0, Sk]) keys.  Rows that see nothing are zeros.  What lies at and past
+ * kv_lengths[b] is never used.  No counterpart in the reference, whose
+ * attention sees every key. */
+int64_t vc_window_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D,
+                                            int causal, int64_t window, int64_t sinks);
+int vc_window_attention_fwd(const void* q, const void* k, const void* v, int dtype, int64_t B, int64_t Hq,
+                            int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D, int64_t q_stride_b, int64_t q_stride_h,
+                            int64_t q_stride_s, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s,
+                            int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_s, const int32_t* kv_lengths,
+                            int causal, int64_t window, int64_t sinks, float sm_scale, void* out, int64_t out_stride_b,
+                            int64_t out_stride_h, int64_t out_stride_s, void* workspace, int64_t workspace_bytes,
+                            void* stream);
 
 /* Failure-detection self-test (no counterpart in the reference, whose
  * kernels wait without bound, csrc/vc/vc_sm90.cu:114-128): one warp waits,
