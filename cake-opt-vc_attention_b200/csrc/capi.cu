@@ -237,7 +237,7 @@ int vc_error_read(int device, uint32_t* code, int clear) {
   if (e == cudaSuccess) e = prep_hadamard_error_word(&words[3], clear != 0);
   if (e == cudaSuccess) e = tensor_peak_error_word(&words[4], clear != 0);
   if (e == cudaSuccess) e = kv4_cache_error_word(&words[6], clear != 0);
-  if (e == cudaSuccess) e = window_attention_error_word(&words[7], clear != 0);
+  if (e == cudaSuccess) e = kv4_attention_error_word(&words[7], clear != 0);
   *code = words[0] | words[1] | words[2] | words[3] | words[4] | words[5] | words[6] | words[7];
   cudaSetDevice(prev);
   if (e != cudaSuccess) {

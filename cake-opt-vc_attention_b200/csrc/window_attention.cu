@@ -1,7 +1,6 @@
 // Attention over 16-bit K/V with a sliding window and sinks: one warp a query
 // row, lanes across the channels, keys one after the other.
 #include "kernels.h"
-#include "kv4.cuh"
 #include "visible.cuh"
 
 namespace vcb {
@@ -13,8 +12,7 @@ struct RowParams {
   const void *q, *k, *v;
   void* out;
   int64_t qsb, qsh, qss, ksb, ksh, kss, vsb, vsh, vss, osb, osh, oss;
-  const int32_t *kv_lengths, *q_lengths;
-  Kv4Pages pages;
+  const int32_t* kv_lengths;
   int64_t B, Hq, Hkv, Sq, Sk;
   Visibility vis;
   float scale;
@@ -27,29 +25,16 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-template <int D, typename T, bool KV4>
+template <int D, typename T>
 __global__ void __launch_bounds__(kThreads) row_attention_kernel(RowParams p) {
   constexpr int C = D / 32;   // channels a lane
   const int64_t row = int64_t(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (row >= p.B * p.Hq * p.Sq) return;
   const int64_t t = row % p.Sq, h = row / p.Sq % p.Hq, b = row / p.Sq / p.Hq, hk = h / (p.Hq / p.Hkv);
-  int64_t len, pos;
-  bool live = true;
-  if constexpr (KV4) {
-    len = __ldg(p.kv_lengths + b);
-    const int64_t nq = p.q_lengths ? min64(__ldg(p.q_lengths + b), p.Sq) : p.Sq;
-    const int64_t most = p.pages.width * p.pages.page_size;
-    if (len < 0 || len > most) {
-      if (lane == 0) raise_error(kErrBadIndex);
-      len = len < 0 ? 0 : most;
-    }
-    pos = len - nq + t;
-    live = t < nq;
-  } else {
-    len = p.kv_lengths ? min64(__ldg(p.kv_lengths + b), p.Sk) : p.Sk;
-    pos = p.Sk - p.Sq + t;
-  }
+  int64_t len = p.Sk;
+  if (p.kv_lengths) len = max(int64_t(0), min64(__ldg(p.kv_lengths + b), p.Sk));
+  const int64_t pos = p.Sk - p.Sq + t;
   const T* q = static_cast<const T*>(p.q) + b * p.qsb + h * p.qsh + t * p.qss + lane * C;
   float qv[C], o[C];
 #pragma unroll
@@ -61,28 +46,10 @@ __global__ void __launch_bounds__(kThreads) row_attention_kernel(RowParams p) {
   const KeyRanges r = visible_keys(p.vis, pos, len);
   auto take = [&](int64_t j) {
     float kv[C], vv[C];
-    if constexpr (KV4) {
-      const int64_t rec = p.pages.record<D>(b, hk, j >> 4);
-      if (rec < 0) {
-        if (lane == 0) raise_error(kErrBadIndex);
-        return;
-      }
-      const uint8_t* rp = p.pages.pool + rec;
-      const int slot = int(j & 15), c0 = lane * C;
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const uint32_t sm = *reinterpret_cast<const uint32_t*>(rp + (w ? Kv4Rec<D>::kVp : Kv4Rec<D>::kKp) + slot * Kv4Rec<D>::kParRow + (c0 >> 6) * 4);
-        const uint8_t* code = rp + (w ? Kv4Rec<D>::kV : Kv4Rec<D>::kK) + slot * Kv4Rec<D>::kCodeRow + c0 / 2;
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-          (w ? vv : kv)[c] = __fadd_rn(__fmul_rn(float((code[c >> 1] >> (4 * (c & 1))) & 15), bf16_lo(sm)), bf16_hi(sm));
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        kv[c] = to_f32((static_cast<const T*>(p.k) + b * p.ksb + hk * p.ksh + j * p.kss)[lane * C + c]);
-        vv[c] = to_f32((static_cast<const T*>(p.v) + b * p.vsb + hk * p.vsh + j * p.vss)[lane * C + c]);
-      }
+    for (int c = 0; c < C; ++c) {
+      kv[c] = to_f32((static_cast<const T*>(p.k) + b * p.ksb + hk * p.ksh + j * p.kss)[lane * C + c]);
+      vv[c] = to_f32((static_cast<const T*>(p.v) + b * p.vsb + hk * p.vsh + j * p.vss)[lane * C + c]);
     }
     float s = 0.f;
 #pragma unroll
@@ -96,46 +63,27 @@ __global__ void __launch_bounds__(kThreads) row_attention_kernel(RowParams p) {
     for (int c = 0; c < C; ++c) o[c] = o[c] * a + e * vv[c];
     m = mn;
   };
-  if (live) {
-    for (int64_t j = 0; j < r.sink_end; ++j) take(j);
-    for (int64_t j = r.lo; j < r.hi; ++j) take(j);
-  }
+  for (int64_t j = 0; j < r.sink_end; ++j) take(j);
+  for (int64_t j = r.lo; j < r.hi; ++j) take(j);
   T* out = static_cast<T*>(p.out) + b * p.osb + h * p.osh + t * p.oss + lane * C;
 #pragma unroll
   for (int c = 0; c < C; ++c) out[c] = from_f32<T>(l == 0.f ? 0.f : o[c] / l);
 }
 
-template <bool KV4>
 int launch_rows(const RowParams& p, int dtype, int64_t D, cudaStream_t st) {
   const int64_t rows = p.B * p.Hq * p.Sq;
   const unsigned blocks = static_cast<unsigned>((rows + kThreads / 32 - 1) / (kThreads / 32));
   if (dtype == VC_DTYPE_BF16) {
-    if (D == 128) row_attention_kernel<128, __nv_bfloat16, KV4><<<blocks, kThreads, 0, st>>>(p);
-    else row_attention_kernel<64, __nv_bfloat16, KV4><<<blocks, kThreads, 0, st>>>(p);
+    if (D == 128) row_attention_kernel<128, __nv_bfloat16><<<blocks, kThreads, 0, st>>>(p);
+    else row_attention_kernel<64, __nv_bfloat16><<<blocks, kThreads, 0, st>>>(p);
   } else {
-    if (D == 128) row_attention_kernel<128, __half, KV4><<<blocks, kThreads, 0, st>>>(p);
-    else row_attention_kernel<64, __half, KV4><<<blocks, kThreads, 0, st>>>(p);
+    if (D == 128) row_attention_kernel<128, __half><<<blocks, kThreads, 0, st>>>(p);
+    else row_attention_kernel<64, __half><<<blocks, kThreads, 0, st>>>(p);
   }
   return cudaGetLastError() == cudaSuccess ? VC_OK : VC_ERR_LAUNCH;
 }
 
 }  // namespace
-
-int64_t kv4_attention_workspace(const Kv4AttnArgs&) { return 0; }
-
-int kv4_attention(const Kv4AttnArgs& a, cudaStream_t st) {
-  RowParams p{};
-  p.q = a.q;
-  p.out = a.out;
-  p.qsb = a.qsb; p.qsh = a.qsh; p.qss = a.qss; p.osb = a.osb; p.osh = a.osh; p.oss = a.oss;
-  p.kv_lengths = a.lengths;
-  p.q_lengths = a.q_lengths;
-  p.pages = kv4_pages(a.cache);
-  p.B = a.cache.B; p.Hq = a.Hq; p.Hkv = a.cache.Hkv; p.Sq = a.Sq;
-  p.vis = Visibility{a.window, a.sinks, a.causal};
-  p.scale = a.sm_scale;
-  return launch_rows<true>(p, a.dtype, a.D, st);
-}
 
 int64_t window_attention_workspace(const WindowAttnArgs&) { return 0; }
 
@@ -148,9 +96,7 @@ int window_attention(const WindowAttnArgs& a, cudaStream_t st) {
   p.B = a.B; p.Hq = a.Hq; p.Hkv = a.Hkv; p.Sq = a.Sq; p.Sk = a.Sk;
   p.vis = Visibility{a.window, a.sinks, a.causal};
   p.scale = a.sm_scale;
-  return launch_rows<false>(p, a.dtype, a.D, st);
+  return launch_rows(p, a.dtype, a.D, st);
 }
-
-cudaError_t window_attention_error_word(uint32_t* code, bool clear) { return read_tu_error_word(code, clear); }
 
 }  // namespace vcb
