@@ -229,7 +229,7 @@ int vc_error_read(int device, uint32_t* code, int clear) {
     set_last_error("vc_error_read: bad device %d", device);
     return VC_ERR_ARG;
   }
-  uint32_t words[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  uint32_t words[10] = {};
   cudaError_t e = attention_error_word(&words[0], clear != 0);
   if (e == cudaSuccess) e = read_tu_error_word(&words[5], clear != 0);   // this file: the wait self-test
   if (e == cudaSuccess) e = prep_qk_error_word(&words[1], clear != 0);
@@ -238,7 +238,9 @@ int vc_error_read(int device, uint32_t* code, int clear) {
   if (e == cudaSuccess) e = tensor_peak_error_word(&words[4], clear != 0);
   if (e == cudaSuccess) e = kv4_cache_error_word(&words[6], clear != 0);
   if (e == cudaSuccess) e = kv4_attention_error_word(&words[7], clear != 0);
-  *code = words[0] | words[1] | words[2] | words[3] | words[4] | words[5] | words[6] | words[7];
+  if (e == cudaSuccess) e = kv4_chunk_error_word(&words[8], clear != 0);
+  if (e == cudaSuccess) e = window_attention_error_word(&words[9], clear != 0);
+  *code = words[8] | words[9] | words[0] | words[1] | words[2] | words[3] | words[4] | words[5] | words[6] | words[7];
   cudaSetDevice(prev);
   if (e != cudaSuccess) {
     set_last_error("vc_error_read: %s", cudaGetErrorString(e));

@@ -158,6 +158,10 @@ struct Kv4AttnArgs {
 int64_t kv4_attention_workspace(const Kv4AttnArgs& a);
 int kv4_attention(const Kv4AttnArgs& a, cudaStream_t st);
 cudaError_t kv4_attention_error_word(uint32_t* code, bool clear);
+// Many rows a K/V head: the tile kernel (kv4_attention chooses).
+int64_t kv4_chunk_workspace(const Kv4AttnArgs& a);
+int kv4_chunk_attention(const Kv4AttnArgs& a, cudaStream_t st);
+cudaError_t kv4_chunk_error_word(uint32_t* code, bool clear);
 struct WindowAttnArgs {
   const void *q, *k, *v;
   void* out;
@@ -173,6 +177,7 @@ struct WindowAttnArgs {
 };
 int64_t window_attention_workspace(const WindowAttnArgs& a);
 int window_attention(const WindowAttnArgs& a, cudaStream_t st);
+cudaError_t window_attention_error_word(uint32_t* code, bool clear);
 
 int expcast_codes(const float* x, uint8_t* y, int64_t n, cudaStream_t st);
 

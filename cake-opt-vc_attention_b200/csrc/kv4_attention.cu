@@ -31,6 +31,7 @@
 // exceeds it by more than 8 (in powers of two): until then p <= 2^8, which
 // costs no precision, and the 32*NT accumulators are not rescaled.
 #include <type_traits>
+#include "join.cuh"
 #include "kernels.h"
 #include "kv4.cuh"
 #include "visible.cuh"
@@ -85,11 +86,6 @@ __device__ __forceinline__ uint32_t bf162_bits(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float exp2_fast(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   uint32_t r;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(a));
@@ -118,13 +114,6 @@ __device__ __forceinline__ void load8(const T* p, float* x) {
     }
   }
 }
-
-template <typename T>
-__device__ __forceinline__ T from_f32(float x);
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
 // The sequence's length and query count, clamped to the table and to Sq.
 __device__ __forceinline__ void sequence(const DecodeParams& p, int64_t b, int64_t& len, int64_t& nq) {
@@ -538,39 +527,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv4_decode_kernel(D
   }
 }
 
-// Joins the splits of a row: one warp a row, D/32 channels a lane.
-template <int D, typename T>
-__global__ void __launch_bounds__(128) kv4_join_kernel(DecodeParams p, int64_t total) {
-  const int64_t i = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (i >= total) return;
-  const float2* ml = p.part_ml + i * p.splits;
-  float top = -INFINITY;
-  for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, ml[s].x);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  constexpr int C = D / 32;
-  float v[C], sum = 0.f;
-#pragma unroll
-  for (int k = 0; k < C; ++k) v[k] = 0.f;
-  const float* src = p.part_o + i * p.splits * D + lane * C;
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 a = ml[s];
-    const float f = a.x == -INFINITY ? 0.f : exp2_fast(a.x - top);
-    sum += a.x == -INFINITY ? a.y : a.y * f;
-#pragma unroll
-    for (int k = 0; k < C; ++k) v[k] += src[s * D + k] * f;
-  }
-  const int row = static_cast<int>(i % p.rows);
-  const int64_t bh = i / p.rows, b = bh / p.pages.heads, hk = bh % p.pages.heads;
-  T h[C];
-#pragma unroll
-  for (int k = 0; k < C; ++k) h[k] = from_f32<T>(sum == 0.f ? 0.f : v[k] / sum);
-  T* dst = static_cast<T*>(p.out) + b * p.osb + (hk * p.G + row % p.G) * p.osh + int64_t(row / p.G) * p.oss + lane * C;
-  if constexpr (C == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(h);
-  else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(h);
-}
-
 struct Plan {
   int nt, blocks, splits;
 };
@@ -592,6 +548,10 @@ Plan plan_of(const Kv4AttnArgs& a) {
   return r;
 }
 
+// From this many rows a K/V head on, the tile kernel.
+constexpr int64_t kTileRows = 64;
+bool use_tiles(const Kv4AttnArgs& a) { return a.Sq * (a.Hq / a.cache.Hkv) >= kTileRows; }
+
 int launched() { return cudaGetLastError() == cudaSuccess ? VC_OK : VC_ERR_LAUNCH; }
 
 template <int D, typename T, int NT>
@@ -601,8 +561,8 @@ int launch_decode(const DecodeParams& p, const Plan& plan, int64_t BH, cudaStrea
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return VC_ERR_LAUNCH;
   k<<<dim3(plan.splits, static_cast<unsigned>(BH), plan.blocks), kThreads, bytes, st>>>(p);
   if (plan.splits > 1) {
-    const int64_t total = BH * p.rows;
-    kv4_join_kernel<D, T><<<static_cast<unsigned>((total + 3) / 4), 128, 0, st>>>(p, total);
+    const JoinParams j{p.part_o, p.part_ml, p.out, p.osb, p.osh, p.oss, p.pages.heads, p.rows, p.G, p.splits};
+    launch_join<D, T>(j, BH * p.rows, st);
   }
   return launched();
 }
@@ -617,12 +577,14 @@ int launch(const DecodeParams& p, const Plan& plan, int64_t BH, cudaStream_t st)
 }  // namespace
 
 int64_t kv4_attention_workspace(const Kv4AttnArgs& a) {
+  if (use_tiles(a)) return kv4_chunk_workspace(a);
   const Plan plan = plan_of(a);
   if (plan.splits == 1) return 0;
   return a.cache.B * a.Hq * a.Sq * plan.splits * (a.D + 2) * 4;
 }
 
 int kv4_attention(const Kv4AttnArgs& a, cudaStream_t st) {
+  if (use_tiles(a)) return kv4_chunk_attention(a, st);
   const Plan plan = plan_of(a);
   const int64_t BH = a.cache.B * a.cache.Hkv;
   DecodeParams p;

@@ -1,0 +1,736 @@
+// Exact-softmax attention on 128-row tiles (tcgen05 kind::f16), the kernel
+// behind window_attention (16-bit K/V through TMA) and behind chunks of
+// queries over the 4-bit cache (K/V dequantised to FP16 on the way).
+// Included by window_attention.cu and kv4_chunk.cu.
+//
+// Rows.  The G query heads that share a K/V head are packed with the tokens:
+// row r of a K/V head is token r / G, query head hk*G + r % G.  So K and V are
+// read once for all G heads, few tokens still fill a tile, and a tile spans
+// only 128/G positions, which keeps the partly masked part of a window small.
+// One CTA owns two 128-row tiles A and B of one (batch, K/V head), or a share
+// of their keys when there are too few CTAs (join.cuh).
+//
+// Two softmax groups of four warps, one tile each; thread t owns row t (tensor
+// memory lane t) with its maximum and sum in registers.  Per key tile of 128:
+//   QK_X(j) -> scores -> P_X(j) over the scores' own columns -> PV_X(j)
+// One warp issues all MMAs in the order PV_A(j), QK_A(j+1), PV_B(j), QK_B(j+1):
+// MMAs of one thread execute in order, so QK_X(j+1) overwrites P_X(j) only
+// after PV_X(j) has read it, and when the scores of j+1 are complete PV_X(j) is
+// too, so O may be rescaled without another wait.  While one group computes,
+// the other group's MMAs run.
+//   tensor memory: S_A/P_A [0,128)  S_B/P_B [128,256)  O_A [256,..)  O_B [384,..)
+// O is rescaled only when a row's maximum has grown by more than 8 (a factor
+// 2^8, far inside the range of FP16 and BF16 probabilities and FP32 sums).
+//
+// Key tiles.  The CTA walks the tiles that some row of it sees: those of the
+// sinks, then those of the window; a tile that a group's rows do not see at
+// all is skipped for that group, and only tiles that are partly visible are
+// masked (by selection, so hidden scores may be anything).
+//
+// K and V stages both hold [64-channel segment][key][128 bytes] with the
+// 128-byte swizzle: K is the K-major B operand of QK^T, V the MN-major B
+// operand of P.V, no transposition anywhere.
+#pragma once
+#include <cuda.h>
+#include <type_traits>
+#include "join.cuh"
+#include "kernels.h"
+#include "kv4.cuh"
+#include "visible.cuh"
+
+namespace vcb {
+namespace {
+
+#include "attention_softmax.cuh"
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazy = 8.f;
+
+struct TileParams {
+  const void* q;
+  void* out;
+  int64_t qsb, qsh, qss, osb, osh, oss;
+  int64_t Hkv, BH, Sq, Sk;     // BH = B * Hkv
+  int G, rows, pairs, splits;  // rows = Sq * G
+  Visibility vis;
+  float scale_log2;            // sm_scale * log2(e)
+  const int32_t *lengths, *q_lengths;
+  Kv4Pages pages;              // 4-bit cache only
+  // 16-bit K/V only: V rows that a tile shares with keys past the end are cleared
+  float* part_o;
+  float2* part_ml;
+};
+
+template <int D, bool KV4>
+struct TileCfg {
+  static constexpr int kThreads = KV4 ? 512 : 384;
+  static constexpr int kTile = 128 * D * 2;                  // bytes of a K, V or Q tile
+  static constexpr int kKS = KV4 ? 2 : D == 128 ? 3 : 4;     // K ring
+  static constexpr int kVS = KV4 ? 2 : D == 128 ? 2 : 4;     // V ring
+  static constexpr int kRS = KV4 ? 3 : 0;                    // ring of raw half tiles (64 keys)
+  static constexpr int kRaw = 4 * Kv4Rec<D>::kBytes;
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffK = kOffQ + 2 * kTile;
+  static constexpr int kOffV = kOffK + kKS * kTile;
+  static constexpr int kOffRaw = kOffV + kVS * kTile;
+  static constexpr int kOffCtl = kOffRaw + kRS * kRaw;
+};
+
+// What the dequantising warps found out about a key tile (4-bit cache).
+struct TileMeta {
+  int e[4], f[4];        // 2^e / 2^f: what the 32-key groups of K / V were divided by
+  uint32_t miss[4];      // keys without a page
+  uint32_t bad[2][4];    // keys whose V (64-channel group) is not finite
+};
+
+struct __align__(16) TileCtl {
+  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], q_ready[2], s_full[2], p_full[2], o_final[2], v_fix;
+  uint64_t raw_full[3], raw_empty[3], meta_full[4];
+  TileMeta meta[4];
+  uint32_t raw_miss[3];
+  uint32_t slot;
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const void* tmap, uint64_t* bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
+          "r"(smem_u32(dst)),
+      "l"(tmap), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+// MN-major operand, 128-byte swizzle: ``lbo`` bytes between 64-element blocks
+// of the MN axis, 1024 between groups of eight K rows.
+__device__ __forceinline__ uint64_t smem_desc_mn128(uint32_t saddr, uint32_t lbo) {
+  return (smem_desc_sw128(saddr) & ~(uint64_t(0x3FFFu) << 16)) | (uint64_t((lbo >> 4) & 0x3FFFu) << 16);
+}
+
+// Byte offset of 16-byte chunk ch (0-7) of row in a 128-byte-swizzled segment.
+__device__ __forceinline__ uint32_t swizzled(int row, int ch) { return row * 128 + ((ch ^ (row & 7)) << 4); }
+
+// The keys a group of rows sees, and which of the CTA's tiles that touches.
+struct GroupKeys {
+  int64_t lo, hi, sink_end;    // union over its rows
+  int64_t hi_all, lo_all;      // what every row sees: [lo_all, hi_all)
+  bool any;
+  __device__ __forceinline__ bool sees(int64_t tile) const {
+    return any && tile * 128 < hi && (tile * 128 + 128 > lo || tile * 128 < sink_end);
+  }
+};
+
+__device__ __forceinline__ GroupKeys group_keys(const Visibility& v, int64_t base, int r0, int live, int G, int64_t len) {
+  GroupKeys k{};
+  k.any = r0 < live;
+  if (!k.any) return k;
+  const int64_t first = base + r0 / G, last = base + (min(r0 + 128, live) - 1) / G;
+  const KeyRanges a = visible_keys(v, first, len), z = visible_keys(v, last, len);
+  k.hi = z.hi;
+  k.lo = a.lo;
+  k.sink_end = v.window ? min64(v.sinks, z.hi) : 0;
+  k.hi_all = a.hi;
+  k.lo_all = z.lo;
+  return k;
+}
+
+template <int D, typename T, typename QT, bool KV4>
+__global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
+    tile_attention_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, TileParams p) {
+  using C = TileCfg<D, KV4>;
+  constexpr int kSegs = D / 64;
+  constexpr int kSeg = 128 * 128;   // bytes of a 64-channel segment of a tile
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  TileCtl* ctl = reinterpret_cast<TileCtl*>(smem + C::kOffCtl);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // the pairs with the most keys come first: under causal order those are the last ones
+  const int64_t idx = blockIdx.x;
+  const int split = blockIdx.y;
+  const int pair = p.pairs - 1 - static_cast<int>(idx / p.BH);
+  const int64_t bh = idx % p.BH, b = bh / p.Hkv, hk = bh % p.Hkv;
+
+  int64_t len, nq, base;
+  if constexpr (KV4) {
+    len = __ldg(p.lengths + b);
+    const int64_t most = p.pages.width << p.pages.page_shift;
+    if (len < 0 || len > most) {
+      if (threadIdx.x == 0) raise_error(kErrBadIndex);
+      len = len < 0 ? 0 : most;
+    }
+    nq = p.q_lengths ? min64(__ldg(p.q_lengths + b), p.Sq) : p.Sq;
+    if (nq < 0) nq = 0;
+    base = len - nq;
+  } else {
+    len = p.Sk;
+    if (p.lengths) len = min64(__ldg(p.lengths + b), p.Sk);
+    if (len < 0) len = 0;
+    nq = p.Sq;
+    base = p.Sk - p.Sq;
+  }
+  const int live = static_cast<int>(nq) * p.G;
+  const GroupKeys ga = group_keys(p.vis, base, pair * 256, live, p.G, len);
+  const GroupKeys gb = group_keys(p.vis, base, pair * 256 + 128, live, p.G, len);
+  // the list of tiles: sinks [0, nsink), then [main0, main0 + ...)
+  int64_t main0 = 0, nsink = 0, total = 0;
+  if (ga.any) {
+    const int64_t hi = gb.any ? max(ga.hi, gb.hi) : ga.hi, sink_end = gb.any ? max(ga.sink_end, gb.sink_end) : ga.sink_end;
+    main0 = ga.lo >> 7;                     // A's rows come first, so its window starts first
+    if (gb.any) main0 = min(main0, gb.lo >> 7);
+    nsink = min64((sink_end + 127) >> 7, main0);
+    const int64_t end = (hi + 127) >> 7;
+    total = nsink + (end > main0 ? end - main0 : 0);
+  }
+  const int64_t i0 = total * split / p.splits;
+  const int steps = static_cast<int>(total * (split + 1) / p.splits - i0);
+  auto tile_of = [&](int n) -> int64_t {
+    const int64_t i = i0 + n;
+    return i < nsink ? i : main0 + (i - nsink);
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&ctl->k_full[s], KV4 ? 128 : 1);
+      mbar_init(&ctl->k_empty[s], 1);
+      mbar_init(&ctl->v_full[s], KV4 ? 128 : 1);
+      mbar_init(&ctl->v_empty[s], 1);
+      mbar_init(&ctl->meta_full[s], 128);
+    }
+    for (int s = 0; s < 3; ++s) {
+      mbar_init(&ctl->raw_full[s], 1);
+      mbar_init(&ctl->raw_empty[s], 4);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&ctl->q_ready[x], 128);
+      mbar_init(&ctl->s_full[x], 1);
+      mbar_init(&ctl->p_full[x], 128);
+      mbar_init(&ctl->o_final[x], 1);
+    }
+    mbar_init(&ctl->v_fix, 1);
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(&ctl->slot, 512);
+    tmem_relinquish();
+  }
+  if constexpr (!KV4) {
+    if (warp == 8 && lane == 0) tma_prefetch_desc(&tmk);
+    if (warp == 10 && lane == 0) tma_prefetch_desc(&tmv);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl->slot;
+
+  if (warp >= 8) {
+    if constexpr (KV4) setmaxnreg_dec<64>();
+    else setmaxnreg_dec<56>();
+    if (warp == 9) {
+      // ------------------------------------------------------------- MMA issuer
+      constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0 : 1;
+      constexpr uint32_t idesc_qk = idesc_make(1, fmt, fmt, 128, 128);
+      constexpr uint32_t idesc_pv = idesc_make(1, fmt, fmt, 128, D) | (1u << 16);   // B is MN-major
+      const uint64_t qd0 = smem_desc_sw128(smem_u32(smem + C::kOffQ));
+      const uint64_t kd0 = smem_desc_sw128(smem_u32(smem + C::kOffK));
+      const uint64_t vd0 = smem_desc_mn128(smem_u32(smem + C::kOffV), kSeg);
+      constexpr uint64_t kStep = C::kTile >> 4;
+      uint32_t done[2] = {0, 0};   // PVs issued, by group
+      bool ok = steps == 0 || (mbar_wait_warp(&ctl->q_ready[0], 0, kErrTimeoutMma) && mbar_wait_warp(&ctl->q_ready[1], 0, kErrTimeoutMma));
+      auto issue_qk = [&](int n, int x) {
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t kd = kd0 + (n % C::kKS) * kStep, qd = qd0 + x * kStep;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint64_t off = (kk >> 2) * (kSeg >> 4) + (kk & 3) * 2;
+            mma_f16_ss(tmem + x * 128, qd + off, kd + off, idesc_qk, kk > 0 ? 1u : 0u);
+          }
+          mma_commit(&ctl->s_full[x]);
+        }
+        __syncwarp();
+      };
+      if (ok && steps > 0) {
+        ok = mbar_wait_warp(&ctl->k_full[0], 0, kErrTimeoutMma);
+        if (ok) {
+          for (int x = 0; x < 2; ++x)
+            if ((x ? gb : ga).sees(tile_of(0))) issue_qk(0, x);
+          if (elect_one()) mma_commit(&ctl->k_empty[0]);
+          __syncwarp();
+        }
+      }
+      for (int n = 0; n < steps && ok; ++n) {
+        const int64_t tile = tile_of(n), next = tile_of(n + 1);
+        const int vs = n % C::kVS;
+        const bool more = n + 1 < steps;
+        bool have_k = false;
+        ok = mbar_wait_warp(&ctl->v_full[vs], (n / C::kVS) & 1, kErrTimeoutMma);
+        for (int x = 0; x < 2 && ok; ++x) {
+          const GroupKeys& g = x ? gb : ga;
+          if (g.sees(tile)) {
+            ok = mbar_wait_warp(&ctl->p_full[x], done[x] & 1, kErrTimeoutMma);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t vd = vd0 + vs * kStep;
+#pragma unroll
+              for (int kk = 0; kk < 8; ++kk)
+                mma_f16_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8, vd + kk * (2048 >> 4), idesc_pv, (done[x] > 0 || kk > 0) ? 1u : 0u);
+            }
+            __syncwarp();
+            ++done[x];
+          }
+          if (more && g.sees(next)) {
+            if (!have_k) {
+              ok = mbar_wait_warp(&ctl->k_full[(n + 1) % C::kKS], ((n + 1) / C::kKS) & 1, kErrTimeoutMma);
+              if (!ok) break;
+              have_k = true;
+            }
+            issue_qk(n + 1, x);
+          }
+        }
+        if (!ok) break;
+        if (elect_one()) mma_commit(&ctl->v_empty[vs]);
+        __syncwarp();
+        if (more) {
+          if (!have_k) ok = mbar_wait_warp(&ctl->k_full[(n + 1) % C::kKS], ((n + 1) / C::kKS) & 1, kErrTimeoutMma);
+          if (!ok) break;
+          if (elect_one()) mma_commit(&ctl->k_empty[(n + 1) % C::kKS]);
+          __syncwarp();
+        }
+      }
+      for (int x = 0; x < 2; ++x) {
+        if (ok && elect_one()) mma_commit(&ctl->o_final[x]);
+        __syncwarp();
+      }
+    } else if constexpr (!KV4) {
+      if (warp == 8 && lane == 0) {
+        // ----------------------------------------------------------- K producer
+        for (int n = 0; n < steps; ++n) {
+          const int s = n % C::kKS;
+          if (n >= C::kKS && !mbar_wait(&ctl->k_empty[s], ((n / C::kKS) & 1) ^ 1, kErrTimeoutProducer)) break;
+          mbar_expect_tx(&ctl->k_full[s], C::kTile);
+          for (int g = 0; g < kSegs; ++g)
+            tma_load_4d(smem + C::kOffK + s * C::kTile + g * kSeg, &tmk, &ctl->k_full[s], g * 64,
+                        static_cast<int>(tile_of(n) * 128), static_cast<int>(hk), static_cast<int>(b));
+        }
+      } else if (warp == 10) {
+        // ----------------------------------------------------------- V producer
+        uint32_t fixes = 0;
+        for (int n = 0; n < steps; ++n) {
+          const int s = n % C::kVS;
+          if (n >= C::kVS && !mbar_wait_warp(&ctl->v_empty[s], ((n / C::kVS) & 1) ^ 1, kErrTimeoutProducer)) break;
+          const int64_t k0 = tile_of(n) * 128;
+          uint8_t* dst = smem + C::kOffV + s * C::kTile;
+          // rows at and past the sequence's end hold whatever the tensor does: 0 x NaN would reach
+          // every row, so they are cleared before the MMA sees them (past Sk, TMA itself fills zeros)
+          const bool fix = k0 + 128 > len && len < p.Sk;
+          uint64_t* bar = fix ? &ctl->v_fix : &ctl->v_full[s];
+          if (lane == 0) {
+            mbar_expect_tx(bar, C::kTile);
+            for (int g = 0; g < kSegs; ++g)
+              tma_load_4d(dst + g * kSeg, &tmv, bar, g * 64, static_cast<int>(k0), static_cast<int>(hk), static_cast<int>(b));
+          }
+          __syncwarp();
+          if (fix) {
+            if (!mbar_wait_warp(&ctl->v_fix, fixes & 1, kErrTimeoutProducer)) break;
+            ++fixes;
+            const int first = len > k0 ? static_cast<int>(len - k0) : 0;
+            for (int i = lane; i < (128 - first) * 8 * kSegs; i += 32) {
+              const int g = i / ((128 - first) * 8), j = i - g * (128 - first) * 8;
+              *reinterpret_cast<uint4*>(dst + g * kSeg + first * 128 + j * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->v_full[s]);
+          }
+        }
+      }
+    } else {
+      if (warp == 8) {
+        // ------------------------------------- records of a half tile (64 keys), four lanes
+        auto locate = [&](int u) -> int64_t {   // offset, -1 past the end, -2 without a page
+          if (lane > 3 || u >= 2 * steps) return -1;
+          const int64_t blk = tile_of(u >> 1) * 8 + (u & 1) * 4 + lane;
+          if (blk * kKv4Block >= len) return -1;
+          const int64_t rec = p.pages.record<D>(b, hk, blk);
+          return rec < 0 ? -2 : rec;
+        };
+        int64_t next = locate(0);
+        for (int u = 0; u < 2 * steps; ++u) {
+          const int s = u % 3;
+          const int64_t rec = next;
+          next = locate(u + 1);
+          if (u >= 3 && !mbar_wait_warp(&ctl->raw_empty[s], ((u / 3) & 1) ^ 1, kErrTimeoutProducer)) break;
+          if (rec == -2) raise_error(kErrBadIndex);
+          const uint32_t got = __ballot_sync(0xffffffffu, rec >= 0), miss = __ballot_sync(0xffffffffu, rec == -2);
+          if (lane == 0) {
+            ctl->raw_miss[s] = (~got & 0xFu) | (miss << 8);
+            mbar_expect_tx(&ctl->raw_full[s], __popc(got) * Kv4Rec<D>::kBytes);
+          }
+          __syncwarp();
+          if (rec >= 0)
+            bulk_load(smem + C::kOffRaw + s * C::kRaw + lane * Kv4Rec<D>::kBytes, p.pages.pool + rec, Kv4Rec<D>::kBytes, &ctl->raw_full[s]);
+        }
+      } else if (warp >= 12) {
+        // ------------------------------------- dequantise to FP16 (four warps)
+        // Thread: key (u & 63) of a half tile, half of the channels.  Values are divided by a power of
+        // two per 32 keys where FP16 could not hold them (2^0 for the usual 2^-8 <= max < 2^15).
+        using R = Kv4Rec<D>;
+        const int u = threadIdx.x & 127, key = u & 63, part = u >> 6;
+        constexpr int kWords = D / 16;             // 32-bit words of codes a thread takes of K (and of V)
+        auto exponent = [](float top) -> int {
+          const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;   // top in [2^e, 2^(e+1))
+          if (top == 0.f || (e >= -8 && e <= 14)) return 0;
+          return max(e - 14, e < 0 ? max(e, -60) : -60);
+        };
+        bool ok = true;
+        for (int n = 0; n < steps && ok; ++n) {
+          const int ks = n % C::kKS, vs = n % C::kVS;
+          TileMeta* meta = &ctl->meta[n & 3];
+          if (n >= C::kKS) ok = mbar_wait_warp(&ctl->k_empty[ks], ((n / C::kKS) & 1) ^ 1, kErrTimeoutProducer);
+          if (ok && n >= C::kVS) ok = mbar_wait_warp(&ctl->v_empty[vs], ((n / C::kVS) & 1) ^ 1, kErrTimeoutProducer);
+          for (int h = 0; h < 2 && ok; ++h) {
+            const int ru = 2 * n + h, rs = ru % 3;
+            ok = mbar_wait_warp(&ctl->raw_full[rs], (ru / 3) & 1, kErrTimeoutProducer);
+            if (!ok) break;
+            const uint8_t* rec = smem + C::kOffRaw + rs * C::kRaw + (key >> 4) * R::kBytes;
+            const uint32_t state = ctl->raw_miss[rs];
+            const bool absent = (state >> (key >> 4)) & 1u, lost = (state >> (8 + (key >> 4))) & 1u;
+            const int t = key & 15;
+            const bool ended = absent || tile_of(n) * 128 + h * 64 + key >= len;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {   // K, V
+              const uint8_t* par = rec + (w ? R::kVp : R::kKp) + t * R::kParRow;
+              uint32_t sm = *reinterpret_cast<const uint32_t*>(par), sm2 = sm;
+              if constexpr (D == 128) sm2 = *reinterpret_cast<const uint32_t*>(par + 4);
+              // the key's largest magnitude; what is past the end counts for nothing
+              float top = fmaxf(fmaxf(fabsf(bf16_hi(sm)), fabsf(fmaf(15.f, bf16_lo(sm), bf16_hi(sm)))),
+                                fmaxf(fabsf(bf16_hi(sm2)), fabsf(fmaf(15.f, bf16_lo(sm2), bf16_hi(sm2)))));
+              if (ended || !(top < INFINITY)) top = 0.f;
+#pragma unroll
+              for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+              const int e = exponent(top);
+              const float down = __uint_as_float(uint32_t(127 - e) << 23);
+              const uint32_t mine = D == 128 && part ? sm2 : sm;
+              const bool fine = fabsf(bf16_lo(mine)) < INFINITY && fabsf(bf16_hi(mine)) < INFINITY;
+              // K that is not finite gives NaN scores for its key alone; V would reach rows that do not see
+              // it, so it is cleared and its key reported
+              const bool clear = ended || (w == 1 && !fine);
+              const uint32_t bad = __ballot_sync(0xffffffffu, w == 1 && !ended && !fine);
+              const uint32_t gone = __ballot_sync(0xffffffffu, lost);
+              if (lane == 0) {
+                const int g32 = h * 2 + ((warp - 12) & 1);
+                if (w == 0) {
+                  meta->e[g32] = e;
+                  meta->miss[g32] = gone;
+                } else {
+                  meta->f[g32] = e;
+                  meta->bad[D == 128 ? part : 0][g32] = bad;
+                }
+              }
+              const __half2 s2 = __float2half2_rn(bf16_lo(mine) * down), m2 = __float2half2_rn(bf16_hi(mine) * down);
+              const uint8_t* codes = rec + (w ? R::kV : R::kK) + t * R::kCodeRow + part * (kWords * 4);
+              uint8_t* dst = smem + (w ? C::kOffV + vs * C::kTile : C::kOffK + ks * C::kTile) + (D == 128 ? part * kSeg : 0);
+              const int row = h * 64 + key;
+              const __half2 minus1024 = __float2half2_rn(-1024.f), sixteenth = __float2half2_rn(0.0625f), minus64 = __float2half2_rn(-64.f);
+#pragma unroll
+              for (int i = 0; i < kWords; ++i) {
+                const uint32_t c0 = *reinterpret_cast<const uint32_t*>(codes + i * 4), c8 = c0 >> 8;
+                uint32_t x[4] = {(c0 & 0x000F000Fu) | 0x64006400u, (c0 & 0x00F000F0u) | 0x64006400u,
+                                 (c8 & 0x000F000Fu) | 0x64006400u, (c8 & 0x00F000F0u) | 0x64006400u};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  __half2 v = *reinterpret_cast<__half2*>(&x[j]);
+                  v = (j & 1) ? __hfma2(v, sixteenth, minus64) : __hadd2(v, minus1024);   // the code, exactly
+                  v = __hfma2(v, s2, m2);
+                  x[j] = clear ? 0u : *reinterpret_cast<uint32_t*>(&v);
+                }
+                // channels 8i + {0,4,1,5,2,6,3,7}: Q is stored and O written in the same order
+                *reinterpret_cast<uint4*>(dst + swizzled(row, (D == 128 ? i : part * 4 + i))) = make_uint4(x[0], x[1], x[2], x[3]);
+              }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->raw_empty[rs]);
+          }
+          if (!ok) break;
+          fence_proxy_async_smem();
+          mbar_arrive(&ctl->meta_full[n & 3]);
+          mbar_arrive(&ctl->k_full[ks]);
+          mbar_arrive(&ctl->v_full[vs]);
+        }
+      }
+    }
+  } else {
+    if constexpr (KV4) setmaxnreg_inc<192>();
+    else setmaxnreg_inc<224>();
+    // ------------------------------------------------------------ softmax group X
+    const int x = warp >> 2, t = threadIdx.x & 127;
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t scol = tmem + lane_base + x * 128, ocol = tmem + lane_base + 256 + x * 128;
+    const GroupKeys g = x ? gb : ga;
+    const int row = pair * 256 + x * 128 + t;
+    const int64_t tok = row / p.G, head = hk * p.G + row % p.G;
+    float c_row = p.scale_log2;
+    {
+      // this row of Q into shared memory, 128-byte swizzle; rows past the end are zeros
+      const QT* src = static_cast<const QT*>(p.q) + b * p.qsb + head * p.qsh + tok * p.qss;
+      uint4 u[D / 8];
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+        u[i] = row < live ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
+      if constexpr (KV4) {
+        float f[8], big = 0.f;
+        auto unpack = [&](const uint4& v) {
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same<QT, __nv_bfloat16>::value) {
+              f[2 * i] = bf16_lo(w[i]);
+              f[2 * i + 1] = bf16_hi(w[i]);
+            } else {
+              const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+              f[2 * i] = a.x;
+              f[2 * i + 1] = a.y;
+            }
+          }
+        };
+        float up = 1.f;
+        if constexpr (std::is_same<QT, __nv_bfloat16>::value) {
+          // BF16 has FP16's significant bits and more range: bring the row's largest value to [2^14, 2^15)
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            unpack(u[i]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(f[j]));
+          }
+          int e = big > 0.f ? 14 + 127 - static_cast<int>(__float_as_uint(big) >> 23) : 0;
+          e = max(-100, min(126, e));
+          up = __uint_as_float(uint32_t(127 + e) << 23);
+          c_row *= __uint_as_float(uint32_t(127 - e) << 23);
+        }
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          unpack(u[i]);
+          u[i] = make_uint4(pack2<__half>(f[0] * up, f[4] * up), pack2<__half>(f[1] * up, f[5] * up),
+                            pack2<__half>(f[2] * up, f[6] * up), pack2<__half>(f[3] * up, f[7] * up));
+        }
+      }
+      uint8_t* dst = smem + C::kOffQ + x * C::kTile;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4*>(dst + (i >> 3) * kSeg + swizzled(t, i & 7)) = u[i];
+      fence_proxy_async_smem();
+      mbar_arrive(&ctl->q_ready[x]);
+    }
+    const KeyRanges mine = visible_keys(p.vis, base + tok, len);
+    float m = -INFINITY, l = 0.f;
+    int frun = 0;              // 4-bit cache: O is in units of 2^frun
+    uint32_t nan_out = 0;      // 4-bit cache: 64-channel groups of this row that saw a value that is not finite
+    uint32_t done = 0;
+    bool ok = true;
+    for (int n = 0; n < steps; ++n) {
+      const int64_t tile = tile_of(n), k0 = tile * 128;
+      if (!g.sees(tile)) continue;
+      float cg[4] = {c_row, c_row, c_row, c_row};
+      int fg[4] = {0, 0, 0, 0};
+      bool odd = false;          // keys without a page, or values that are not finite
+      const TileMeta* meta = &ctl->meta[n & 3];
+      if constexpr (KV4) {
+        ok = mbar_wait_warp(&ctl->meta_full[n & 3], (n >> 2) & 1, kErrTimeoutSoftmax);
+        if (!ok) break;
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          cg[i] = c_row * __uint_as_float(uint32_t(127 + meta->e[i]) << 23);
+          fg[i] = meta->f[i];
+          any |= meta->miss[i] | meta->bad[0][i] | (D == 128 ? meta->bad[1][i] : 0u);
+        }
+        odd = any != 0;
+      }
+      ok = mbar_wait_warp(&ctl->s_full[x], done & 1, kErrTimeoutSoftmax);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t raw[128];
+      tmem_ld32(scol + 0, *reinterpret_cast<uint32_t(*)[32]>(raw + 0));
+      tmem_ld32(scol + 32, *reinterpret_cast<uint32_t(*)[32]>(raw + 32));
+      tmem_ld32(scol + 64, *reinterpret_cast<uint32_t(*)[32]>(raw + 64));
+      tmem_ld32(scol + 96, *reinterpret_cast<uint32_t(*)[32]>(raw + 96));
+      tmem_wait_ld();
+      const bool whole = k0 + 128 <= g.hi_all && (p.vis.window == 0 || k0 >= g.lo_all || k0 + 128 <= p.vis.sinks);
+      if (!whole) {
+        const int hi = static_cast<int>(max(int64_t(0), min64(128, mine.hi - k0)));
+        const int lo = static_cast<int>(max(int64_t(0), min64(128, mine.lo - k0)));
+        const int sk = static_cast<int>(max(int64_t(0), min64(128, mine.sink_end - k0)));
+#pragma unroll
+        for (int c = 0; c < 128; ++c)
+          if (c >= hi || (c < lo && c >= sk)) raw[c] = 0xFF800000u;
+      }
+      if constexpr (KV4) {
+        if (odd) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c) {
+            const uint32_t bit = 1u << (c & 31);
+            if (meta->miss[c >> 5] & bit) raw[c] = 0xFF800000u;
+            if (raw[c] != 0xFF800000u) {
+              if (meta->bad[0][c >> 5] & bit) nan_out |= 1u;
+              if (D == 128 && (meta->bad[1][c >> 5] & bit)) nan_out |= 2u;
+            }
+          }
+        }
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        float a = max3f(__uint_as_float(raw[32 * q4]), __uint_as_float(raw[32 * q4 + 1]), __uint_as_float(raw[32 * q4 + 2]));
+        float b2 = max3f(__uint_as_float(raw[32 * q4 + 3]), __uint_as_float(raw[32 * q4 + 4]), __uint_as_float(raw[32 * q4 + 5]));
+#pragma unroll
+        for (int c = 6; c < 30; c += 4) {
+          a = max3f(a, __uint_as_float(raw[32 * q4 + c]), __uint_as_float(raw[32 * q4 + c + 1]));
+          b2 = max3f(b2, __uint_as_float(raw[32 * q4 + c + 2]), __uint_as_float(raw[32 * q4 + c + 3]));
+        }
+        a = max3f(a, __uint_as_float(raw[32 * q4 + 30]), __uint_as_float(raw[32 * q4 + 31]));
+        top = fmaxf(top, fmaxf(a, b2) * cg[q4]);
+      }
+      int fnew = frun;
+      if constexpr (KV4) {
+        fnew = max(max(fg[0], fg[1]), max(fg[2], fg[3]));
+        if (done > 0) fnew = max(fnew, frun);
+      }
+      const bool grow = top > m + kLazy;
+      if (__any_sync(0xffffffffu, grow) || fnew != frun) {
+        const float mn = grow ? top : m;
+        const float alpha = grow ? exp2_fast(m - mn) : 1.f;
+        m = mn;
+        l *= alpha;
+        if (done > 0) {
+          const float by = KV4 ? alpha * __uint_as_float(uint32_t(127 + max(-126, frun - fnew)) << 23) : alpha;
+          const uint64_t by2 = pk2f(by, by);
+#pragma unroll
+          for (int cc = 0; cc < D / 32; ++cc) {
+            uint32_t o[32];
+            tmem_ld32(ocol + cc * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) up2(f2_mul(pk2(o[2 * i], o[2 * i + 1]), by2), o[2 * i], o[2 * i + 1]);
+            tmem_st32(ocol + cc * 32, o);
+          }
+        }
+        frun = fnew;
+      }
+      const float mneg = m == -INFINITY ? 0.f : -m;
+      uint32_t pw[64];
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const float shift = KV4 ? static_cast<float>(max(-126, fg[q4] - frun)) : 0.f;
+        const uint64_t c2 = pk2f(cg[q4], cg[q4]), n2 = pk2f(mneg + shift, mneg + shift);
+        uint64_t sum2 = pk2f(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          uint32_t a, d;
+          up2(f2_fma(pk2(raw[32 * q4 + 2 * i], raw[32 * q4 + 2 * i + 1]), c2, n2), a, d);
+          const float ea = exp2_fast(__uint_as_float(a)), ed = exp2_fast(__uint_as_float(d));
+          sum2 = f2_add(sum2, pk2f(ea, ed));
+          pw[16 * q4 + i] = pack2<T>(ea, ed);
+        }
+        uint32_t a, d;
+        up2(sum2, a, d);
+        const float s = __uint_as_float(a) + __uint_as_float(d);
+        l += KV4 ? s * exp2_fast(-shift) : s;
+      }
+      tmem_st32(scol, *reinterpret_cast<uint32_t(*)[32]>(pw));
+      tmem_st32(scol + 32, *reinterpret_cast<uint32_t(*)[32]>(pw + 32));
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&ctl->p_full[x]);
+      ++done;
+    }
+    // ------------------------------------------------------------------ epilogue
+    if (ok && done > 0) ok = mbar_wait_warp(&ctl->o_final[x], 0, kErrTimeoutSoftmax);
+    if (ok) {
+      tc_fence_after();
+      const bool seen = row < live && done > 0 && !(l == 0.f);
+      const float unit = KV4 ? __uint_as_float(uint32_t(127 + max(-126, frun)) << 23) : 1.f;
+      const float inv = seen ? (p.splits == 1 ? unit / l : unit) : 0.f;
+      const int64_t at = (bh * p.rows + row) * p.splits + split;
+      QT* orow = static_cast<QT*>(p.out) + b * p.osb + head * p.osh + tok * p.oss;
+#pragma unroll
+      for (int cc = 0; cc < D / 32; ++cc) {
+        uint32_t o[32];
+        tmem_ld32(ocol + cc * 32, o);
+        tmem_wait_ld();
+        if (row < p.rows) {
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            // 4-bit cache: column 8a + {0..7} holds channel 8a + {0,4,1,5,2,6,3,7}
+            const int from = KV4 ? (i & ~7) + ((i & 3) * 2 + ((i >> 2) & 1)) : i;
+            v[i] = seen ? __uint_as_float(o[from]) * inv : 0.f;
+            if (KV4 && seen && ((nan_out >> (cc >> 1)) & 1u)) v[i] = NAN;
+          }
+          if (p.splits == 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              reinterpret_cast<uint4*>(orow + cc * 32)[i] =
+                  make_uint4(pack2<QT>(v[8 * i], v[8 * i + 1]), pack2<QT>(v[8 * i + 2], v[8 * i + 3]),
+                             pack2<QT>(v[8 * i + 4], v[8 * i + 5]), pack2<QT>(v[8 * i + 6], v[8 * i + 7]));
+          } else {
+            float4* dst = reinterpret_cast<float4*>(p.part_o + at * D + cc * 32);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          }
+        }
+      }
+      if (p.splits > 1 && row < p.rows) p.part_ml[at] = seen ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Pairs of 128-row tiles, and splits of their keys where the pairs alone would
+// leave SMs idle.  ``keys``: the most keys that one row's CTA can see.
+struct TilePlan {
+  int64_t pairs = 0, splits = 1;
+};
+inline TilePlan tile_plan(int64_t BH, int64_t rows, int64_t G, int64_t keys, const Visibility& v) {
+  TilePlan r;
+  r.pairs = (rows + 255) / 256;
+  if (v.window > 0) keys = min64(keys, v.window + (255 + G) / G + v.sinks + 256);
+  const int64_t tiles = (keys + 127) / 128, items = BH * r.pairs;
+  int64_t s = 148 / items;
+  s = min64(s, tiles / 4);
+  r.splits = s < 1 ? 1 : s;
+  return r;
+}
+
+template <int D, typename T, typename QT, bool KV4>
+int launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, const TileParams& p, cudaStream_t st) {
+  auto* k = tile_attention_kernel<D, T, QT, KV4>;
+  using C = TileCfg<D, KV4>;
+  constexpr int bytes = C::kOffCtl + int(sizeof(TileCtl)) + 1024;
+  static_assert(bytes <= 227 * 1024, "shared memory");
+  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return VC_ERR_LAUNCH;
+  k<<<dim3(static_cast<unsigned>(p.BH * p.pairs), static_cast<unsigned>(p.splits)), C::kThreads, bytes, st>>>(mk, mv, p);
+  if (p.splits > 1) {
+    const JoinParams j{p.part_o, p.part_ml, p.out, p.osb, p.osh, p.oss, p.Hkv, p.rows, p.G, p.splits};
+    launch_join<D, QT>(j, p.BH * p.rows, st);
+  }
+  return cudaGetLastError() == cudaSuccess ? VC_OK : VC_ERR_LAUNCH;
+}
+
+}  // namespace
+}  // namespace vcb
