@@ -109,6 +109,16 @@ int check_serving(const char* fn, int dtype, int64_t B, int64_t Hq, int64_t Hkv,
   return VC_OK;
 }
 
+// Rows of a K/V head (tokens x shared query heads) are numbered in 32 bits.
+int check_rows(const char* fn, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq) {
+  const int64_t rows = Sq * (Hq / Hkv);
+  if (rows > (int64_t(1) << 31) - 65536 || (rows + 31) / 32 * B * Hkv > (int64_t(1) << 31) - 1) {
+    set_last_error("%s: too many query rows (Sq*Hq/Hkv must stay below 2^31 - 65536, B*Hq*Sq below 2^36)", fn);
+    return VC_ERR_ARG;
+  }
+  return VC_OK;
+}
+
 int check_tokens(const char* fn, const char* name, int64_t n) {
   if (n < 0 || n > (int64_t(1) << 31) - 65536) {
     set_last_error("%s: %s must be in [0, 2^31 - 65536] (got %lld)", fn, name, (long long)n);
@@ -594,6 +604,7 @@ int vc_kv4_attention_fwd(const void* q, int dtype, int64_t B, int64_t Hq, int64_
   const char* fn = "vc_kv4_attention_fwd";
   if (int rc = check_serving(fn, dtype, B, Hq, Hkv, D)) return rc;
   if (int rc = check_tokens(fn, "Sq", Sq)) return rc;
+  if (int rc = check_rows(fn, B, Hq, Hkv, Sq)) return rc;
   if (int rc = check_tokens(fn, "max_length", max_length)) return rc;
   if (int rc = check_cache(fn, pool, pages, page_size, page_table, table_width)) return rc;
   if (int rc = check_visibility(fn, window, sinks, sm_scale)) return rc;
@@ -638,6 +649,7 @@ int vc_window_attention_fwd(const void* q, const void* k, const void* v, int dty
   const char* fn = "vc_window_attention_fwd";
   if (int rc = check_serving(fn, dtype, B, Hq, Hkv, D)) return rc;
   if (int rc = check_tokens(fn, "Sq", Sq)) return rc;
+  if (int rc = check_rows(fn, B, Hq, Hkv, Sq)) return rc;
   if (int rc = check_tokens(fn, "Sk", Sk)) return rc;
   if (int rc = check_visibility(fn, window, sinks, sm_scale)) return rc;
   if (Sq == 0) return VC_OK;

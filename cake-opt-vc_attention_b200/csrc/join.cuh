@@ -6,9 +6,22 @@
 // its sum l_s.  The row is sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s with
 // m = max m_s, summed in the order of s.
 #pragma once
+#include <atomic>
 #include "common.cuh"
 
 namespace vcb {
+
+// Allows ``bytes`` of dynamic shared memory for a kernel, once a device (the
+// attribute call costs about as much as a launch).  ``ready``: devices done.
+inline bool allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& ready) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return false;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (bit && (ready.load(std::memory_order_relaxed) & bit)) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  ready.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
 
 struct JoinParams {
   const float* part_o;    // [rows of all heads, splits, D]

@@ -558,7 +558,8 @@ template <int D, typename T, int NT>
 int launch_decode(const DecodeParams& p, const Plan& plan, int64_t BH, cudaStream_t st) {
   auto* k = kv4_decode_kernel<D, T, NT>;
   constexpr int bytes = DecodeSmem<D, NT>::kBytes;
-  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return VC_ERR_LAUNCH;
+  static std::atomic<uint64_t> ready{0};
+  if (!allow_smem(reinterpret_cast<const void*>(k), bytes, ready)) return VC_ERR_LAUNCH;
   k<<<dim3(plan.splits, static_cast<unsigned>(BH), plan.blocks), kThreads, bytes, st>>>(p);
   if (plan.splits > 1) {
     const JoinParams j{p.part_o, p.part_ml, p.out, p.osb, p.osh, p.oss, p.pages.heads, p.rows, p.G, p.splits};

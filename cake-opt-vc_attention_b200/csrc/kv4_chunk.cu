@@ -26,8 +26,8 @@ int kv4_chunk_attention(const Kv4AttnArgs& a, cudaStream_t st) {
   p.out = a.out;
   p.qsb = a.qsb; p.qsh = a.qsh; p.qss = a.qss;
   p.osb = a.osb; p.osh = a.osh; p.oss = a.oss;
-  p.Hkv = a.cache.Hkv;
-  p.BH = a.cache.B * a.cache.Hkv;
+  p.Hkv = static_cast<int>(a.cache.Hkv);
+  p.BH = static_cast<int>(a.cache.B * a.cache.Hkv);
   p.Sq = a.Sq;
   p.G = static_cast<int>(a.Hq / a.cache.Hkv);
   p.rows = static_cast<int>(a.Sq * p.G);
@@ -39,7 +39,7 @@ int kv4_chunk_attention(const Kv4AttnArgs& a, cudaStream_t st) {
   p.q_lengths = a.q_lengths;
   p.pages = kv4_pages(a.cache);
   p.part_o = static_cast<float*>(a.workspace);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + p.BH * p.rows * t.splits * a.D);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + int64_t(p.BH) * p.rows * t.splits * a.D);
   const CUtensorMap none{};   // K/V come from the cache's records
   if (a.dtype == VC_DTYPE_BF16)
     return a.D == 128 ? launch_tiles<128, __half, __nv_bfloat16, true>(none, none, p, st)

@@ -50,7 +50,8 @@ struct TileParams {
   const void* q;
   void* out;
   int64_t qsb, qsh, qss, osb, osh, oss;
-  int64_t Hkv, BH, Sq, Sk;     // BH = B * Hkv
+  int64_t Sq, Sk;
+  int Hkv, BH;                 // BH = B * Hkv
   int G, rows, pairs, splits;  // rows = Sq * G
   Visibility vis;
   float scale_log2;            // sm_scale * log2(e)
@@ -88,6 +89,7 @@ struct __align__(16) TileCtl {
   uint64_t raw_full[3], raw_empty[3], meta_full[4];
   TileMeta meta[4];
   uint32_t raw_miss[3];
+  float q_unit[2][128];   // 4-bit cache, BF16 queries: what a row of Q was divided by
   uint32_t slot;
 };
 
@@ -121,13 +123,19 @@ __device__ __forceinline__ uint32_t swizzled(int row, int ch) { return row * 128
 
 // The keys a group of rows sees, and which of the CTA's tiles that touches.
 struct GroupKeys {
-  int64_t lo, hi, sink_end;    // union over its rows
-  int64_t hi_all, lo_all;      // what every row sees: [lo_all, hi_all)
+  int lo, hi, sink_end;    // union over its rows (keys fit 32 bits: at most 2^31 - 65536 tokens)
+  int hi_all, lo_all;      // what every row sees: [lo_all, hi_all)
   bool any;
-  __device__ __forceinline__ bool sees(int64_t tile) const {
+  __device__ __forceinline__ bool sees(int tile) const {
     return any && tile * 128 < hi && (tile * 128 + 128 > lo || tile * 128 < sink_end);
   }
 };
+
+// Which of keys k .. k + 31 lie in [lo, hi) or [0, sink).
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
+__device__ __forceinline__ uint32_t visible_bits(int lo, int hi, int sink, int k) {
+  return (bits_below(hi - k) & ~bits_below(lo - k)) | bits_below(sink - k);
+}
 
 __device__ __forceinline__ GroupKeys group_keys(const Visibility& v, int64_t base, int r0, int live, int G, int64_t len) {
   GroupKeys k{};
@@ -135,11 +143,11 @@ __device__ __forceinline__ GroupKeys group_keys(const Visibility& v, int64_t bas
   if (!k.any) return k;
   const int64_t first = base + r0 / G, last = base + (min(r0 + 128, live) - 1) / G;
   const KeyRanges a = visible_keys(v, first, len), z = visible_keys(v, last, len);
-  k.hi = z.hi;
-  k.lo = a.lo;
-  k.sink_end = v.window ? min64(v.sinks, z.hi) : 0;
-  k.hi_all = a.hi;
-  k.lo_all = z.lo;
+  k.hi = static_cast<int>(z.hi);
+  k.lo = static_cast<int>(a.lo);
+  k.sink_end = v.window ? static_cast<int>(min64(v.sinks, z.hi)) : 0;
+  k.hi_all = static_cast<int>(a.hi);
+  k.lo_all = static_cast<int>(z.lo);
   return k;
 }
 
@@ -155,10 +163,9 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   // the pairs with the most keys come first: under causal order those are the last ones
-  const int64_t idx = blockIdx.x;
   const int split = blockIdx.y;
-  const int pair = p.pairs - 1 - static_cast<int>(idx / p.BH);
-  const int64_t bh = idx % p.BH, b = bh / p.Hkv, hk = bh % p.Hkv;
+  const int pair = p.pairs - 1 - static_cast<int>(blockIdx.x) / p.BH;
+  const int bh = static_cast<int>(blockIdx.x) % p.BH, b = bh / p.Hkv, hk = bh - b * p.Hkv;
 
   int64_t len, nq, base;
   if constexpr (KV4) {
@@ -182,27 +189,28 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
   const GroupKeys ga = group_keys(p.vis, base, pair * 256, live, p.G, len);
   const GroupKeys gb = group_keys(p.vis, base, pair * 256 + 128, live, p.G, len);
   // the list of tiles: sinks [0, nsink), then [main0, main0 + ...)
-  int64_t main0 = 0, nsink = 0, total = 0;
+  int main0 = 0, nsink = 0, total = 0;
   if (ga.any) {
-    const int64_t hi = gb.any ? max(ga.hi, gb.hi) : ga.hi, sink_end = gb.any ? max(ga.sink_end, gb.sink_end) : ga.sink_end;
+    const int hi = gb.any ? max(ga.hi, gb.hi) : ga.hi, sink_end = gb.any ? max(ga.sink_end, gb.sink_end) : ga.sink_end;
     main0 = ga.lo >> 7;                     // A's rows come first, so its window starts first
     if (gb.any) main0 = min(main0, gb.lo >> 7);
-    nsink = min64((sink_end + 127) >> 7, main0);
-    const int64_t end = (hi + 127) >> 7;
+    nsink = min((sink_end + 127) >> 7, main0);
+    const int end = (hi + 127) >> 7;
     total = nsink + (end > main0 ? end - main0 : 0);
   }
-  const int64_t i0 = total * split / p.splits;
-  const int steps = static_cast<int>(total * (split + 1) / p.splits - i0);
-  auto tile_of = [&](int n) -> int64_t {
-    const int64_t i = i0 + n;
+  // (at most 2^24 tiles times 148 splits: 32 unsigned bits)
+  const int i0 = p.splits == 1 ? 0 : static_cast<int>(unsigned(total) * unsigned(split) / unsigned(p.splits));
+  const int steps = (p.splits == 1 ? total : static_cast<int>(unsigned(total) * unsigned(split + 1) / unsigned(p.splits))) - i0;
+  auto tile_of = [&](int n) -> int {
+    const int i = i0 + n;
     return i < nsink ? i : main0 + (i - nsink);
   };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < 4; ++s) {
-      mbar_init(&ctl->k_full[s], KV4 ? 128 : 1);
+      mbar_init(&ctl->k_full[s], KV4 ? 64 : 1);
       mbar_init(&ctl->k_empty[s], 1);
-      mbar_init(&ctl->v_full[s], KV4 ? 128 : 1);
+      mbar_init(&ctl->v_full[s], KV4 ? 64 : 1);
       mbar_init(&ctl->v_empty[s], 1);
       mbar_init(&ctl->meta_full[s], 128);
     }
@@ -233,7 +241,7 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
   const uint32_t tmem = ctl->slot;
 
   if (warp >= 8) {
-    if constexpr (KV4) setmaxnreg_dec<64>();
+    if constexpr (KV4) setmaxnreg_dec<80>();
     else setmaxnreg_dec<56>();
     if (warp == 9) {
       // ------------------------------------------------------------- MMA issuer
@@ -245,6 +253,9 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
       const uint64_t vd0 = smem_desc_mn128(smem_u32(smem + C::kOffV), kSeg);
       constexpr uint64_t kStep = C::kTile >> 4;
       uint32_t done[2] = {0, 0};   // PVs issued, by group
+      int last[2] = {steps - 1, steps - 1};   // the last tile a group sees
+      for (int x = 0; x < 2; ++x)
+        while (last[x] >= 0 && !(x ? gb : ga).sees(tile_of(last[x]))) --last[x];
       bool ok = steps == 0 || (mbar_wait_warp(&ctl->q_ready[0], 0, kErrTimeoutMma) && mbar_wait_warp(&ctl->q_ready[1], 0, kErrTimeoutMma));
       auto issue_qk = [&](int n, int x) {
         tc_fence_after();
@@ -269,7 +280,7 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
         }
       }
       for (int n = 0; n < steps && ok; ++n) {
-        const int64_t tile = tile_of(n), next = tile_of(n + 1);
+        const int tile = tile_of(n), next = tile_of(n + 1);
         const int vs = n % C::kVS;
         const bool more = n + 1 < steps;
         bool have_k = false;
@@ -286,6 +297,7 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
               for (int kk = 0; kk < 8; ++kk)
                 mma_f16_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8, vd + kk * (2048 >> 4), idesc_pv, (done[x] > 0 || kk > 0) ? 1u : 0u);
             }
+            if (n == last[x] && elect_one()) mma_commit(&ctl->o_final[x]);
             __syncwarp();
             ++done[x];
           }
@@ -308,10 +320,6 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
           __syncwarp();
         }
       }
-      for (int x = 0; x < 2; ++x) {
-        if (ok && elect_one()) mma_commit(&ctl->o_final[x]);
-        __syncwarp();
-      }
     } else if constexpr (!KV4) {
       if (warp == 8 && lane == 0) {
         // ----------------------------------------------------------- K producer
@@ -321,7 +329,7 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
           mbar_expect_tx(&ctl->k_full[s], C::kTile);
           for (int g = 0; g < kSegs; ++g)
             tma_load_4d(smem + C::kOffK + s * C::kTile + g * kSeg, &tmk, &ctl->k_full[s], g * 64,
-                        static_cast<int>(tile_of(n) * 128), static_cast<int>(hk), static_cast<int>(b));
+                        tile_of(n) * 128, static_cast<int>(hk), static_cast<int>(b));
         }
       } else if (warp == 10) {
         // ----------------------------------------------------------- V producer
@@ -329,7 +337,7 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
         for (int n = 0; n < steps; ++n) {
           const int s = n % C::kVS;
           if (n >= C::kVS && !mbar_wait_warp(&ctl->v_empty[s], ((n / C::kVS) & 1) ^ 1, kErrTimeoutProducer)) break;
-          const int64_t k0 = tile_of(n) * 128;
+          const int k0 = tile_of(n) * 128;
           uint8_t* dst = smem + C::kOffV + s * C::kTile;
           // rows at and past the sequence's end hold whatever the tensor does: 0 x NaN would reach
           // every row, so they are cleared before the MMA sees them (past Sk, TMA itself fills zeros)
@@ -338,7 +346,7 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
           if (lane == 0) {
             mbar_expect_tx(bar, C::kTile);
             for (int g = 0; g < kSegs; ++g)
-              tma_load_4d(dst + g * kSeg, &tmv, bar, g * 64, static_cast<int>(k0), static_cast<int>(hk), static_cast<int>(b));
+              tma_load_4d(dst + g * kSeg, &tmv, bar, g * 64, k0, static_cast<int>(hk), static_cast<int>(b));
           }
           __syncwarp();
           if (fix) {
@@ -360,8 +368,8 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
         // ------------------------------------- records of a half tile (64 keys), four lanes
         auto locate = [&](int u) -> int64_t {   // offset, -1 past the end, -2 without a page
           if (lane > 3 || u >= 2 * steps) return -1;
-          const int64_t blk = tile_of(u >> 1) * 8 + (u & 1) * 4 + lane;
-          if (blk * kKv4Block >= len) return -1;
+          const int blk = tile_of(u >> 1) * 8 + (u & 1) * 4 + lane;
+          if (int64_t(blk) * kKv4Block >= len) return -1;
           const int64_t rec = p.pages.record<D>(b, hk, blk);
           return rec < 0 ? -2 : rec;
         };
@@ -383,69 +391,82 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
         }
       } else if (warp >= 12) {
         // ------------------------------------- dequantise to FP16 (four warps)
-        // Thread: key (u & 63) of a half tile, half of the channels.  Values are divided by a power of
-        // two per 32 keys where FP16 could not hold them (2^0 for the usual 2^-8 <= max < 2^15).
+        // Warps 12 and 13 take K, 14 and 15 V; each 32 of the 64 keys of a raw half tile, 16 bytes of codes
+        // (32 channels) a lane, D/32 lanes a key, so that reads are contiguous and the swizzled 16-byte
+        // writes of eight lanes hit all banks.  Values are divided by a power of two per 32 keys where FP16
+        // could not hold them (2^0 for the usual 2^-8 <= max < 2^15).
         using R = Kv4Rec<D>;
-        const int u = threadIdx.x & 127, key = u & 63, part = u >> 6;
-        constexpr int kWords = D / 16;             // 32-bit words of codes a thread takes of K (and of V)
-        auto exponent = [](float top) -> int {
-          const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;   // top in [2^e, 2^(e+1))
-          if (top == 0.f || (e >= -8 && e <= 14)) return 0;
-          return max(e - 14, e < 0 ? max(e, -60) : -60);
-        };
+        constexpr int kPer = D / 32, kKeys = 32 / kPer;   // lanes a key, keys a pass
+        const bool is_v = warp >= 14;
+        const int w32 = (warp & 1) * 32;                  // first key in the half tile
+        const int q = lane % kPer, part = q >> 1;         // 32 channels; their 64-channel group (D = 128)
+        const __half2 minus1024 = __float2half2_rn(-1024.f), sixteenth = __float2half2_rn(0.0625f), minus64 = __float2half2_rn(-64.f);
+        uint64_t* empty = is_v ? ctl->v_empty : ctl->k_empty;
+        uint64_t* full = is_v ? ctl->v_full : ctl->k_full;
+        const int depth = is_v ? C::kVS : C::kKS;
         bool ok = true;
         for (int n = 0; n < steps && ok; ++n) {
-          const int ks = n % C::kKS, vs = n % C::kVS;
+          const int st = n % depth;
           TileMeta* meta = &ctl->meta[n & 3];
-          if (n >= C::kKS) ok = mbar_wait_warp(&ctl->k_empty[ks], ((n / C::kKS) & 1) ^ 1, kErrTimeoutProducer);
-          if (ok && n >= C::kVS) ok = mbar_wait_warp(&ctl->v_empty[vs], ((n / C::kVS) & 1) ^ 1, kErrTimeoutProducer);
+          if (n >= depth) ok = mbar_wait_warp(&empty[st], ((n / depth) & 1) ^ 1, kErrTimeoutProducer);
           for (int h = 0; h < 2 && ok; ++h) {
             const int ru = 2 * n + h, rs = ru % 3;
             ok = mbar_wait_warp(&ctl->raw_full[rs], (ru / 3) & 1, kErrTimeoutProducer);
             if (!ok) break;
-            const uint8_t* rec = smem + C::kOffRaw + rs * C::kRaw + (key >> 4) * R::kBytes;
+            const uint8_t* raw = smem + C::kOffRaw + rs * C::kRaw;
             const uint32_t state = ctl->raw_miss[rs];
-            const bool absent = (state >> (key >> 4)) & 1u, lost = (state >> (8 + (key >> 4))) & 1u;
-            const int t = key & 15;
-            const bool ended = absent || tile_of(n) * 128 + h * 64 + key >= len;
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {   // K, V
-              const uint8_t* par = rec + (w ? R::kVp : R::kKp) + t * R::kParRow;
-              uint32_t sm = *reinterpret_cast<const uint32_t*>(par), sm2 = sm;
-              if constexpr (D == 128) sm2 = *reinterpret_cast<const uint32_t*>(par + 4);
-              // the key's largest magnitude; what is past the end counts for nothing
-              float top = fmaxf(fmaxf(fabsf(bf16_hi(sm)), fabsf(fmaf(15.f, bf16_lo(sm), bf16_hi(sm)))),
-                                fmaxf(fabsf(bf16_hi(sm2)), fabsf(fmaf(15.f, bf16_lo(sm2), bf16_hi(sm2)))));
-              if (ended || !(top < INFINITY)) top = 0.f;
-#pragma unroll
-              for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-              const int e = exponent(top);
-              const float down = __uint_as_float(uint32_t(127 - e) << 23);
-              const uint32_t mine = D == 128 && part ? sm2 : sm;
-              const bool fine = fabsf(bf16_lo(mine)) < INFINITY && fabsf(bf16_hi(mine)) < INFINITY;
-              // K that is not finite gives NaN scores for its key alone; V would reach rows that do not see
-              // it, so it is cleared and its key reported
-              const bool clear = ended || (w == 1 && !fine);
-              const uint32_t bad = __ballot_sync(0xffffffffu, w == 1 && !ended && !fine);
-              const uint32_t gone = __ballot_sync(0xffffffffu, lost);
-              if (lane == 0) {
-                const int g32 = h * 2 + ((warp - 12) & 1);
-                if (w == 0) {
-                  meta->e[g32] = e;
-                  meta->miss[g32] = gone;
-                } else {
-                  meta->f[g32] = e;
-                  meta->bad[D == 128 ? part : 0][g32] = bad;
-                }
+            // lane = key: the largest magnitude of the 32 keys, and which keys are missing or not finite
+            const int key = w32 + lane;
+            const uint8_t* par = raw + (key >> 4) * R::kBytes + (is_v ? R::kVp : R::kKp) + (key & 15) * R::kParRow;
+            const uint32_t sm = *reinterpret_cast<const uint32_t*>(par);
+            uint32_t sm2 = sm;
+            if constexpr (D == 128) sm2 = *reinterpret_cast<const uint32_t*>(par + 4);
+            const bool lost = (state >> (8 + (key >> 4))) & 1u;
+            const bool ended = ((state >> (key >> 4)) & 1u) || tile_of(n) * 128 + h * 64 + key >= len;
+            const bool fine = fabsf(bf16_lo(sm)) < INFINITY && fabsf(bf16_hi(sm)) < INFINITY;
+            const bool fine2 = fabsf(bf16_lo(sm2)) < INFINITY && fabsf(bf16_hi(sm2)) < INFINITY;
+            float top = fmaxf(fmaxf(fabsf(bf16_hi(sm)), fabsf(fmaf(15.f, bf16_lo(sm), bf16_hi(sm)))),
+                              fmaxf(fabsf(bf16_hi(sm2)), fabsf(fmaf(15.f, bf16_lo(sm2), bf16_hi(sm2)))));
+            if (ended || !(top < INFINITY)) top = 0.f;
+            // (the exponent's bits order like the values)
+            const uint32_t top_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+            const int te = static_cast<int>(top_bits >> 23) - 127;   // the maximum lies in [2^te, 2^(te+1))
+            const int e = top_bits == 0u || (te >= -8 && te <= 14) ? 0 : te > 14 ? te - 14 : max(te, -60);
+            const float down = __uint_as_float(uint32_t(127 - e) << 23);
+            // K that is not finite gives NaN scores for its key alone; V would reach rows that do not see it
+            // (0 * NaN), so it is cleared and its key reported.  Keys past the end are cleared.
+            const uint32_t gone = __ballot_sync(0xffffffffu, ended);
+            const uint32_t bad = __ballot_sync(0xffffffffu, !ended && !fine), bad2 = __ballot_sync(0xffffffffu, !ended && !fine2);
+            const uint32_t clear0 = gone | (is_v ? bad : 0u), clear1 = gone | (is_v ? bad2 : 0u);
+            const uint32_t missing = __ballot_sync(0xffffffffu, lost);
+            if (lane == 0) {
+              const int g32 = h * 2 + (warp & 1);
+              if (is_v) {
+                meta->f[g32] = e;
+                meta->bad[0][g32] = bad;
+                meta->bad[1][g32] = bad2;
+              } else {
+                meta->e[g32] = e;
+                meta->miss[g32] = missing;
               }
-              const __half2 s2 = __float2half2_rn(bf16_lo(mine) * down), m2 = __float2half2_rn(bf16_hi(mine) * down);
-              const uint8_t* codes = rec + (w ? R::kV : R::kK) + t * R::kCodeRow + part * (kWords * 4);
-              uint8_t* dst = smem + (w ? C::kOffV + vs * C::kTile : C::kOffK + ks * C::kTile) + (D == 128 ? part * kSeg : 0);
-              const int row = h * 64 + key;
-              const __half2 minus1024 = __float2half2_rn(-1024.f), sixteenth = __float2half2_rn(0.0625f), minus64 = __float2half2_rn(-64.f);
+            }
+            const uint32_t clear = D == 128 && part ? clear1 : clear0;
+            uint8_t* dst = smem + (is_v ? C::kOffV : C::kOffK) + st * C::kTile + (D == 128 ? part * kSeg : 0);
+#pragma unroll 2
+            for (int pass = 0; pass < kPer; ++pass) {
+              const int k32 = pass * kKeys + lane / kPer, kk = w32 + k32;
+              const uint8_t* rec = raw + (kk >> 4) * R::kBytes;
+              const uint4 codes = *reinterpret_cast<const uint4*>(rec + (is_v ? R::kV : R::kK) + (kk & 15) * R::kCodeRow + q * 16);
+              const uint32_t ms = *reinterpret_cast<const uint32_t*>(rec + (is_v ? R::kVp : R::kKp) + (kk & 15) * R::kParRow + (D == 128 ? part * 4 : 0));
+              const __half2 s2 = __float2half2_rn(bf16_lo(ms) * down), m2 = __float2half2_rn(bf16_hi(ms) * down);
+              const bool zero = (clear >> k32) & 1u;
+              // the second group's lanes take their words in the order 2, 3, 0, 1: see the banks above
+              const bool swap = D == 128 && part;
+              const uint32_t cw[4] = {swap ? codes.z : codes.x, swap ? codes.w : codes.y, swap ? codes.x : codes.z, swap ? codes.y : codes.w};
+              const int row = h * 64 + kk;
 #pragma unroll
-              for (int i = 0; i < kWords; ++i) {
-                const uint32_t c0 = *reinterpret_cast<const uint32_t*>(codes + i * 4), c8 = c0 >> 8;
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t c0 = cw[i], c8 = c0 >> 8;
                 uint32_t x[4] = {(c0 & 0x000F000Fu) | 0x64006400u, (c0 & 0x00F000F0u) | 0x64006400u,
                                  (c8 & 0x000F000Fu) | 0x64006400u, (c8 & 0x00F000F0u) | 0x64006400u};
 #pragma unroll
@@ -453,10 +474,11 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
                   __half2 v = *reinterpret_cast<__half2*>(&x[j]);
                   v = (j & 1) ? __hfma2(v, sixteenth, minus64) : __hadd2(v, minus1024);   // the code, exactly
                   v = __hfma2(v, s2, m2);
-                  x[j] = clear ? 0u : *reinterpret_cast<uint32_t*>(&v);
+                  x[j] = zero ? 0u : *reinterpret_cast<uint32_t*>(&v);
                 }
-                // channels 8i + {0,4,1,5,2,6,3,7}: Q is stored and O written in the same order
-                *reinterpret_cast<uint4*>(dst + swizzled(row, (D == 128 ? i : part * 4 + i))) = make_uint4(x[0], x[1], x[2], x[3]);
+                // channels 8a + {0,4,1,5,2,6,3,7}: Q is stored and O written in the same order
+                const int a = (q & 1) * 4 + (swap ? i ^ 2 : i);
+                *reinterpret_cast<uint4*>(dst + swizzled(row, a)) = make_uint4(x[0], x[1], x[2], x[3]);
               }
             }
             __syncwarp();
@@ -465,96 +487,97 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
           if (!ok) break;
           fence_proxy_async_smem();
           mbar_arrive(&ctl->meta_full[n & 3]);
-          mbar_arrive(&ctl->k_full[ks]);
-          mbar_arrive(&ctl->v_full[vs]);
+          mbar_arrive(&full[st]);
         }
       }
     }
   } else {
-    if constexpr (KV4) setmaxnreg_inc<192>();
+    if constexpr (KV4) setmaxnreg_inc<176>();
     else setmaxnreg_inc<224>();
     // ------------------------------------------------------------ softmax group X
     const int x = warp >> 2, t = threadIdx.x & 127;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t scol = tmem + lane_base + x * 128, ocol = tmem + lane_base + 256 + x * 128;
     const GroupKeys g = x ? gb : ga;
-    const int row = pair * 256 + x * 128 + t;
-    const int64_t tok = row / p.G, head = hk * p.G + row % p.G;
+    const int row0 = pair * 256 + x * 128 + (warp & 3) * 32;   // this warp's first row
+    const int row = row0 + lane;
+    const int tok = row / p.G;
     float c_row = p.scale_log2;
+    // Q and the output move between global memory and the tile of shared memory a warp's 32 rows at a
+    // time, D/8 lanes a row (16 bytes each), so that rows are read and written whole
+    constexpr int kRowLanes = D / 8, kRowsAt = 32 / kRowLanes;
+    const int rl = lane / kRowLanes, ch = lane % kRowLanes;
+    uint8_t* tile_mem = smem + C::kOffQ + x * C::kTile;
     {
-      // this row of Q into shared memory, 128-byte swizzle; rows past the end are zeros
-      const QT* src = static_cast<const QT*>(p.q) + b * p.qsb + head * p.qsh + tok * p.qss;
-      uint4 u[D / 8];
+#pragma unroll 4
+      for (int i = 0; i < 32 / kRowsAt; ++i) {
+        const int lr = i * kRowsAt + rl, r = row0 + lr, rt = r / p.G, rh = hk * p.G + (r - rt * p.G);
+        const QT* src = static_cast<const QT*>(p.q) + b * p.qsb + rh * p.qsh + rt * p.qss + ch * 8;
+        uint4 u = r < live ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
+        if constexpr (KV4) {
+          float f[8];
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i)
-        u[i] = row < live ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
-      if constexpr (KV4) {
-        float f[8], big = 0.f;
-        auto unpack = [&](const uint4& v) {
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int j = 0; j < 4; ++j) {
             if constexpr (std::is_same<QT, __nv_bfloat16>::value) {
-              f[2 * i] = bf16_lo(w[i]);
-              f[2 * i + 1] = bf16_hi(w[i]);
+              f[2 * j] = bf16_lo(w[j]);
+              f[2 * j + 1] = bf16_hi(w[j]);
             } else {
-              const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-              f[2 * i] = a.x;
-              f[2 * i + 1] = a.y;
+              const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+              f[2 * j] = a.x;
+              f[2 * j + 1] = a.y;
             }
           }
-        };
-        float up = 1.f;
-        if constexpr (std::is_same<QT, __nv_bfloat16>::value) {
-          // BF16 has FP16's significant bits and more range: bring the row's largest value to [2^14, 2^15)
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
-            unpack(u[i]);
+          float up = 1.f;
+          if constexpr (std::is_same<QT, __nv_bfloat16>::value) {
+            // BF16 has FP16's significant bits and more range: bring the row's largest value to [2^14, 2^15)
+            float big = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(f[j]));
+#pragma unroll
+            for (int o = 1; o < kRowLanes; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+            int e = big > 0.f ? 14 + 127 - static_cast<int>(__float_as_uint(big) >> 23) : 0;
+            e = max(-100, min(126, e));
+            up = __uint_as_float(uint32_t(127 + e) << 23);
+            if (ch == 0) ctl->q_unit[x][(warp & 3) * 32 + lr] = __uint_as_float(uint32_t(127 - e) << 23);
           }
-          int e = big > 0.f ? 14 + 127 - static_cast<int>(__float_as_uint(big) >> 23) : 0;
-          e = max(-100, min(126, e));
-          up = __uint_as_float(uint32_t(127 + e) << 23);
-          c_row *= __uint_as_float(uint32_t(127 - e) << 23);
+          u = make_uint4(pack2<__half>(f[0] * up, f[4] * up), pack2<__half>(f[1] * up, f[5] * up),
+                         pack2<__half>(f[2] * up, f[6] * up), pack2<__half>(f[3] * up, f[7] * up));
         }
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          unpack(u[i]);
-          u[i] = make_uint4(pack2<__half>(f[0] * up, f[4] * up), pack2<__half>(f[1] * up, f[5] * up),
-                            pack2<__half>(f[2] * up, f[6] * up), pack2<__half>(f[3] * up, f[7] * up));
-        }
+        *reinterpret_cast<uint4*>(tile_mem + (ch >> 3) * kSeg + swizzled((warp & 3) * 32 + lr, ch & 7)) = u;
       }
-      uint8_t* dst = smem + C::kOffQ + x * C::kTile;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4*>(dst + (i >> 3) * kSeg + swizzled(t, i & 7)) = u[i];
+      if constexpr (KV4 && std::is_same<QT, __nv_bfloat16>::value) {
+        __syncwarp();
+        c_row *= ctl->q_unit[x][t];
+      }
       fence_proxy_async_smem();
       mbar_arrive(&ctl->q_ready[x]);
     }
-    const KeyRanges mine = visible_keys(p.vis, base + tok, len);
+    const KeyRanges seen_keys = visible_keys(p.vis, base + tok, len);
+    const int my_hi = static_cast<int>(seen_keys.hi), my_lo = static_cast<int>(seen_keys.lo), my_sink = static_cast<int>(seen_keys.sink_end);
     float m = -INFINITY, l = 0.f;
     int frun = 0;              // 4-bit cache: O is in units of 2^frun
     uint32_t nan_out = 0;      // 4-bit cache: 64-channel groups of this row that saw a value that is not finite
     uint32_t done = 0;
     bool ok = true;
     for (int n = 0; n < steps; ++n) {
-      const int64_t tile = tile_of(n), k0 = tile * 128;
+      const int tile = tile_of(n), k0 = tile * 128;
       if (!g.sees(tile)) continue;
       float cg[4] = {c_row, c_row, c_row, c_row};
       int fg[4] = {0, 0, 0, 0};
-      bool odd = false;          // keys without a page, or values that are not finite
-      const TileMeta* meta = &ctl->meta[n & 3];
+      uint32_t miss[4] = {0, 0, 0, 0}, bad[2][4] = {};   // 4-bit cache: see TileMeta
       if constexpr (KV4) {
+        const TileMeta* meta = &ctl->meta[n & 3];
         ok = mbar_wait_warp(&ctl->meta_full[n & 3], (n >> 2) & 1, kErrTimeoutSoftmax);
         if (!ok) break;
-        uint32_t any = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           cg[i] = c_row * __uint_as_float(uint32_t(127 + meta->e[i]) << 23);
           fg[i] = meta->f[i];
-          any |= meta->miss[i] | meta->bad[0][i] | (D == 128 ? meta->bad[1][i] : 0u);
+          miss[i] = meta->miss[i];
+          bad[0][i] = meta->bad[0][i];
+          bad[1][i] = meta->bad[1][i];
         }
-        odd = any != 0;
       }
       ok = mbar_wait_warp(&ctl->s_full[x], done & 1, kErrTimeoutSoftmax);
       if (!ok) break;
@@ -565,26 +588,24 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
       tmem_ld32(scol + 64, *reinterpret_cast<uint32_t(*)[32]>(raw + 64));
       tmem_ld32(scol + 96, *reinterpret_cast<uint32_t(*)[32]>(raw + 96));
       tmem_wait_ld();
-      const bool whole = k0 + 128 <= g.hi_all && (p.vis.window == 0 || k0 >= g.lo_all || k0 + 128 <= p.vis.sinks);
-      if (!whole) {
-        const int hi = static_cast<int>(max(int64_t(0), min64(128, mine.hi - k0)));
-        const int lo = static_cast<int>(max(int64_t(0), min64(128, mine.lo - k0)));
-        const int sk = static_cast<int>(max(int64_t(0), min64(128, mine.sink_end - k0)));
-#pragma unroll
-        for (int c = 0; c < 128; ++c)
-          if (c >= hi || (c < lo && c >= sk)) raw[c] = 0xFF800000u;
-      }
+      bool whole = k0 + 128 <= g.hi_all && (p.vis.window == 0 || k0 >= g.lo_all || k0 + 128 <= p.vis.sinks);
+      if constexpr (KV4) whole = whole && (miss[0] | miss[1] | miss[2] | miss[3]) == 0;
       if constexpr (KV4) {
-        if (odd) {
+        if (bad[0][0] | bad[0][1] | bad[0][2] | bad[0][3] | bad[1][0] | bad[1][1] | bad[1][2] | bad[1][3]) {
 #pragma unroll
-          for (int c = 0; c < 128; ++c) {
-            const uint32_t bit = 1u << (c & 31);
-            if (meta->miss[c >> 5] & bit) raw[c] = 0xFF800000u;
-            if (raw[c] != 0xFF800000u) {
-              if (meta->bad[0][c >> 5] & bit) nan_out |= 1u;
-              if (D == 128 && (meta->bad[1][c >> 5] & bit)) nan_out |= 2u;
-            }
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t v = visible_bits(my_lo, my_hi, my_sink, k0 + 32 * i) & ~miss[i];
+            nan_out |= ((bad[0][i] & v) ? 1u : 0u) | ((bad[1][i] & v) ? 2u : 0u);
           }
+        }
+      }
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t v = visible_bits(my_lo, my_hi, my_sink, k0 + 32 * i) & ~miss[i];
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (!((v >> c) & 1u)) raw[32 * i + c] = 0xFF800000u;
         }
       }
       float top = -INFINITY;
@@ -614,7 +635,7 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
         if (done > 0) {
           const float by = KV4 ? alpha * __uint_as_float(uint32_t(127 + max(-126, frun - fnew)) << 23) : alpha;
           const uint64_t by2 = pk2f(by, by);
-#pragma unroll
+#pragma unroll 1
           for (int cc = 0; cc < D / 32; ++cc) {
             uint32_t o[32];
             tmem_ld32(ocol + cc * 32, o);
@@ -660,33 +681,40 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
       const bool seen = row < live && done > 0 && !(l == 0.f);
       const float unit = KV4 ? __uint_as_float(uint32_t(127 + max(-126, frun)) << 23) : 1.f;
       const float inv = seen ? (p.splits == 1 ? unit / l : unit) : 0.f;
-      const int64_t at = (bh * p.rows + row) * p.splits + split;
-      QT* orow = static_cast<QT*>(p.out) + b * p.osb + head * p.osh + tok * p.oss;
-#pragma unroll
+      const int64_t at = (int64_t(bh) * p.rows + row) * p.splits + split;
+#pragma unroll 1
       for (int cc = 0; cc < D / 32; ++cc) {
         uint32_t o[32];
         tmem_ld32(ocol + cc * 32, o);
         tmem_wait_ld();
-        if (row < p.rows) {
-          float v[32];
+        float v[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            // 4-bit cache: column 8a + {0..7} holds channel 8a + {0,4,1,5,2,6,3,7}
-            const int from = KV4 ? (i & ~7) + ((i & 3) * 2 + ((i >> 2) & 1)) : i;
-            v[i] = seen ? __uint_as_float(o[from]) * inv : 0.f;
-            if (KV4 && seen && ((nan_out >> (cc >> 1)) & 1u)) v[i] = NAN;
-          }
-          if (p.splits == 1) {
+        for (int i = 0; i < 32; ++i) {
+          // 4-bit cache: column 8a + {0..7} holds channel 8a + {0,4,1,5,2,6,3,7}
+          const int from = KV4 ? (i & ~7) + ((i & 3) * 2 + ((i >> 2) & 1)) : i;
+          v[i] = seen ? __uint_as_float(o[from]) * inv : 0.f;
+          if (KV4 && seen && ((nan_out >> (cc >> 1)) & 1u)) v[i] = NAN;
+        }
+        if (p.splits == 1) {
+          // all MMAs are done: the Q tile's memory stages the output
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              reinterpret_cast<uint4*>(orow + cc * 32)[i] =
-                  make_uint4(pack2<QT>(v[8 * i], v[8 * i + 1]), pack2<QT>(v[8 * i + 2], v[8 * i + 3]),
-                             pack2<QT>(v[8 * i + 4], v[8 * i + 5]), pack2<QT>(v[8 * i + 6], v[8 * i + 7]));
-          } else {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + at * D + cc * 32);
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(tile_mem + (cc >> 1) * kSeg + swizzled(t, (cc & 1) * 4 + i)) =
+                make_uint4(pack2<QT>(v[8 * i], v[8 * i + 1]), pack2<QT>(v[8 * i + 2], v[8 * i + 3]),
+                           pack2<QT>(v[8 * i + 4], v[8 * i + 5]), pack2<QT>(v[8 * i + 6], v[8 * i + 7]));
+        } else if (row < p.rows) {
+          float4* dst = reinterpret_cast<float4*>(p.part_o + at * D + cc * 32);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-          }
+          for (int i = 0; i < 8; ++i) dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        }
+      }
+      if (p.splits == 1) {
+        __syncwarp();
+#pragma unroll 2
+        for (int i = 0; i < 32 / kRowsAt; ++i) {
+          const int lr = i * kRowsAt + rl, r = row0 + lr, rt = r / p.G, rh = hk * p.G + (r - rt * p.G);
+          const uint4 u = *reinterpret_cast<const uint4*>(tile_mem + (ch >> 3) * kSeg + swizzled((warp & 3) * 32 + lr, ch & 7));
+          if (r < p.rows) *reinterpret_cast<uint4*>(static_cast<QT*>(p.out) + b * p.osb + rh * p.osh + rt * p.oss + ch * 8) = u;
         }
       }
       if (p.splits > 1 && row < p.rows) p.part_ml[at] = seen ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
@@ -723,11 +751,12 @@ int launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, const TileParams&
   using C = TileCfg<D, KV4>;
   constexpr int bytes = C::kOffCtl + int(sizeof(TileCtl)) + 1024;
   static_assert(bytes <= 227 * 1024, "shared memory");
-  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return VC_ERR_LAUNCH;
-  k<<<dim3(static_cast<unsigned>(p.BH * p.pairs), static_cast<unsigned>(p.splits)), C::kThreads, bytes, st>>>(mk, mv, p);
+  static std::atomic<uint64_t> ready{0};
+  if (!allow_smem(reinterpret_cast<const void*>(k), bytes, ready)) return VC_ERR_LAUNCH;
+  k<<<dim3(static_cast<unsigned>(p.BH) * static_cast<unsigned>(p.pairs), static_cast<unsigned>(p.splits)), C::kThreads, bytes, st>>>(mk, mv, p);
   if (p.splits > 1) {
     const JoinParams j{p.part_o, p.part_ml, p.out, p.osb, p.osh, p.oss, p.Hkv, p.rows, p.G, p.splits};
-    launch_join<D, QT>(j, p.BH * p.rows, st);
+    launch_join<D, QT>(j, int64_t(p.BH) * p.rows, st);
   }
   return cudaGetLastError() == cudaSuccess ? VC_OK : VC_ERR_LAUNCH;
 }

@@ -62,8 +62,8 @@ int window_attention(const WindowAttnArgs& a, cudaStream_t st) {
   p.out = a.out;
   p.qsb = a.qsb; p.qsh = a.qsh; p.qss = a.qss;
   p.osb = a.osb; p.osh = a.osh; p.oss = a.oss;
-  p.Hkv = a.Hkv;
-  p.BH = a.B * a.Hkv;
+  p.Hkv = static_cast<int>(a.Hkv);
+  p.BH = static_cast<int>(a.B * a.Hkv);
   p.Sq = a.Sq;
   p.Sk = a.Sk;
   p.G = static_cast<int>(a.Hq / a.Hkv);
@@ -74,7 +74,7 @@ int window_attention(const WindowAttnArgs& a, cudaStream_t st) {
   p.scale_log2 = a.sm_scale * kLog2e;
   p.lengths = a.kv_lengths;
   p.part_o = static_cast<float*>(a.workspace);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + p.BH * p.rows * t.splits * a.D);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + int64_t(p.BH) * p.rows * t.splits * a.D);
   if (a.dtype == VC_DTYPE_BF16)
     return a.D == 128 ? launch_tiles<128, __nv_bfloat16, __nv_bfloat16, false>(mk, mv, p, st)
                       : launch_tiles<64, __nv_bfloat16, __nv_bfloat16, false>(mk, mv, p, st);

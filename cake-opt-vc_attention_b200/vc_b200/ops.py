@@ -268,93 +268,105 @@ def attention_fwd(q8, qs, k8, ks, v8, vs, means, *, out_dtype=torch.bfloat16, sm
 
 # ---------------------------------------------------------------------------
 # Paged 4-bit K/V cache and window attention (inference only).
+#
+# A decoding step makes several of these calls, and for one sequence their GPU
+# time is a few microseconds each: the wrappers therefore read each tensor's
+# shape and strides once and make no views (NHD is a matter of the order in
+# which the axes are read).
 # ---------------------------------------------------------------------------
 KV4_RECORD_TOKENS = 16
-_LAYOUTS = ("HND", "NHD")
+_F16, _BF16, _I32, _U8, _F32 = torch.float16, torch.bfloat16, torch.int32, torch.uint8, torch.float32
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # current_stream(i).cuda_stream without the object
 
 
-def _aligned(x: torch.Tensor) -> torch.Tensor:
-    """``_rowmajor`` for any strides: an axis of one element may have any
-    stride, a broadcast token axis is copied."""
-    es = x.element_size()
-    st = x.stride()
-    if st[3] == 1 and x.data_ptr() % 16 == 0 and (st[2] > 0 or x.shape[2] < 2) and \
-            all(n < 2 or (s * es) % 16 == 0 for s, n in zip(st[:3], x.shape[:3])):
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
+def _bhsd(name, what, t, layout, dtype, device):
+    """(tensor, address, B, H, S, D, stride_b, stride_h, stride_s) of a 16-bit
+    tensor in ``layout``, copied first if its strides or address are not what
+    the library takes (unit channel stride, 16-byte multiples).  Axes of one
+    element address nothing; their stride is given as one row."""
+    if t.dtype is not dtype or t.device != device:
+        raise ValueError(f"{name}: {what} must be {dtype} on {device} as the first tensor is, got {t.dtype} on {t.device}")
+    if t.dim() != 4:
+        raise ValueError(f"{name}: {what} must be four-dimensional, got shape {tuple(t.shape)}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} has no backward pass; detach its inputs or call it under torch.no_grad()")
+    if layout == "HND":
+        B, H, S, D = t.shape
+        sb, sh, ss, sd = t.stride()
+    else:
+        B, S, H, D = t.shape
+        sb, ss, sh, sd = t.stride()
+    if B < 2:
+        sb = D
+    if H < 2:
+        sh = D
+    if S < 2:
+        ss = D
+    ptr = t.data_ptr()
+    if (sb | sh | ss) & 7 or ptr & 15 or (sd != 1 and D > 1) or ss <= 0:
+        t = t.clone(memory_format=torch.contiguous_format)
+        ptr = t.data_ptr()
+        sb, sh, ss = (H * S * D, S * D, D) if layout == "HND" else (H * S * D, D, H * D)
+    return t, ptr, B, H, S, D, sb, sh, ss
 
 
-def _strides(x: torch.Tensor) -> tuple:
-    """(b, h, s) strides in elements; those of one-element axes, which address nothing, as one row."""
-    d = x.shape[3]
-    st = x.stride()
-    return tuple(s if n > 1 else d for s, n in zip(st[:3], x.shape[:3]))
-
-
-def _serving(name, layout, dtype, device, *tensors):
-    """Layout, type and device checks shared by the cache and window ops; the
-    tensors (None allowed) as aligned [B,H,S,D] views."""
-    if layout not in _LAYOUTS:
+def _serving(name, layout, t):
+    if layout != "HND" and layout != "NHD":
         raise ValueError(f"{name}: tensor_layout must be HND or NHD")
-    out = []
-    grad = torch.is_grad_enabled()
-    for t in tensors:
-        if t is None:
-            out.append(None)
-            continue
-        if t.dtype is not dtype or t.device != device:
-            raise ValueError(f"{name}: tensors must share one dtype and device, got {t.dtype} on {t.device} "
-                             f"and {dtype} on {device}")
-        if t.dim() != 4:
-            raise ValueError(f"{name}: expected four-dimensional tensors, got shape {tuple(t.shape)}")
-        if grad and t.requires_grad:
-            raise ValueError(f"{name} has no backward pass; detach its inputs or call it under torch.no_grad()")
-        out.append(_aligned(t if layout == "HND" else t.transpose(1, 2)))
-    if device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name}: tensors must be on a CUDA device (no CPU fallback)")
-    if dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"{name}: FP16 or BF16 tensors required, got {dtype}")
-    return out
+    if t.dtype is not _BF16 and t.dtype is not _F16:
+        raise ValueError(f"{name}: FP16 or BF16 tensors required, got {t.dtype}")
 
 
 def _ints(name, what, t, shape, device):
     """An int32 contiguous device tensor of ``shape`` (None passes through)."""
     if t is None:
         return None
-    if tuple(t.shape) != shape or t.dtype not in (torch.int32, torch.int64) or t.device != device:
-        raise ValueError(f"{name}: {what} must be an integer tensor of shape {shape} on {device}, got "
+    if t.shape != shape or (t.dtype is not _I32 and t.dtype is not torch.int64) or t.device != device:
+        raise ValueError(f"{name}: {what} must be an integer tensor of shape {tuple(shape)} on {device}, got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
-    return (t if t.dtype is torch.int32 else t.to(torch.int32)).contiguous()
+    return (t if t.dtype is _I32 else t.to(_I32)).contiguous()
 
 
 def _cache(name, pool, page_table, device):
-    """(kv heads, head dim, page size, batch) of a pool and its page table."""
-    if pool.dtype is not torch.uint8 or pool.dim() != 4 or not pool.is_contiguous() or pool.shape[3] not in (1152, 2304):
+    """(kv heads, head dim, page size, batch, table width, pages) of a pool and its page table."""
+    if pool.dtype is not _U8 or pool.dim() != 4 or not pool.is_contiguous() or pool.shape[3] not in (1152, 2304):
         raise ValueError(f"{name}: pool must be a contiguous uint8 tensor [pages, kv_heads, page_size/16, 18*head_dim], "
                          f"got {tuple(pool.shape)} {pool.dtype}")
     if pool.device != device or page_table.device != device:
         raise ValueError(f"{name}: pool and page_table must be on {device}")
-    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous():
+    if page_table.dtype is not _I32 or page_table.dim() != 2 or not page_table.is_contiguous():
         raise ValueError(f"{name}: page_table must be a contiguous int32 tensor [batch, pages per sequence]")
-    return pool.shape[1], pool.shape[3] // 18, pool.shape[2] * KV4_RECORD_TOKENS, page_table.shape[0]
+    pages, heads, records, size = pool.shape
+    B, width = page_table.shape
+    return heads, size // 18, records * KV4_RECORD_TOKENS, B, width, pages
 
 
-def _empty_like_layout(B, H, S, D, layout, dtype, device):
-    """A fresh contiguous tensor in ``layout`` and its [B,H,S,D] view."""
-    if layout == "HND":
-        t = torch.empty((B, H, S, D), dtype=dtype, device=device)
-        return t, t
-    t = torch.empty((B, S, H, D), dtype=dtype, device=device)
-    return t, t.transpose(1, 2)
+def _output(name, out, q, view, layout):
+    """(out, address, stride_b, stride_h, stride_s, tensor to copy into out or
+    None) for a result like ``q``, whose ``_bhsd`` is ``view``."""
+    _, _, B, H, S, D, sb, sh, ss = view
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        if layout == "HND":
+            return out, out.data_ptr(), H * S * D, S * D, D, None
+        return out, out.data_ptr(), H * S * D, D, H * D, None
+    if out.shape != q.shape:
+        raise ValueError(f"{name}: out must have q's shape {tuple(q.shape)}, got {tuple(out.shape)}")
+    t, ptr, _, _, _, _, sb, sh, ss = _bhsd(name, "out", out, layout, q.dtype, q.device)
+    return out, ptr, sb, sh, ss, None if t is out else t
 
 
 def _call(what, device, fn, *args):
     """One library call with ``device`` current and its current stream as the last argument."""
-    if torch.cuda.current_device() == device.index:
-        N.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
-        return
-    with torch.cuda.device(device):
-        N.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+    i = device.index
+    if torch.cuda.current_device() != i:
+        with torch.cuda.device(device):
+            return _call(what, device, fn, *args)
+    rc = fn(*args, _raw_stream(i) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream)
+    if rc:
+        N.check(rc, what)
 
 
 def kv4_pool(pages: int, kv_heads: int, head_dim: int, page_size: int = 64, *, device=None) -> torch.Tensor:
@@ -391,42 +403,42 @@ def kv4_append(pool: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tens
     index has no page is not written and bit 0x80 of ``error_word`` is set.
     """
     name = "kv4_append"
+    _serving(name, tensor_layout, k)
     dev, dt = k.device, k.dtype
-    kk, vv, qq = _serving(name, tensor_layout, dt, dev, k, v, q)
-    H, D, page, B = _cache(name, pool, page_table, dev)
-    S = kk.shape[2]
-    if kk.shape != (B, H, S, D) or vv.shape != kk.shape:
-        raise ValueError(f"{name}: k and v must be [{B},{H},S,{D}] as the cache and page table say, got "
-                         f"{tuple(kk.shape)} and {tuple(vv.shape)}")
-    Hq, out, oo = 0, None, None
-    if qq is not None:
-        Hq = qq.shape[1]
-        if qq.shape != (B, Hq, S, D) or Hq < 1 or Hq % H:
-            raise ValueError(f"{name}: q must be [{B}, a multiple of {H}, {S}, {D}], got {tuple(qq.shape)}")
-        out, oo = _empty_like_layout(B, Hq, S, D, tensor_layout, dt, dev)
-    rows = rot = 0
-    if (cos is None) != (sin is None):
-        raise ValueError(f"{name}: cos and sin come together")
-    if cos is not None:
-        if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32 \
-                or cos.device != dev or sin.device != dev:
-            raise ValueError(f"{name}: cos and sin must be FP32 [positions, R/2] on {dev}")
-        rows, rot = cos.shape[0], 2 * cos.shape[1]
+    H, D, page, B, width, pages = _cache(name, pool, page_table, dev)
+    k, kp, kB, kH, S, kD, ksb, ksh, kss = _bhsd(name, "k", k, tensor_layout, dt, dev)
+    v, vp, vB, vH, vS, vD, vsb, vsh, vss = _bhsd(name, "v", v, tensor_layout, dt, dev)
+    if kB != B or kH != H or kD != D or vB != B or vH != H or vD != D or vS != S:
+        raise ValueError(f"{name}: k and v must be {B} x {H} heads x S x {D} as the cache and page table say, got "
+                         f"{tuple(k.shape)} and {tuple(v.shape)} ({tensor_layout})")
+    out, Hq, qp, op, qsb, qsh, qss, osb, osh, oss = None, 0, None, None, D, D, D, D, D, D
+    if q is not None:
+        q0 = q
+        view = q, qp, qB, Hq, qS, qD, qsb, qsh, qss = _bhsd(name, "q", q, tensor_layout, dt, dev)
+        if qB != B or qS != S or qD != D or Hq < 1 or Hq % H:
+            raise ValueError(f"{name}: q must be {B} x a multiple of {H} heads x {S} x {D}, got {tuple(q.shape)} "
+                             f"({tensor_layout})")
+        out, op, osb, osh, oss, _ = _output(name, None, q0, view, tensor_layout)
+    rows, rot, cp, sp = 0, 0, None, None
+    if cos is not None or sin is not None:
+        if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or cos.dtype is not _F32 or \
+                sin.dtype is not _F32 or cos.device != dev or sin.device != dev:
+            raise ValueError(f"{name}: cos and sin come together, FP32 [positions, R/2] on {dev}")
+        rows, rot = cos.shape
+        rot *= 2
         if rot % 16 or rot > D or rows < 1 or rot < 16:
             raise ValueError(f"{name}: cos/sin must have at least one row and R/2 columns with R a multiple of 16, at "
                              f"most {D}")
         cos, sin = cos.contiguous(), sin.contiguous()
+        cp, sp = cos.data_ptr(), sin.data_ptr()
     lengths = _ints(name, "lengths", lengths, (B,), dev)
     positions = _ints(name, "positions", positions, (B, S), dev)
     counts = _ints(name, "counts", counts, (B,), dev)
-    if S == 0:
+    if S == 0 or B == 0:
         return out
-    ks, vs = _strides(kk), _strides(vv)
-    qs, os_ = (_strides(qq), _strides(oo)) if qq is not None else (ks, ks)
-    _call(name, dev, N.load().vc_kv4_append, kk.data_ptr(), vv.data_ptr(), _p(qq), _p(oo), _DT[dt], B, Hq, H, S, D,
-          ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], qs[0], qs[1], qs[2], os_[0], os_[1], os_[2], _p(cos), _p(sin), rows,
-          rot, int(interleaved), _p(positions), lengths.data_ptr(), _p(counts), pool.data_ptr(), pool.shape[0], page,
-          page_table.data_ptr(), page_table.shape[1])
+    _call(name, dev, N.load().vc_kv4_append, kp, vp, qp, op, _DT[dt], B, Hq, H, S, D, ksb, ksh, kss, vsb, vsh, vss,
+          qsb, qsh, qss, osb, osh, oss, cp, sp, rows, rot, interleaved, _p(positions), lengths.data_ptr(), _p(counts),
+          pool.data_ptr(), pages, page, page_table.data_ptr(), width)
     return out
 
 
@@ -436,24 +448,25 @@ def kv4_read(pool: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor |
     0) to ``start[b] + count - 1`` of every sequence: (K, V) in ``dtype``
     (FP16, BF16 or FP32), [B,Hkv,count,D] or [B,count,Hkv,D] for NHD."""
     name = "kv4_read"
-    if tensor_layout not in _LAYOUTS:
+    if tensor_layout != "HND" and tensor_layout != "NHD":
         raise ValueError(f"{name}: tensor_layout must be HND or NHD")
     if dtype not in _DT:
         raise ValueError(f"{name}: dtype must be FP16, BF16 or FP32")
-    _require_cuda(name, pool, page_table, start)
+    if not pool.is_cuda:
+        raise ValueError(f"{name}: tensors must be on a CUDA device (no CPU fallback)")
     dev = pool.device
-    H, D, page, B = _cache(name, pool, page_table, dev)
+    H, D, page, B, width, pages = _cache(name, pool, page_table, dev)
     count = int(count)
     if count < 0:
         raise ValueError(f"{name}: count must not be negative")
     start = _ints(name, "start", start, (B,), dev)
-    k, kk = _empty_like_layout(B, H, count, D, tensor_layout, dtype, dev)
-    v, vv = _empty_like_layout(B, H, count, D, tensor_layout, dtype, dev)
+    shape = (B, H, count, D) if tensor_layout == "HND" else (B, count, H, D)
+    k = torch.empty(shape, dtype=dtype, device=dev)
+    v = torch.empty_like(k)
     if count and B:
-        ks, vs = _strides(kk), _strides(vv)
-        _call(name, dev, N.load().vc_kv4_read, pool.data_ptr(), pool.shape[0], page, page_table.data_ptr(),
-              page_table.shape[1], _p(start), B, H, count, D, kk.data_ptr(), vv.data_ptr(), _DT[dtype], ks[0], ks[1],
-              ks[2], vs[0], vs[1], vs[2])
+        sb, sh, ss = (H * count * D, count * D, D) if tensor_layout == "HND" else (H * count * D, D, H * D)
+        _call(name, dev, N.load().vc_kv4_read, pool.data_ptr(), pages, page, page_table.data_ptr(), width, _p(start), B,
+              H, count, D, k.data_ptr(), v.data_ptr(), _DT[dtype], sb, sh, ss, sb, sh, ss)
     return k, v
 
 
@@ -462,7 +475,7 @@ def _visibility(name, window, sinks, causal, sm_scale, D):
         raise ValueError(f"{name}: window must be None or a positive integer")
     if isinstance(sinks, bool) or not isinstance(sinks, int) or sinks < 0:
         raise ValueError(f"{name}: sinks must be a non-negative integer")
-    if not isinstance(causal, bool):
+    if causal is not True and causal is not False:
         raise ValueError(f"{name}: causal must be a bool")
     scale = D ** -0.5 if sm_scale is None else float(sm_scale)
     if not (0 < scale <= 3.4028234663852886e38):
@@ -488,46 +501,33 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor,
     tensor like ``q``, or ``out``.
     """
     name = "kv4_attention"
-    dev, dt = q.device, q.dtype
-    qq, oo = _serving(name, tensor_layout, dt, dev, q, None)
-    H, D, page, B = _cache(name, pool, page_table, dev)
-    Hq, Sq = qq.shape[1], qq.shape[2]
-    if qq.shape != (B, Hq, Sq, D) or Hq < 1 or Hq % H:
-        raise ValueError(f"{name}: q must be [{B}, a multiple of {H}, Sq, {D}] as the cache and page table say, got "
-                         f"{tuple(qq.shape)}")
+    _serving(name, tensor_layout, q)
+    dev, dt, q0 = q.device, q.dtype, q
+    H, D, page, B, width, pages = _cache(name, pool, page_table, dev)
+    view = q, qp, qB, Hq, Sq, qD, qsb, qsh, qss = _bhsd(name, "q", q, tensor_layout, dt, dev)
+    if qB != B or qD != D or Hq < 1 or Hq % H:
+        raise ValueError(f"{name}: q must be {B} x a multiple of {H} heads x Sq x {D} as the cache and page table say, got "
+                         f"{tuple(q.shape)} ({tensor_layout})")
     window, sinks, scale = _visibility(name, window, sinks, causal, sm_scale, D)
     lengths = _ints(name, "lengths", lengths, (B,), dev)
     q_lengths = _ints(name, "q_lengths", q_lengths, (B,), dev)
-    width = page_table.shape[1]
-    most = width * page if max_length is None else int(max_length)
-    if most < 0:
-        raise ValueError(f"{name}: max_length must not be negative")
-    most = min(most, width * page)
-    out, oo, copy = _output(name, out, q, tensor_layout, B, Hq, Sq, D)
-    if Sq == 0:
+    most = width * page
+    if max_length is not None:
+        if max_length < 0:
+            raise ValueError(f"{name}: max_length must not be negative")
+        most = min(most, int(max_length))
+    out, op, osb, osh, oss, copy = _output(name, out, q0, view, tensor_layout)
+    if Sq == 0 or B == 0:
         return out
     lib = N.load()
     wsb = lib.vc_kv4_attention_workspace_bytes(B, Hq, H, Sq, D, causal, window, sinks, page, width, most)
-    ws = _workspace(wsb, dev) if wsb else None
-    qs, os_ = _strides(qq), _strides(oo)
-    _call(name, dev, lib.vc_kv4_attention_fwd, qq.data_ptr(), _DT[dt], B, Hq, H, Sq, D, qs[0], qs[1], qs[2],
-          pool.data_ptr(), pool.shape[0], page, page_table.data_ptr(), width, lengths.data_ptr(), _p(q_lengths), causal,
-          window, sinks, most, scale, oo.data_ptr(), os_[0], os_[1], os_[2], _p(ws), wsb)
+    ws = torch.empty(wsb, dtype=_U8, device=dev) if wsb else None
+    _call(name, dev, lib.vc_kv4_attention_fwd, qp, _DT[dt], B, Hq, H, Sq, D, qsb, qsh, qss, pool.data_ptr(), pages, page,
+          page_table.data_ptr(), width, lengths.data_ptr(), _p(q_lengths), causal, window, sinks, most, scale, op, osb,
+          osh, oss, _p(ws), wsb)
     if copy is not None:
-        copy.copy_(oo)
+        out.copy_(copy)
     return out
-
-
-def _output(name, out, q, layout, B, H, S, D):
-    """(out, aligned [B,H,S,D] view that the library writes, view to copy it to or None)."""
-    if out is None:
-        out, oo = _empty_like_layout(B, H, S, D, layout, q.dtype, q.device)
-        return out, oo, None
-    if out.shape != q.shape or out.dtype is not q.dtype or out.device != q.device:
-        raise ValueError(f"{name}: out must have q's shape, dtype and device")
-    view = out if layout == "HND" else out.transpose(1, 2)
-    oo = _aligned(view)
-    return out, oo, (None if oo is view else view)
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int | None = None, sinks: int = 0,
@@ -541,32 +541,33 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     iff j < ``kv_lengths[b]`` (default Sk), (``causal`` implies j <= i) and (no
     ``window``, or j > i - window, or j < ``sinks``).  Rows that see nothing are
     zeros; keys and values at and past ``kv_lengths[b]`` are not used, whatever
-    they hold.  Returns a new tensor like ``q``, or ``out``.
+    they hold.  Values of keys before that should be finite: one that is not may
+    reach rows that do not see it (0 * inf).  Returns a new tensor like ``q``,
+    or ``out``.
     """
     name = "window_attention"
-    dev, dt = q.device, q.dtype
-    qq, kk, vv = _serving(name, tensor_layout, dt, dev, q, k, v)
-    B, Hq, Sq, D = qq.shape
-    H, Sk = kk.shape[1], kk.shape[2]
-    if D not in (64, 128):
+    _serving(name, tensor_layout, q)
+    dev, dt, q0 = q.device, q.dtype, q
+    view = q, qp, B, Hq, Sq, D, qsb, qsh, qss = _bhsd(name, "q", q, tensor_layout, dt, dev)
+    k, kp, kB, H, Sk, kD, ksb, ksh, kss = _bhsd(name, "k", k, tensor_layout, dt, dev)
+    v, vp, vB, vH, vS, vD, vsb, vsh, vss = _bhsd(name, "v", v, tensor_layout, dt, dev)
+    if D != 64 and D != 128:
         raise ValueError(f"{name}: head dim must be 64 or 128, got {D}")
-    if kk.shape != (B, H, Sk, D) or vv.shape != kk.shape or B < 1 or H < 1 or Hq < 1 or Hq % H:
+    if kB != B or kD != D or vB != B or vH != H or vS != Sk or vD != D or H < 1 or Hq < 1 or Hq % H:
         raise ValueError(f"{name}: k and v must share one shape with q's batch and head dim and a head count that divides "
-                         f"q's, got q {tuple(qq.shape)}, k {tuple(kk.shape)}, v {tuple(vv.shape)}")
+                         f"q's, got q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} ({tensor_layout})")
     window, sinks, scale = _visibility(name, window, sinks, causal, sm_scale, D)
     kv_lengths = _ints(name, "kv_lengths", kv_lengths, (B,), dev)
-    out, oo, copy = _output(name, out, q, tensor_layout, B, Hq, Sq, D)
-    if Sq == 0:
+    out, op, osb, osh, oss, copy = _output(name, out, q0, view, tensor_layout)
+    if Sq == 0 or B == 0:
         return out
     lib = N.load()
     wsb = lib.vc_window_attention_workspace_bytes(B, Hq, H, Sq, Sk, D, causal, window, sinks)
-    ws = _workspace(wsb, dev) if wsb else None
-    qs, ks, vs, os_ = _strides(qq), _strides(kk), _strides(vv), _strides(oo)
-    _call(name, dev, lib.vc_window_attention_fwd, qq.data_ptr(), kk.data_ptr(), vv.data_ptr(), _DT[dt], B, Hq, H, Sq, Sk,
-          D, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], _p(kv_lengths), causal, window, sinks, scale,
-          oo.data_ptr(), os_[0], os_[1], os_[2], _p(ws), wsb)
+    ws = torch.empty(wsb, dtype=_U8, device=dev) if wsb else None
+    _call(name, dev, lib.vc_window_attention_fwd, qp, kp, vp, _DT[dt], B, Hq, H, Sq, Sk, D, qsb, qsh, qss, ksb, ksh, kss,
+          vsb, vsh, vss, _p(kv_lengths), causal, window, sinks, scale, op, osb, osh, oss, _p(ws), wsb)
     if copy is not None:
-        copy.copy_(oo)
+        out.copy_(copy)
     return out
 
 
