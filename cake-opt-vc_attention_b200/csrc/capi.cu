@@ -120,8 +120,8 @@ int check_rows(const char* fn, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq) {
 }
 
 int check_tokens(const char* fn, const char* name, int64_t n) {
-  if (n < 0 || n > (int64_t(1) << 31) - 65536) {
-    set_last_error("%s: %s must be in [0, 2^31 - 65536] (got %lld)", fn, name, (long long)n);
+  if (n < 0 || n >= (int64_t(1) << 30)) {
+    set_last_error("%s: %s must be in [0, 2^30) (got %lld)", fn, name, (long long)n);
     return VC_ERR_ARG;
   }
   return VC_OK;
@@ -137,8 +137,9 @@ int check_cache(const char* fn, const void* pool, int64_t pages, int64_t page_si
     set_last_error("%s: page_size must be 16, 32, 64, 128 or 256 (got %lld)", fn, (long long)page_size);
     return VC_ERR_ARG;
   }
-  if (pages < 1 || pages > INT32_MAX || width < 0 || width > INT32_MAX / page_size || (width > 0 && !table)) {
-    set_last_error("%s: need 1 <= pages < 2^31, 0 <= table_width * page_size < 2^31 and a page table", fn);
+  if (pages < 1 || pages > INT32_MAX || width < 0 || width > INT32_MAX || width * page_size >= (int64_t(1) << 30) ||
+      (width > 0 && !table)) {
+    set_last_error("%s: need 1 <= pages < 2^31, 0 <= table_width * page_size < 2^30 and a page table", fn);
     return VC_ERR_ARG;
   }
   return VC_OK;

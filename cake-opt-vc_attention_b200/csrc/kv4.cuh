@@ -54,6 +54,18 @@ inline Kv4Pages kv4_pages(const Kv4CacheArgs& c) {
   return g;
 }
 
+// The length and query count of sequence b, clamped to the table and to Sq.
+__device__ __forceinline__ void kv4_sequence(const Kv4Pages& pages, const int32_t* lengths, const int32_t* q_lengths,
+                                             int Sq, int64_t b, int& len, int& nq) {
+  len = __ldg(lengths + b);
+  const int most = static_cast<int>(pages.width) << pages.page_shift;
+  if (len < 0 || len > most) {
+    if (threadIdx.x == 0) raise_error(kErrBadIndex);
+    len = len < 0 ? 0 : most;
+  }
+  nq = q_lengths ? max(0, min(__ldg(q_lengths + b), Sq)) : Sq;
+}
+
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 

@@ -115,17 +115,6 @@ __device__ __forceinline__ void load8(const T* p, float* x) {
   }
 }
 
-// The sequence's length and query count, clamped to the table and to Sq.
-__device__ __forceinline__ void sequence(const DecodeParams& p, int64_t b, int64_t& len, int64_t& nq) {
-  len = __ldg(p.lengths + b);
-  const int64_t most = p.pages.width << p.pages.page_shift;
-  if (len < 0 || len > most) {
-    if (threadIdx.x == 0) raise_error(kErrBadIndex);
-    len = len < 0 ? 0 : most;
-  }
-  nq = p.q_lengths ? min64(__ldg(p.q_lengths + b), p.Sq) : p.Sq;
-  if (nq < 0) nq = 0;
-}
 
 template <int D, int NT>
 struct DecodeSmem {
@@ -148,9 +137,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv4_decode_kernel(D
   const int split = blockIdx.x;
   const int64_t bh = blockIdx.y, b = bh / p.pages.heads, hk = bh % p.pages.heads;
   const int row0 = blockIdx.z * 8 * NT;
-  int64_t len, nq;
-  sequence(p, b, len, nq);
-  const int live_rows = static_cast<int>(nq) * p.G;
+  int len, nq;
+  kv4_sequence(p.pages, p.lengths, p.q_lengths, static_cast<int>(p.Sq), b, len, nq);
+  const int live_rows = nq * p.G;
 
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar) + warp * L::kStages;
   if (lane == 0)
@@ -159,34 +148,35 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv4_decode_kernel(D
   __syncwarp();
 
   // keys that some row of this CTA sees, in tiles of 32: sinks [0, nsink) and [main0, main0 + nmain)
-  int64_t nsink = 0, main0 = 0, ntiles = 0;
+  int nsink = 0, main0 = 0, ntiles = 0;
   const int last_row = min(row0 + 8 * NT, live_rows) - 1;
-  int64_t pos_first = 0, pos_last = 0;
+  int pos_first = 0, pos_last = 0;
   if (last_row >= row0) {
     pos_first = len - nq + row0 / p.G;
     pos_last = len - nq + last_row / p.G;
     const KeyRanges a = visible_keys(p.vis, pos_first, len), z = visible_keys(p.vis, pos_last, len);
-    const int64_t lo = p.vis.window ? a.lo : 0, hi = z.hi;   // the last row reaches furthest, the first starts first
-    const int64_t sink_end = p.vis.window ? min64(p.vis.sinks, hi) : 0;
+    const int lo = p.vis.window ? a.lo : 0, hi = z.hi;   // the last row reaches furthest, the first starts first
+    const int sink_end = p.vis.window ? min(p.vis.sinks, hi) : 0;
     main0 = lo / kTile;
-    const int64_t end = (hi + kTile - 1) / kTile;
-    nsink = min64((sink_end + kTile - 1) / kTile, main0);
+    const int end = (hi + kTile - 1) / kTile;
+    nsink = min((sink_end + kTile - 1) / kTile, main0);
     ntiles = nsink + (end > main0 ? end - main0 : 0);
   }
-  const int64_t t_begin = ntiles * split / p.splits, t_end = ntiles * (split + 1) / p.splits;
-  const int64_t i0 = t_begin + warp;
-  const int mine = i0 < t_end ? static_cast<int>((t_end - i0 + kWarps - 1) / kWarps) : 0;
+  const int t_begin = static_cast<int>(int64_t(ntiles) * split / p.splits);
+  const int t_end = static_cast<int>(int64_t(ntiles) * (split + 1) / p.splits);
+  const int i0 = t_begin + warp;
+  const int mine = i0 < t_end ? (t_end - i0 + kWarps - 1) / kWarps : 0;
 
   // ring: lanes 0 and 1 bring a record each; okbits: which of the lane's stages hold one
   uint8_t* ring = smem + warp * L::kStages * L::kTileBytes;
   uint32_t okbits = 0;
-  auto tile_of = [&](int i) -> int64_t {
-    const int64_t t = i0 + int64_t(i) * kWarps;
+  auto tile_of = [&](int i) -> int {
+    const int t = i0 + i * kWarps;
     return t < nsink ? t : main0 + (t - nsink);
   };
   auto locate = [&](int i) -> int64_t {   // lanes 0 and 1: the record's offset, -1 past the end, -2 without a page
     if (lane > 1 || i >= mine) return -1;
-    const int64_t blk = tile_of(i) * 2 + lane;
+    const int blk = tile_of(i) * 2 + lane;
     if (blk * kKv4Block >= len) return -1;
     const int64_t rec = p.pages.record<D>(b, hk, blk);
     return rec < 0 ? -2 : rec;
@@ -276,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv4_decode_kernel(D
   const int tok = (r >> 1) + 4 * (r & 1);
   // rows see all of a tile iff it ends before every row's last key and starts after every row's first
   const KeyRanges first = visible_keys(p.vis, pos_first, len);
-  const int64_t last_lo = visible_keys(p.vis, pos_last, len).lo;
+  const int last_lo = visible_keys(p.vis, pos_last, len).lo;
   bool ok = true;
   for (int i = 0; i < mine; ++i) {
     {
@@ -288,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv4_decode_kernel(D
     ok = __all_sync(0xffffffffu, mbar_wait(&bars[s], (i / L::kStages) & 1, kErrTimeoutTma));
     if (!ok) break;
     const uint32_t have = __ballot_sync(0xffffffffu, (okbits >> s) & 1u) & 3u;
-    const int64_t key0 = tile_of(i) * kTile;
+    const int key0 = tile_of(i) * kTile;
     const bool whole = have == 3u && key0 + kTile <= first.hi &&
                        (p.vis.window == 0 || key0 >= last_lo || key0 + kTile <= p.vis.sinks);
     const uint32_t base = smem_u32(ring + s * L::kTileBytes);
@@ -354,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv4_decode_kernel(D
           for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              const int64_t key = key0 + 16 * k + tok + 8 * half;
+              const int key = key0 + 16 * k + tok + 8 * half;
               const bool see = ((have >> k) & 1u) && key < v.hi && (key >= v.lo || key < v.sink_end);
               if (!see) x[k][nt][2 * half + j] = -INFINITY;
             }
@@ -601,7 +591,7 @@ int kv4_attention(const Kv4AttnArgs& a, cudaStream_t st) {
   p.G = static_cast<int>(a.Hq / a.cache.Hkv);
   p.rows = static_cast<int>(a.Sq * p.G);
   p.splits = plan.splits;
-  p.vis = Visibility{a.window, a.sinks, a.causal};
+  p.vis = visibility(a.window, a.sinks, a.causal);
   p.scale_log2 = a.sm_scale * kLog2e;
   p.part_o = static_cast<float*>(a.workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + BH * p.rows * plan.splits * a.D);

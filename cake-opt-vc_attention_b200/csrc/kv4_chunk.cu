@@ -9,7 +9,7 @@ TilePlan plan_of(const Kv4AttnArgs& a) {
   const int64_t G = a.Hq / a.cache.Hkv;
   int64_t keys = a.cache.width * a.cache.page_size;
   if (a.max_length > 0) keys = min64(keys, a.max_length);
-  return tile_plan(a.cache.B * a.cache.Hkv, a.Sq * G, G, keys, Visibility{a.window, a.sinks, a.causal});
+  return tile_plan(a.cache.B * a.cache.Hkv, a.Sq * G, G, keys, visibility(a.window, a.sinks, a.causal));
 }
 
 }  // namespace
@@ -33,7 +33,7 @@ int kv4_chunk_attention(const Kv4AttnArgs& a, cudaStream_t st) {
   p.rows = static_cast<int>(a.Sq * p.G);
   p.pairs = static_cast<int>(t.pairs);
   p.splits = static_cast<int>(t.splits);
-  p.vis = Visibility{a.window, a.sinks, a.causal};
+  p.vis = visibility(a.window, a.sinks, a.causal);
   p.scale_log2 = a.sm_scale * kLog2e;
   p.lengths = a.lengths;
   p.q_lengths = a.q_lengths;

@@ -50,14 +50,13 @@ struct TileParams {
   const void* q;
   void* out;
   int64_t qsb, qsh, qss, osb, osh, oss;
-  int64_t Sq, Sk;
+  int Sq, Sk;
   int Hkv, BH;                 // BH = B * Hkv
   int G, rows, pairs, splits;  // rows = Sq * G
   Visibility vis;
   float scale_log2;            // sm_scale * log2(e)
   const int32_t *lengths, *q_lengths;
   Kv4Pages pages;              // 4-bit cache only
-  // 16-bit K/V only: V rows that a tile shares with keys past the end are cleared
   float* part_o;
   float2* part_ml;
 };
@@ -69,6 +68,7 @@ struct TileCfg {
   static constexpr int kKS = KV4 ? 2 : D == 128 ? 3 : 4;     // K ring
   static constexpr int kVS = KV4 ? 2 : D == 128 ? 2 : 4;     // V ring
   static constexpr int kRS = KV4 ? 3 : 0;                    // ring of raw half tiles (64 keys)
+  static constexpr int kPoly = KV4 ? 0 : 2;   // of eight pairs of exponentials, on the FMA pipe
   static constexpr int kRaw = 4 * Kv4Rec<D>::kBytes;
   static constexpr int kOffQ = 0;
   static constexpr int kOffK = kOffQ + 2 * kTile;
@@ -85,7 +85,7 @@ struct TileMeta {
 };
 
 struct __align__(16) TileCtl {
-  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], q_ready[2], s_full[2], p_full[2], o_final[2], v_fix;
+  uint64_t k_full[4], v_full[4], step_done[4], q_ready[2], s_full[2], p_full[2], o_final[2], v_fix;
   uint64_t raw_full[3], raw_empty[3], meta_full[4];
   TileMeta meta[4];
   uint32_t raw_miss[3];
@@ -123,7 +123,7 @@ __device__ __forceinline__ uint32_t swizzled(int row, int ch) { return row * 128
 
 // The keys a group of rows sees, and which of the CTA's tiles that touches.
 struct GroupKeys {
-  int lo, hi, sink_end;    // union over its rows (keys fit 32 bits: at most 2^31 - 65536 tokens)
+  int lo, hi, sink_end;    // union over its rows
   int hi_all, lo_all;      // what every row sees: [lo_all, hi_all)
   bool any;
   __device__ __forceinline__ bool sees(int tile) const {
@@ -131,23 +131,62 @@ struct GroupKeys {
   }
 };
 
+// 2^x of the first N pairs of e on the FMA pipe: the special-function unit
+// gives 16 results a clock and SM, and a 128 x 128 tile wants 16384 of them, as
+// many clocks as its MMAs take.  x = n + f, n the nearest integer (adding
+// 1.5*2^23 rounds, and leaves n in the low bits), 2^f on [-1/2, 1/2] by the
+// polynomial of degree 4 with the least relative error (2.6e-6, by iteratively
+// reweighted least squares; far below a probability's 16-bit rounding), n added
+// to the exponent field.  x below -125 counts as -125.  The pairs go through
+// the steps side by side.
+template <int N>
+__device__ __forceinline__ void exp2_fma(uint32_t (&e)[16]) {
+  if constexpr (N > 0) {
+    const uint64_t magic = pk2f(12582912.f, 12582912.f);
+    const float c[5] = {0.009570102207362652f, 0.05591786280274391f, 0.240247443318367f, 0.6931217908859253f, 0.9999992847442627f};
+    uint64_t t[N], f[N], r[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = pk2f(fmaxf(__uint_as_float(e[2 * i]), -125.f), fmaxf(__uint_as_float(e[2 * i + 1]), -125.f));
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = f2_add(f[i], magic);
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = f2_sub(t[i], magic);
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = f2_sub(f[i], r[i]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = f2_fma(pk2f(c[0], c[0]), f[i], pk2f(c[1], c[1]));
+#pragma unroll
+    for (int k = 2; k < 5; ++k)
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[i] = f2_fma(r[i], f[i], pk2f(c[k], c[k]));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      uint32_t ta, tb, ra, rb;
+      up2(t[i], ta, tb);
+      up2(r[i], ra, rb);
+      e[2 * i] = ra + (ta << 23);
+      e[2 * i + 1] = rb + (tb << 23);
+    }
+  }
+}
+
 // Which of keys k .. k + 31 lie in [lo, hi) or [0, sink).
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
 __device__ __forceinline__ uint32_t visible_bits(int lo, int hi, int sink, int k) {
   return (bits_below(hi - k) & ~bits_below(lo - k)) | bits_below(sink - k);
 }
 
-__device__ __forceinline__ GroupKeys group_keys(const Visibility& v, int64_t base, int r0, int live, int G, int64_t len) {
+__device__ __forceinline__ GroupKeys group_keys(const Visibility& v, int base, int r0, int live, int G, int len) {
   GroupKeys k{};
   k.any = r0 < live;
   if (!k.any) return k;
-  const int64_t first = base + r0 / G, last = base + (min(r0 + 128, live) - 1) / G;
-  const KeyRanges a = visible_keys(v, first, len), z = visible_keys(v, last, len);
-  k.hi = static_cast<int>(z.hi);
-  k.lo = static_cast<int>(a.lo);
-  k.sink_end = v.window ? static_cast<int>(min64(v.sinks, z.hi)) : 0;
-  k.hi_all = static_cast<int>(a.hi);
-  k.lo_all = static_cast<int>(z.lo);
+  const KeyRanges a = visible_keys(v, base + r0 / G, len);
+  const KeyRanges z = visible_keys(v, base + (min(r0 + 128, live) - 1) / G, len);
+  k.hi = z.hi;
+  k.lo = a.lo;
+  k.sink_end = v.window ? min(v.sinks, z.hi) : 0;
+  k.hi_all = a.hi;
+  k.lo_all = z.lo;
   return k;
 }
 
@@ -167,25 +206,43 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
   const int pair = p.pairs - 1 - static_cast<int>(blockIdx.x) / p.BH;
   const int bh = static_cast<int>(blockIdx.x) % p.BH, b = bh / p.Hkv, hk = bh - b * p.Hkv;
 
-  int64_t len, nq, base;
-  if constexpr (KV4) {
-    len = __ldg(p.lengths + b);
-    const int64_t most = p.pages.width << p.pages.page_shift;
-    if (len < 0 || len > most) {
-      if (threadIdx.x == 0) raise_error(kErrBadIndex);
-      len = len < 0 ? 0 : most;
+  if (warp == 9) {
+    tmem_alloc(&ctl->slot, 512);
+    tmem_relinquish();
+  }
+  if (threadIdx.x == 256) {
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&ctl->k_full[s], KV4 ? 64 : 1);
+      mbar_init(&ctl->step_done[s], 1);
+      mbar_init(&ctl->v_full[s], KV4 ? 64 : 1);
+      if constexpr (KV4) mbar_init(&ctl->meta_full[s], 128);
     }
-    nq = p.q_lengths ? min64(__ldg(p.q_lengths + b), p.Sq) : p.Sq;
-    if (nq < 0) nq = 0;
+    if constexpr (KV4) {
+      for (int s = 0; s < 3; ++s) {
+        mbar_init(&ctl->raw_full[s], 1);
+        mbar_init(&ctl->raw_empty[s], 4);
+      }
+    } else {
+      mbar_init(&ctl->v_fix, 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&ctl->q_ready[x], 128);
+      mbar_init(&ctl->s_full[x], 1);
+      mbar_init(&ctl->p_full[x], 128);
+      mbar_init(&ctl->o_final[x], 1);
+    }
+    fence_barrier_init();
+  }
+  int len, nq, base;
+  if constexpr (KV4) {
+    kv4_sequence(p.pages, p.lengths, p.q_lengths, p.Sq, b, len, nq);
     base = len - nq;
   } else {
-    len = p.Sk;
-    if (p.lengths) len = min64(__ldg(p.lengths + b), p.Sk);
-    if (len < 0) len = 0;
+    len = p.lengths ? max(0, min(__ldg(p.lengths + b), p.Sk)) : p.Sk;
     nq = p.Sq;
     base = p.Sk - p.Sq;
   }
-  const int live = static_cast<int>(nq) * p.G;
+  const int live = nq * p.G;
   const GroupKeys ga = group_keys(p.vis, base, pair * 256, live, p.G, len);
   const GroupKeys gb = group_keys(p.vis, base, pair * 256 + 128, live, p.G, len);
   // the list of tiles: sinks [0, nsink), then [main0, main0 + ...)
@@ -206,31 +263,6 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
     return i < nsink ? i : main0 + (i - nsink);
   };
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < 4; ++s) {
-      mbar_init(&ctl->k_full[s], KV4 ? 64 : 1);
-      mbar_init(&ctl->k_empty[s], 1);
-      mbar_init(&ctl->v_full[s], KV4 ? 64 : 1);
-      mbar_init(&ctl->v_empty[s], 1);
-      mbar_init(&ctl->meta_full[s], 128);
-    }
-    for (int s = 0; s < 3; ++s) {
-      mbar_init(&ctl->raw_full[s], 1);
-      mbar_init(&ctl->raw_empty[s], 4);
-    }
-    for (int x = 0; x < 2; ++x) {
-      mbar_init(&ctl->q_ready[x], 128);
-      mbar_init(&ctl->s_full[x], 1);
-      mbar_init(&ctl->p_full[x], 128);
-      mbar_init(&ctl->o_final[x], 1);
-    }
-    mbar_init(&ctl->v_fix, 1);
-    fence_barrier_init();
-  }
-  if (warp == 9) {
-    tmem_alloc(&ctl->slot, 512);
-    tmem_relinquish();
-  }
   if constexpr (!KV4) {
     if (warp == 8 && lane == 0) tma_prefetch_desc(&tmk);
     if (warp == 10 && lane == 0) tma_prefetch_desc(&tmv);
@@ -241,8 +273,8 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
   const uint32_t tmem = ctl->slot;
 
   if (warp >= 8) {
-    if constexpr (KV4) setmaxnreg_dec<80>();
-    else setmaxnreg_dec<56>();
+    if constexpr (KV4) setmaxnreg_dec<64>();
+    else setmaxnreg_dec<88>();
     if (warp == 9) {
       // ------------------------------------------------------------- MMA issuer
       constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0 : 1;
@@ -252,72 +284,50 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
       const uint64_t kd0 = smem_desc_sw128(smem_u32(smem + C::kOffK));
       const uint64_t vd0 = smem_desc_mn128(smem_u32(smem + C::kOffV), kSeg);
       constexpr uint64_t kStep = C::kTile >> 4;
-      uint32_t done[2] = {0, 0};   // PVs issued, by group
+      uint32_t done[2] = {0, 0};              // PVs issued, by group
       int last[2] = {steps - 1, steps - 1};   // the last tile a group sees
       for (int x = 0; x < 2; ++x)
         while (last[x] >= 0 && !(x ? gb : ga).sees(tile_of(last[x]))) --last[x];
       bool ok = steps == 0 || (mbar_wait_warp(&ctl->q_ready[0], 0, kErrTimeoutMma) && mbar_wait_warp(&ctl->q_ready[1], 0, kErrTimeoutMma));
-      auto issue_qk = [&](int n, int x) {
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t kd = kd0 + (n % C::kKS) * kStep, qd = qd0 + x * kStep;
+      // Step n, group after group: P.V of tile n - 1, then QK^T of tile n over its scores' columns, issued in
+      // one go: an MMA takes 64 cycles and the queue is short, so what the issuer waits for between MMAs
+      // idles the tensor core (a wait that does not wait takes about 150 cycles).  The waits for the stages,
+      // which are there long before the probabilities, are therefore spread over the gaps.
+      ok = ok && (steps == 0 || mbar_wait_warp(&ctl->k_full[0], 0, kErrTimeoutMma));
+      for (int n = 0; n <= steps && ok; ++n) {
+        const int vs = (n - 1) % C::kVS, ks = n % C::kKS;
+        const uint64_t vd = vd0 + vs * kStep, kd = kd0 + ks * kStep;
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint64_t off = (kk >> 2) * (kSeg >> 4) + (kk & 3) * 2;
-            mma_f16_ss(tmem + x * 128, qd + off, kd + off, idesc_qk, kk > 0 ? 1u : 0u);
-          }
-          mma_commit(&ctl->s_full[x]);
-        }
-        __syncwarp();
-      };
-      if (ok && steps > 0) {
-        ok = mbar_wait_warp(&ctl->k_full[0], 0, kErrTimeoutMma);
-        if (ok) {
-          for (int x = 0; x < 2; ++x)
-            if ((x ? gb : ga).sees(tile_of(0))) issue_qk(0, x);
-          if (elect_one()) mma_commit(&ctl->k_empty[0]);
-          __syncwarp();
-        }
-      }
-      for (int n = 0; n < steps && ok; ++n) {
-        const int tile = tile_of(n), next = tile_of(n + 1);
-        const int vs = n % C::kVS;
-        const bool more = n + 1 < steps;
-        bool have_k = false;
-        ok = mbar_wait_warp(&ctl->v_full[vs], (n / C::kVS) & 1, kErrTimeoutMma);
-        for (int x = 0; x < 2 && ok; ++x) {
+        for (int x = 0; x < 2; ++x) {
+          if (!ok) break;
           const GroupKeys& g = x ? gb : ga;
-          if (g.sees(tile)) {
-            ok = mbar_wait_warp(&ctl->p_full[x], done[x] & 1, kErrTimeoutMma);
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-              const uint64_t vd = vd0 + vs * kStep;
+          const uint32_t scol = tmem + x * 128, ocol = tmem + 256 + x * 128;
+          const bool pv = n > 0 && g.sees(tile_of(n - 1)), qk = n < steps && g.sees(tile_of(n));
+          if (pv) ok = mbar_wait_warp(&ctl->p_full[x], done[x] & 1, kErrTimeoutMma);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            if (pv) {
 #pragma unroll
               for (int kk = 0; kk < 8; ++kk)
-                mma_f16_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8, vd + kk * (2048 >> 4), idesc_pv, (done[x] > 0 || kk > 0) ? 1u : 0u);
+                mma_f16_ts(ocol, scol + kk * 8, vd + kk * (2048 >> 4), idesc_pv, (done[x] > 0 || kk > 0) ? 1u : 0u);
+              if (n - 1 == last[x]) mma_commit(&ctl->o_final[x]);
             }
-            if (n == last[x] && elect_one()) mma_commit(&ctl->o_final[x]);
-            __syncwarp();
-            ++done[x];
-          }
-          if (more && g.sees(next)) {
-            if (!have_k) {
-              ok = mbar_wait_warp(&ctl->k_full[(n + 1) % C::kKS], ((n + 1) / C::kKS) & 1, kErrTimeoutMma);
-              if (!ok) break;
-              have_k = true;
+            if (qk) {
+              const uint64_t qd = qd0 + x * kStep;
+#pragma unroll
+              for (int kk = 0; kk < D / 16; ++kk) {
+                const uint64_t off = (kk >> 2) * (kSeg >> 4) + (kk & 3) * 2;
+                mma_f16_ss(scol, qd + off, kd + off, idesc_qk, kk > 0 ? 1u : 0u);
+              }
+              mma_commit(&ctl->s_full[x]);
             }
-            issue_qk(n + 1, x);
+            if (x == 1) mma_commit(&ctl->step_done[n & 3]);   // V of tile n - 1 and K of tile n are read
           }
-        }
-        if (!ok) break;
-        if (elect_one()) mma_commit(&ctl->v_empty[vs]);
-        __syncwarp();
-        if (more) {
-          if (!have_k) ok = mbar_wait_warp(&ctl->k_full[(n + 1) % C::kKS], ((n + 1) / C::kKS) & 1, kErrTimeoutMma);
-          if (!ok) break;
-          if (elect_one()) mma_commit(&ctl->k_empty[(n + 1) % C::kKS]);
           __syncwarp();
+          if (pv) ++done[x];
+          if (x == 0 && n < steps) ok = mbar_wait_warp(&ctl->v_full[n % C::kVS], (n / C::kVS) & 1, kErrTimeoutMma);
+          if (x == 1 && n + 1 < steps) ok = mbar_wait_warp(&ctl->k_full[(n + 1) % C::kKS], ((n + 1) / C::kKS) & 1, kErrTimeoutMma);
         }
       }
     } else if constexpr (!KV4) {
@@ -325,7 +335,7 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
         // ----------------------------------------------------------- K producer
         for (int n = 0; n < steps; ++n) {
           const int s = n % C::kKS;
-          if (n >= C::kKS && !mbar_wait(&ctl->k_empty[s], ((n / C::kKS) & 1) ^ 1, kErrTimeoutProducer)) break;
+          if (n >= C::kKS && !mbar_wait(&ctl->step_done[(n - C::kKS) & 3], ((n - C::kKS) >> 2) & 1, kErrTimeoutProducer)) break;
           mbar_expect_tx(&ctl->k_full[s], C::kTile);
           for (int g = 0; g < kSegs; ++g)
             tma_load_4d(smem + C::kOffK + s * C::kTile + g * kSeg, &tmk, &ctl->k_full[s], g * 64,
@@ -336,7 +346,7 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
         uint32_t fixes = 0;
         for (int n = 0; n < steps; ++n) {
           const int s = n % C::kVS;
-          if (n >= C::kVS && !mbar_wait_warp(&ctl->v_empty[s], ((n / C::kVS) & 1) ^ 1, kErrTimeoutProducer)) break;
+          if (n >= C::kVS && !mbar_wait_warp(&ctl->step_done[(n - C::kVS + 1) & 3], ((n - C::kVS + 1) >> 2) & 1, kErrTimeoutProducer)) break;
           const int k0 = tile_of(n) * 128;
           uint8_t* dst = smem + C::kOffV + s * C::kTile;
           // rows at and past the sequence's end hold whatever the tensor does: 0 x NaN would reach
@@ -401,14 +411,20 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
         const int w32 = (warp & 1) * 32;                  // first key in the half tile
         const int q = lane % kPer, part = q >> 1;         // 32 channels; their 64-channel group (D = 128)
         const __half2 minus1024 = __float2half2_rn(-1024.f), sixteenth = __float2half2_rn(0.0625f), minus64 = __float2half2_rn(-64.f);
-        uint64_t* empty = is_v ? ctl->v_empty : ctl->k_empty;
         uint64_t* full = is_v ? ctl->v_full : ctl->k_full;
         const int depth = is_v ? C::kVS : C::kKS;
+        const bool swap = D == 128 && part;
+        uint32_t chunk_at[4];   // where the four 16-byte chunks of a key's row go (the row's swizzle is the lane's)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) chunk_at[i] = ((((q & 1) * 4 + (swap ? i ^ 2 : i)) ^ ((lane / kPer) & 7)) << 4);
         bool ok = true;
         for (int n = 0; n < steps && ok; ++n) {
           const int st = n % depth;
           TileMeta* meta = &ctl->meta[n & 3];
-          if (n >= depth) ok = mbar_wait_warp(&empty[st], ((n / depth) & 1) ^ 1, kErrTimeoutProducer);
+          if (n >= depth) {
+            const int free_at = n - depth + (is_v ? 1 : 0);   // the step that reads the stage's last tile
+            ok = mbar_wait_warp(&ctl->step_done[free_at & 3], (free_at >> 2) & 1, kErrTimeoutProducer);
+          }
           for (int h = 0; h < 2 && ok; ++h) {
             const int ru = 2 * n + h, rs = ru % 3;
             ok = mbar_wait_warp(&ctl->raw_full[rs], (ru / 3) & 1, kErrTimeoutProducer);
@@ -451,19 +467,20 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
               }
             }
             const uint32_t clear = D == 128 && part ? clear1 : clear0;
-            uint8_t* dst = smem + (is_v ? C::kOffV : C::kOffK) + st * C::kTile + (D == 128 ? part * kSeg : 0);
-#pragma unroll 2
+            uint8_t* dst = smem + (is_v ? C::kOffV : C::kOffK) + st * C::kTile + (D == 128 ? part * kSeg : 0) + (h * 64 + w32 + lane / kPer) * 128;
+            const uint8_t* rec = raw + (w32 >> 4) * R::kBytes + (lane / kPer) * R::kCodeRow + (is_v ? R::kV : R::kK) + q * 16;
+            const uint8_t* pr = raw + (w32 >> 4) * R::kBytes + (lane / kPer) * R::kParRow + (is_v ? R::kVp : R::kKp) + (D == 128 ? part * 4 : 0);
+#pragma unroll
             for (int pass = 0; pass < kPer; ++pass) {
-              const int k32 = pass * kKeys + lane / kPer, kk = w32 + k32;
-              const uint8_t* rec = raw + (kk >> 4) * R::kBytes;
-              const uint4 codes = *reinterpret_cast<const uint4*>(rec + (is_v ? R::kV : R::kK) + (kk & 15) * R::kCodeRow + q * 16);
-              const uint32_t ms = *reinterpret_cast<const uint32_t*>(rec + (is_v ? R::kVp : R::kKp) + (kk & 15) * R::kParRow + (D == 128 ? part * 4 : 0));
+              // key pass * kKeys + lane / kPer of the 32: record key / 16, token key % 16
+              constexpr int kPerRec = 16 / kKeys;
+              const int ro = (pass / kPerRec) * R::kBytes;
+              const uint4 codes = *reinterpret_cast<const uint4*>(rec + ro + (pass % kPerRec) * kKeys * R::kCodeRow);
+              uint32_t ms = *reinterpret_cast<const uint32_t*>(pr + ro + (pass % kPerRec) * kKeys * R::kParRow);
+              if ((clear >> (pass * kKeys + lane / kPer)) & 1u) ms = 0u;   // scale and minimum 0
               const __half2 s2 = __float2half2_rn(bf16_lo(ms) * down), m2 = __float2half2_rn(bf16_hi(ms) * down);
-              const bool zero = (clear >> k32) & 1u;
               // the second group's lanes take their words in the order 2, 3, 0, 1: see the banks above
-              const bool swap = D == 128 && part;
               const uint32_t cw[4] = {swap ? codes.z : codes.x, swap ? codes.w : codes.y, swap ? codes.x : codes.z, swap ? codes.y : codes.w};
-              const int row = h * 64 + kk;
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const uint32_t c0 = cw[i], c8 = c0 >> 8;
@@ -474,11 +491,10 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
                   __half2 v = *reinterpret_cast<__half2*>(&x[j]);
                   v = (j & 1) ? __hfma2(v, sixteenth, minus64) : __hadd2(v, minus1024);   // the code, exactly
                   v = __hfma2(v, s2, m2);
-                  x[j] = zero ? 0u : *reinterpret_cast<uint32_t*>(&v);
+                  x[j] = *reinterpret_cast<uint32_t*>(&v);
                 }
                 // channels 8a + {0,4,1,5,2,6,3,7}: Q is stored and O written in the same order
-                const int a = (q & 1) * 4 + (swap ? i ^ 2 : i);
-                *reinterpret_cast<uint4*>(dst + swizzled(row, a)) = make_uint4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<uint4*>(dst + pass * kKeys * 128 + chunk_at[i]) = make_uint4(x[0], x[1], x[2], x[3]);
               }
             }
             __syncwarp();
@@ -492,8 +508,8 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
       }
     }
   } else {
-    if constexpr (KV4) setmaxnreg_inc<176>();
-    else setmaxnreg_inc<224>();
+    if constexpr (KV4) setmaxnreg_inc<192>();
+    else setmaxnreg_inc<208>();
     // ------------------------------------------------------------ softmax group X
     const int x = warp >> 2, t = threadIdx.x & 127;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -511,8 +527,8 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
     {
 #pragma unroll 4
       for (int i = 0; i < 32 / kRowsAt; ++i) {
-        const int lr = i * kRowsAt + rl, r = row0 + lr, rt = r / p.G, rh = hk * p.G + (r - rt * p.G);
-        const QT* src = static_cast<const QT*>(p.q) + b * p.qsb + rh * p.qsh + rt * p.qss + ch * 8;
+        const int lr = i * kRowsAt + rl, r = row0 + lr, rt = __shfl_sync(0xffffffffu, tok, lr), rh = hk * p.G + (r - rt * p.G);
+        const QT* src = static_cast<const QT*>(p.q) + int64_t(b) * p.qsb + rh * p.qsh + rt * p.qss + ch * 8;
         uint4 u = r < live ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
         if constexpr (KV4) {
           float f[8];
@@ -554,7 +570,7 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
       mbar_arrive(&ctl->q_ready[x]);
     }
     const KeyRanges seen_keys = visible_keys(p.vis, base + tok, len);
-    const int my_hi = static_cast<int>(seen_keys.hi), my_lo = static_cast<int>(seen_keys.lo), my_sink = static_cast<int>(seen_keys.sink_end);
+    const int my_hi = seen_keys.hi, my_lo = seen_keys.lo, my_sink = seen_keys.sink_end;
     float m = -INFINITY, l = 0.f;
     int frun = 0;              // 4-bit cache: O is in units of 2^frun
     uint32_t nan_out = 0;      // 4-bit cache: 64-channel groups of this row that saw a value that is not finite
@@ -608,65 +624,83 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
             if (!((v >> c) & 1u)) raw[32 * i + c] = 0xFF800000u;
         }
       }
-      float top = -INFINITY;
+      float top4[4][2];   // eight independent chains
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
-        float a = max3f(__uint_as_float(raw[32 * q4]), __uint_as_float(raw[32 * q4 + 1]), __uint_as_float(raw[32 * q4 + 2]));
-        float b2 = max3f(__uint_as_float(raw[32 * q4 + 3]), __uint_as_float(raw[32 * q4 + 4]), __uint_as_float(raw[32 * q4 + 5]));
-#pragma unroll
-        for (int c = 6; c < 30; c += 4) {
-          a = max3f(a, __uint_as_float(raw[32 * q4 + c]), __uint_as_float(raw[32 * q4 + c + 1]));
-          b2 = max3f(b2, __uint_as_float(raw[32 * q4 + c + 2]), __uint_as_float(raw[32 * q4 + c + 3]));
-        }
-        a = max3f(a, __uint_as_float(raw[32 * q4 + 30]), __uint_as_float(raw[32 * q4 + 31]));
-        top = fmaxf(top, fmaxf(a, b2) * cg[q4]);
+        top4[q4][0] = fmaxf(__uint_as_float(raw[32 * q4]), __uint_as_float(raw[32 * q4 + 1]));
+        top4[q4][1] = fmaxf(__uint_as_float(raw[32 * q4 + 2]), __uint_as_float(raw[32 * q4 + 3]));
       }
-      int fnew = frun;
+#pragma unroll
+      for (int c = 4; c < 32; c += 4)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          top4[q4][0] = max3f(top4[q4][0], __uint_as_float(raw[32 * q4 + c]), __uint_as_float(raw[32 * q4 + c + 1]));
+          top4[q4][1] = max3f(top4[q4][1], __uint_as_float(raw[32 * q4 + c + 2]), __uint_as_float(raw[32 * q4 + c + 3]));
+        }
+      float top;
       if constexpr (KV4) {
-        fnew = max(max(fg[0], fg[1]), max(fg[2], fg[3]));
-        if (done > 0) fnew = max(fnew, frun);
+        top = fmaxf(fmaxf(fmaxf(top4[0][0], top4[0][1]) * cg[0], fmaxf(top4[1][0], top4[1][1]) * cg[1]),
+                    fmaxf(fmaxf(top4[2][0], top4[2][1]) * cg[2], fmaxf(top4[3][0], top4[3][1]) * cg[3]));
+      } else {
+        top = max3f(max3f(top4[0][0], top4[0][1], top4[1][0]), max3f(top4[1][1], top4[2][0], top4[2][1]),
+                    fmaxf(top4[3][0], top4[3][1])) * c_row;
       }
-      const bool grow = top > m + kLazy;
-      if (__any_sync(0xffffffffu, grow) || fnew != frun) {
-        const float mn = grow ? top : m;
-        const float alpha = grow ? exp2_fast(m - mn) : 1.f;
-        m = mn;
-        l *= alpha;
-        if (done > 0) {
-          const float by = KV4 ? alpha * __uint_as_float(uint32_t(127 + max(-126, frun - fnew)) << 23) : alpha;
-          const uint64_t by2 = pk2f(by, by);
-#pragma unroll 1
-          for (int cc = 0; cc < D / 32; ++cc) {
-            uint32_t o[32];
-            tmem_ld32(ocol + cc * 32, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) up2(f2_mul(pk2(o[2 * i], o[2 * i + 1]), by2), o[2 * i], o[2 * i + 1]);
-            tmem_st32(ocol + cc * 32, o);
-          }
-        }
+      float by = 1.f;   // what O has to be multiplied by
+      if constexpr (KV4) {
+        int fnew = max(max(fg[0], fg[1]), max(fg[2], fg[3]));
+        if (done > 0) fnew = max(fnew, frun);
+        if (fnew != frun) by = __uint_as_float(uint32_t(127 + max(-126, frun - fnew)) << 23);
         frun = fnew;
+      }
+      if (top > m + kLazy) {
+        const float alpha = exp2_fast(m - top);
+        m = top;
+        l *= alpha;
+        by *= alpha;
+      }
+      if (done > 0 && __any_sync(0xffffffffu, by != 1.f)) {
+        const uint64_t by2 = pk2f(by, by);
+#pragma unroll 1
+        for (int cc = 0; cc < D / 32; ++cc) {
+          uint32_t o[32];
+          tmem_ld32(ocol + cc * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) up2(f2_mul(pk2(o[2 * i], o[2 * i + 1]), by2), o[2 * i], o[2 * i + 1]);
+          tmem_st32(ocol + cc * 32, o);
+        }
       }
       const float mneg = m == -INFINITY ? 0.f : -m;
       uint32_t pw[64];
+      auto half = [&](int h) {
 #pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const float shift = KV4 ? static_cast<float>(max(-126, fg[q4] - frun)) : 0.f;
-        const uint64_t c2 = pk2f(cg[q4], cg[q4]), n2 = pk2f(mneg + shift, mneg + shift);
-        uint64_t sum2 = pk2f(0.f, 0.f);
+        for (int q4 = 2 * h; q4 < 2 * h + 2; ++q4) {
+          const float shift = KV4 ? static_cast<float>(max(-126, fg[q4] - frun)) : 0.f;
+          const uint64_t c2 = pk2f(cg[q4], cg[q4]), n2 = pk2f(mneg + shift, mneg + shift);
+          uint64_t sum2[2] = {0, 0};   // bits of (0.f, 0.f)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+          for (int i8 = 0; i8 < 16; i8 += 8) {   // eight pairs: kPoly of them by polynomial, side by side
+            uint32_t e[16];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              up2(f2_fma(pk2(raw[32 * q4 + 2 * (i8 + i)], raw[32 * q4 + 2 * (i8 + i) + 1]), c2, n2), e[2 * i], e[2 * i + 1]);
+#pragma unroll
+            for (int i = 2 * C::kPoly; i < 16; ++i) e[i] = __float_as_uint(exp2_fast(__uint_as_float(e[i])));
+            exp2_fma<C::kPoly>(e);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              sum2[i & 1] = f2_add(sum2[i & 1], pk2(e[2 * i], e[2 * i + 1]));
+              pw[16 * q4 + i8 + i] = pack2<T>(__uint_as_float(e[2 * i]), __uint_as_float(e[2 * i + 1]));
+            }
+          }
           uint32_t a, d;
-          up2(f2_fma(pk2(raw[32 * q4 + 2 * i], raw[32 * q4 + 2 * i + 1]), c2, n2), a, d);
-          const float ea = exp2_fast(__uint_as_float(a)), ed = exp2_fast(__uint_as_float(d));
-          sum2 = f2_add(sum2, pk2f(ea, ed));
-          pw[16 * q4 + i] = pack2<T>(ea, ed);
+          up2(f2_add(sum2[0], sum2[1]), a, d);
+          const float s = __uint_as_float(a) + __uint_as_float(d);
+          l += KV4 ? s * exp2_fast(-shift) : s;
         }
-        uint32_t a, d;
-        up2(sum2, a, d);
-        const float s = __uint_as_float(a) + __uint_as_float(d);
-        l += KV4 ? s * exp2_fast(-shift) : s;
-      }
+      };
+      half(0);
+      half(1);
       tmem_st32(scol, *reinterpret_cast<uint32_t(*)[32]>(pw));
       tmem_st32(scol + 32, *reinterpret_cast<uint32_t(*)[32]>(pw + 32));
       tmem_wait_st();
@@ -678,7 +712,8 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
     if (ok && done > 0) ok = mbar_wait_warp(&ctl->o_final[x], 0, kErrTimeoutSoftmax);
     if (ok) {
       tc_fence_after();
-      const bool seen = row < live && done > 0 && !(l == 0.f);
+      // (hidden keys leave traces of 2^-125 in l, so the maximum tells whether a row saw any; NaN logits leave it alone)
+      const bool seen = row < live && done > 0 && (m > -INFINITY || l != l);
       const float unit = KV4 ? __uint_as_float(uint32_t(127 + max(-126, frun)) << 23) : 1.f;
       const float inv = seen ? (p.splits == 1 ? unit / l : unit) : 0.f;
       const int64_t at = (int64_t(bh) * p.rows + row) * p.splits + split;
@@ -712,9 +747,9 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
         __syncwarp();
 #pragma unroll 2
         for (int i = 0; i < 32 / kRowsAt; ++i) {
-          const int lr = i * kRowsAt + rl, r = row0 + lr, rt = r / p.G, rh = hk * p.G + (r - rt * p.G);
+          const int lr = i * kRowsAt + rl, r = row0 + lr, rt = __shfl_sync(0xffffffffu, tok, lr), rh = hk * p.G + (r - rt * p.G);
           const uint4 u = *reinterpret_cast<const uint4*>(tile_mem + (ch >> 3) * kSeg + swizzled((warp & 3) * 32 + lr, ch & 7));
-          if (r < p.rows) *reinterpret_cast<uint4*>(static_cast<QT*>(p.out) + b * p.osb + rh * p.osh + rt * p.oss + ch * 8) = u;
+          if (r < p.rows) *reinterpret_cast<uint4*>(static_cast<QT*>(p.out) + int64_t(b) * p.osb + rh * p.osh + rt * p.oss + ch * 8) = u;
         }
       }
       if (p.splits > 1 && row < p.rows) p.part_ml[at] = seen ? make_float2(m, l) : make_float2(-INFINITY, 0.f);

@@ -36,7 +36,7 @@ bool make_map(CUtensorMap* m, const void* base, int dtype, int64_t B, int64_t H,
 
 TilePlan plan_of(const WindowAttnArgs& a) {
   const int64_t G = a.Hq / a.Hkv;
-  return tile_plan(a.B * a.Hkv, a.Sq * G, G, a.Sk, Visibility{a.window, a.sinks, a.causal});
+  return tile_plan(a.B * a.Hkv, a.Sq * G, G, a.Sk, visibility(a.window, a.sinks, a.causal));
 }
 
 }  // namespace
@@ -70,7 +70,7 @@ int window_attention(const WindowAttnArgs& a, cudaStream_t st) {
   p.rows = static_cast<int>(a.Sq * p.G);
   p.pairs = static_cast<int>(t.pairs);
   p.splits = static_cast<int>(t.splits);
-  p.vis = Visibility{a.window, a.sinks, a.causal};
+  p.vis = visibility(a.window, a.sinks, a.causal);
   p.scale_log2 = a.sm_scale * kLog2e;
   p.lengths = a.kv_lengths;
   p.part_o = static_cast<float*>(a.workspace);
