@@ -158,8 +158,8 @@ int check_visibility(const char* fn, int64_t window, int64_t sinks, float sm_sca
 }
 
 int check_workspace(const char* fn, const void* workspace, int64_t have, int64_t need) {
-  if (need > 0 && (!workspace || have < need || !aligned16(workspace))) {
-    set_last_error("%s: workspace needs %lld bytes (16-byte aligned)", fn, (long long)need);
+  if (need > 0 && (!workspace || have < need || (reinterpret_cast<uintptr_t>(workspace) & 127u))) {
+    set_last_error("%s: workspace needs %lld bytes (128-byte aligned)", fn, (long long)need);
     return VC_ERR_WORKSPACE;
   }
   return VC_OK;

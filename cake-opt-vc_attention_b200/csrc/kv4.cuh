@@ -33,6 +33,7 @@ struct Kv4Pages {
   const int32_t* table;     // [B, width]
   int64_t width, pages, heads;
   int page_size, page_shift;   // page_size = 1 << page_shift, at least 16
+  int most;                    // no sequence is longer: the table's width, or the caller's bound
 
   // Byte offset of the record that holds tokens 16*blk .. 16*blk+15 of
   // sequence b and head h, or -1.
@@ -48,8 +49,14 @@ struct Kv4Pages {
   }
 };
 
-inline Kv4Pages kv4_pages(const Kv4CacheArgs& c) {
-  Kv4Pages g{c.pool, c.table, c.width, c.pages, c.Hkv, static_cast<int>(c.page_size), 0};
+// The longest sequence that a call may meet.
+inline int64_t kv4_most(const Kv4CacheArgs& c, int64_t max_length) {
+  const int64_t tokens = c.width * c.page_size;
+  return max_length > 0 && max_length < tokens ? max_length : tokens;
+}
+
+inline Kv4Pages kv4_pages(const Kv4CacheArgs& c, int64_t max_length = 0) {
+  Kv4Pages g{c.pool, c.table, c.width, c.pages, c.Hkv, static_cast<int>(c.page_size), 0, static_cast<int>(kv4_most(c, max_length))};
   while ((int64_t(1) << g.page_shift) < c.page_size) ++g.page_shift;
   return g;
 }
@@ -58,10 +65,9 @@ inline Kv4Pages kv4_pages(const Kv4CacheArgs& c) {
 __device__ __forceinline__ void kv4_sequence(const Kv4Pages& pages, const int32_t* lengths, const int32_t* q_lengths,
                                              int Sq, int64_t b, int& len, int& nq) {
   len = __ldg(lengths + b);
-  const int most = static_cast<int>(pages.width) << pages.page_shift;
-  if (len < 0 || len > most) {
+  if (len < 0 || len > pages.most) {
     if (threadIdx.x == 0) raise_error(kErrBadIndex);
-    len = len < 0 ? 0 : most;
+    len = len < 0 ? 0 : pages.most;
   }
   nq = q_lengths ? max(0, min(__ldg(q_lengths + b), Sq)) : Sq;
 }

@@ -528,8 +528,7 @@ Plan plan_of(const Kv4AttnArgs& a) {
   Plan r;
   r.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
   r.blocks = static_cast<int>((rows + 8 * r.nt - 1) / (8 * r.nt));
-  int64_t keys = a.cache.width * a.cache.page_size;
-  if (a.max_length > 0) keys = min64(keys, a.max_length);
+  int64_t keys = kv4_most(a.cache, a.max_length);
   if (a.window > 0) keys = min64(keys, a.window + a.Sq + a.sinks + 2 * kTile);
   const int64_t tiles = (keys + kTile - 1) / kTile, items = a.cache.B * a.cache.Hkv * r.blocks;
   int64_t s = (4 * 148 + items - 1) / items;
@@ -585,7 +584,7 @@ int kv4_attention(const Kv4AttnArgs& a, cudaStream_t st) {
   p.osb = a.osb; p.osh = a.osh; p.oss = a.oss;
   p.lengths = a.lengths;
   p.q_lengths = a.q_lengths;
-  p.pages = kv4_pages(a.cache);
+  p.pages = kv4_pages(a.cache, a.max_length);
   p.Hq = a.Hq;
   p.Sq = a.Sq;
   p.G = static_cast<int>(a.Hq / a.cache.Hkv);

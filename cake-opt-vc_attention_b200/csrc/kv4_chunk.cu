@@ -1,26 +1,204 @@
-// Chunks of queries over the 4-bit cache: dispatch of the tile kernel
-// (tile_attention.cuh) with its dequantising producers.
+// Many rows a K/V head over the 4-bit cache: the tile kernel
+// (tile_attention.cuh), either with its own dequantising warps or after the
+// visible part of the cache has been unpacked to FP16 tiles.
+//
+// Every CTA (256 rows) reads all keys of its head, so with several CTAs a head
+// the dequantising warps of each do the same work again, and they take issue
+// slots from the softmax: the chunk of 1024 tokens over 16384 (28/4 heads,
+// D 128; 28 CTAs a head) takes 396 us that way and KUNPACKED us unpacked first,
+// of which the unpacking is KUNPACK.  So: unpack when a head has two CTAs or
+// more and the FP16 tiles fit kMostUnpacked bytes; the workspace is otherwise
+// only needed for split keys.
 #include "tile_attention.cuh"
 
 namespace vcb {
 namespace {
 
-TilePlan plan_of(const Kv4AttnArgs& a) {
-  const int64_t G = a.Hq / a.cache.Hkv;
-  int64_t keys = a.cache.width * a.cache.page_size;
-  if (a.max_length > 0) keys = min64(keys, a.max_length);
-  return tile_plan(a.cache.B * a.cache.Hkv, a.Sq * G, G, keys, visibility(a.window, a.sinks, a.causal));
+constexpr int64_t kMostUnpacked = int64_t(1) << 30;
+
+struct ChunkPlan {
+  TilePlan tiles;
+  int64_t slots = 0;        // unpacked tiles a K/V head, 0: not unpacked
+  int64_t tile_bytes = 0;   // of K (and of V)
+  int64_t meta_bytes = 0, bytes = 0;
+};
+
+ChunkPlan plan_of(const Kv4AttnArgs& a) {
+  ChunkPlan r;
+  const int64_t G = a.Hq / a.cache.Hkv, BH = a.cache.B * a.cache.Hkv;
+  const int64_t keys = kv4_most(a.cache, a.max_length);
+  const Visibility v = visibility(a.window, a.sinks, a.causal);
+  r.tiles = tile_plan(BH, a.Sq * G, G, keys, v);
+  // the tiles that some row sees: those of the sinks and, under a window, at most ceil((window + Sq - 1) / 128) + 1
+  int64_t slots = (keys + 127) / 128;
+  if (v.window > 0) slots = min64(slots, (int64_t(v.sinks) + 127) / 128 + (int64_t(v.window) + a.Sq + 126) / 128 + 1);
+  const int64_t each = BH * slots * 128 * a.D * 2;
+  if (r.tiles.pairs >= 2 && slots > 0 && 2 * each <= kMostUnpacked) {
+    r.slots = slots;
+    r.tile_bytes = each;
+    r.meta_bytes = (BH * slots * int64_t(sizeof(TileMeta)) + 127) / 128 * 128;
+  }
+  r.bytes = 2 * r.tile_bytes + r.meta_bytes;
+  if (r.tiles.splits > 1) r.bytes += a.cache.B * a.Hq * a.Sq * r.tiles.splits * (a.D + 2) * 4;
+  return r;
+}
+
+struct UnpackParams {
+  Kv4Pages pages;
+  const int32_t *lengths, *q_lengths;
+  int Sq, slots;
+  Visibility vis;
+  uint8_t *k, *v;      // FP16 [BH, slots * 128, D]
+  TileMeta* meta;      // [BH, slots]
+};
+
+// One CTA unpacks one tile of 128 keys: first a thread a key finds the tile's
+// largest magnitudes and the keys that are missing or not finite, then 16 bytes
+// of codes (32 channels, 64 bytes of FP16) a thread and turn.
+template <int D>
+__global__ void __launch_bounds__(256) kv4_unpack_kernel(UnpackParams p) {
+  using R = Kv4Rec<D>;
+  constexpr int kPer = D / 32;   // threads a key
+  __shared__ int64_t rec[8];
+  __shared__ uint32_t top[2][8], state[3][4];   // largest magnitude by warp; cleared K, V group 0, V group 1
+  const int bh = blockIdx.y, b = bh / static_cast<int>(p.pages.heads), hk = bh % static_cast<int>(p.pages.heads);
+  int len, nq;
+  kv4_sequence(p.pages, p.lengths, p.q_lengths, p.Sq, b, len, nq);
+  const UnpackedTiles un = unpacked_tiles(p.vis, len, nq);
+  const int slot = blockIdx.x, tile = slot < un.sink ? slot : un.base + (slot - un.sink);
+  if (tile >= un.end) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x < 8) {
+    const int blk = tile * 8 + threadIdx.x;
+    int64_t at = -1;   // past the end
+    if (int64_t(blk) * kKv4Block < len) {
+      at = p.pages.record<D>(b, hk, blk);
+      if (at < 0) {
+        raise_error(kErrBadIndex);
+        at = -2;
+      }
+    }
+    rec[threadIdx.x] = at;
+  }
+  __syncthreads();
+  TileMeta* meta = p.meta + int64_t(bh) * p.slots + slot;
+  // warps 0-3: K of 32 keys each, warps 4-7: V
+  const int key = threadIdx.x & 127, is_v = threadIdx.x >> 7;
+  const int64_t at = rec[key >> 4];
+  uint32_t sm[2] = {0, 0};
+  const bool ended = at == -1 || tile * 128 + key >= len, lost = at == -2 && !ended;
+  if (at >= 0) {
+    const uint8_t* par = p.pages.pool + at + (is_v ? R::kVp : R::kKp) + (key & 15) * R::kParRow;
+#pragma unroll
+    for (int g = 0; g < D / 64; ++g) sm[g] = __ldg(reinterpret_cast<const uint32_t*>(par) + g);
+    if constexpr (D == 64) sm[1] = sm[0];
+  }
+  const bool gone = ended || lost;
+  bool fine[2];
+  float big = 0.f;
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    fine[g] = fabsf(bf16_lo(sm[g])) < INFINITY && fabsf(bf16_hi(sm[g])) < INFINITY;
+    const float m = fmaxf(fabsf(bf16_hi(sm[g])), fabsf(fmaf(15.f, bf16_lo(sm[g]), bf16_hi(sm[g]))));
+    if (!gone && m < INFINITY) big = fmaxf(big, m);
+  }
+  const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
+  const uint32_t clear = __ballot_sync(0xffffffffu, gone), miss = __ballot_sync(0xffffffffu, lost);
+  const uint32_t bad0 = __ballot_sync(0xffffffffu, !gone && !fine[0]), bad1 = __ballot_sync(0xffffffffu, !gone && !fine[1]);
+  if (lane == 0) {
+    top[is_v][warp & 3] = most;
+    if (is_v) {
+      state[1][warp & 3] = clear | bad0;
+      state[2][warp & 3] = clear | bad1;
+      meta->bad[0][warp & 3] = bad0;
+      meta->bad[1][warp & 3] = bad1;
+      top[1][4 + (warp & 3)] = bad0 | bad1;
+    } else {
+      state[0][warp & 3] = clear;
+      meta->miss[warp & 3] = miss;
+      top[0][4 + (warp & 3)] = miss;
+    }
+  }
+  __syncthreads();
+  float down[2];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const uint32_t bits = max(max(top[w][0], top[w][1]), max(top[w][2], top[w][3]));
+    const int te = static_cast<int>(bits >> 23) - 127;   // the maximum lies in [2^te, 2^(te+1))
+    const int e = bits == 0u || (te >= -8 && te <= 14) ? 0 : te > 14 ? te - 14 : max(te, -60);
+    down[w] = __uint_as_float(uint32_t(127 - e) << 23);
+    if (threadIdx.x == 0) meta->e[w] = e;
+  }
+  if (threadIdx.x == 0) {
+    uint32_t any = 0;
+    for (int w = 0; w < 2; ++w)
+      for (int i = 4; i < 8; ++i) any |= top[w][i];
+    meta->e[2] = any != 0;
+  }
+  const __half2 minus1024 = __float2half2_rn(-1024.f), sixteenth = __float2half2_rn(0.0625f), minus64 = __float2half2_rn(-64.f);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int u = i * 256 + threadIdx.x, w = u / (128 * kPer), k = u / kPer & 127, q = u % kPer;
+    const int64_t r = rec[k >> 4];
+    uint4 codes = make_uint4(0, 0, 0, 0);
+    uint32_t ms = 0;
+    const bool hide = (state[w == 0 ? 0 : 1 + (D == 128 ? q >> 1 : 0)][k >> 5] >> (k & 31)) & 1u;
+    if (r >= 0 && !hide) {
+      const uint8_t* base = p.pages.pool + r;
+      codes = __ldg(reinterpret_cast<const uint4*>(base + (w ? R::kV : R::kK) + (k & 15) * R::kCodeRow + q * 16));
+      ms = __ldg(reinterpret_cast<const uint32_t*>(base + (w ? R::kVp : R::kKp) + (k & 15) * R::kParRow + (D == 128 ? (q >> 1) * 4 : 0)));
+    }
+    const __half2 s2 = __float2half2_rn(bf16_lo(ms) * down[w]), m2 = __float2half2_rn(bf16_hi(ms) * down[w]);
+    uint8_t* dst = (w ? p.v : p.k) + ((int64_t(bh) * p.slots + slot) * 128 + k) * (D * 2) + q * 64;
+    const uint32_t cw[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t c0 = cw[j], c8 = c0 >> 8;
+      uint32_t x[4] = {(c0 & 0x000F000Fu) | 0x64006400u, (c0 & 0x00F000F0u) | 0x64006400u,
+                       (c8 & 0x000F000Fu) | 0x64006400u, (c8 & 0x00F000F0u) | 0x64006400u};
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        __half2 v = *reinterpret_cast<__half2*>(&x[h]);
+        v = (h & 1) ? __hfma2(v, sixteenth, minus64) : __hadd2(v, minus1024);   // the code, exactly
+        v = __hfma2(v, s2, m2);
+        x[h] = *reinterpret_cast<uint32_t*>(&v);
+      }
+      // channels 8a + {0,4,1,5,2,6,3,7}, as the tile kernel stores Q and writes O
+      reinterpret_cast<uint4*>(dst)[j] = make_uint4(x[0], x[1], x[2], x[3]);
+    }
+  }
+}
+
+template <int D, typename QT>
+int run(const Kv4AttnArgs& a, const ChunkPlan& plan, TileParams& p, cudaStream_t st) {
+  if (plan.slots == 0) {
+    const CUtensorMap none{};   // K and V come from the cache's records
+    return launch_tiles<D, __half, QT, kRecords>(none, none, p, st);
+  }
+  uint8_t* k = static_cast<uint8_t*>(a.workspace);
+  uint8_t* v = k + plan.tile_bytes;
+  TileMeta* meta = reinterpret_cast<TileMeta*>(v + plan.tile_bytes);
+  const UnpackParams u{p.pages, a.lengths, a.q_lengths, p.Sq, static_cast<int>(plan.slots), p.vis, k, v, meta};
+  kv4_unpack_kernel<D><<<dim3(static_cast<unsigned>(plan.slots), static_cast<unsigned>(p.BH)), 256, 0, st>>>(u);
+  if (cudaGetLastError() != cudaSuccess) return VC_ERR_LAUNCH;
+  CUtensorMap mk, mv;
+  const int64_t S = plan.slots * 128, H = a.cache.Hkv;
+  if (!make_map(&mk, k, VC_DTYPE_F16, a.cache.B, H, S, D, H * S * D, S * D, D) ||
+      !make_map(&mv, v, VC_DTYPE_F16, a.cache.B, H, S, D, H * S * D, S * D, D)) {
+    set_last_error("vc_kv4_attention_fwd: cuTensorMapEncodeTiled failed");
+    return VC_ERR_LAUNCH;
+  }
+  p.meta = meta;
+  p.slots = static_cast<int>(plan.slots);
+  return launch_tiles<D, __half, QT, kUnpacked>(mk, mv, p, st);
 }
 
 }  // namespace
 
-int64_t kv4_chunk_workspace(const Kv4AttnArgs& a) {
-  const TilePlan t = plan_of(a);
-  return t.splits == 1 ? 0 : a.cache.B * a.Hq * a.Sq * t.splits * (a.D + 2) * 4;
-}
+int64_t kv4_chunk_workspace(const Kv4AttnArgs& a) { return plan_of(a).bytes; }
 
 int kv4_chunk_attention(const Kv4AttnArgs& a, cudaStream_t st) {
-  const TilePlan t = plan_of(a);
+  const ChunkPlan plan = plan_of(a);
   TileParams p{};
   p.q = a.q;
   p.out = a.out;
@@ -28,24 +206,20 @@ int kv4_chunk_attention(const Kv4AttnArgs& a, cudaStream_t st) {
   p.osb = a.osb; p.osh = a.osh; p.oss = a.oss;
   p.Hkv = static_cast<int>(a.cache.Hkv);
   p.BH = static_cast<int>(a.cache.B * a.cache.Hkv);
-  p.Sq = a.Sq;
+  p.Sq = static_cast<int>(a.Sq);
   p.G = static_cast<int>(a.Hq / a.cache.Hkv);
-  p.rows = static_cast<int>(a.Sq * p.G);
-  p.pairs = static_cast<int>(t.pairs);
-  p.splits = static_cast<int>(t.splits);
+  p.rows = p.Sq * p.G;
+  p.pairs = static_cast<int>(plan.tiles.pairs);
+  p.splits = static_cast<int>(plan.tiles.splits);
   p.vis = visibility(a.window, a.sinks, a.causal);
   p.scale_log2 = a.sm_scale * kLog2e;
   p.lengths = a.lengths;
   p.q_lengths = a.q_lengths;
-  p.pages = kv4_pages(a.cache);
-  p.part_o = static_cast<float*>(a.workspace);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + int64_t(p.BH) * p.rows * t.splits * a.D);
-  const CUtensorMap none{};   // K/V come from the cache's records
-  if (a.dtype == VC_DTYPE_BF16)
-    return a.D == 128 ? launch_tiles<128, __half, __nv_bfloat16, true>(none, none, p, st)
-                      : launch_tiles<64, __half, __nv_bfloat16, true>(none, none, p, st);
-  return a.D == 128 ? launch_tiles<128, __half, __half, true>(none, none, p, st)
-                    : launch_tiles<64, __half, __half, true>(none, none, p, st);
+  p.pages = kv4_pages(a.cache, a.max_length);
+  p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + 2 * plan.tile_bytes + plan.meta_bytes);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + int64_t(p.BH) * p.rows * p.splits * a.D);
+  if (a.dtype == VC_DTYPE_BF16) return a.D == 128 ? run<128, __nv_bfloat16>(a, plan, p, st) : run<64, __nv_bfloat16>(a, plan, p, st);
+  return a.D == 128 ? run<128, __half>(a, plan, p, st) : run<64, __half>(a, plan, p, st);
 }
 
 cudaError_t kv4_chunk_error_word(uint32_t* code, bool clear) { return read_tu_error_word(code, clear); }

@@ -46,6 +46,56 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;
 
+// Where K and V come from: 16-bit tensors, the 4-bit cache's records
+// (dequantised by four warps of every CTA), or the cache unpacked to FP16 tiles
+// beforehand (kv4_chunk.cu).
+enum KvSource { kTensors, kRecords, kUnpacked };
+
+template <int D, KvSource SRC>
+struct TileCfg {
+  static constexpr bool KV4 = SRC == kRecords;
+  static constexpr int kThreads = KV4 ? 512 : 384;
+  static constexpr int kTile = 128 * D * 2;                  // bytes of a K, V or Q tile
+  static constexpr int kKS = KV4 ? 2 : D == 128 ? 3 : 4;     // K ring
+  static constexpr int kVS = KV4 ? 2 : D == 128 ? 2 : 4;     // V ring
+  static constexpr int kRS = KV4 ? 3 : 0;                    // ring of raw half tiles (64 keys)
+  static constexpr int kPoly = SRC == kRecords ? 0 : 2;   // of eight pairs of exponentials, on the FMA pipe
+  static constexpr int kRaw = 4 * Kv4Rec<D>::kBytes;
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffK = kOffQ + 2 * kTile;
+  static constexpr int kOffV = kOffK + kKS * kTile;
+  static constexpr int kOffRaw = kOffV + kVS * kTile;
+  static constexpr int kOffCtl = kOffRaw + kRS * kRaw;
+};
+
+// What was found out about a key tile while it was dequantised (4-bit cache).
+// Unpacked tiles have one exponent each for K and V: e[0] and e[1], and e[2]
+// tells whether any bit of miss or bad is set.
+struct __align__(16) TileMeta {
+  int e[4], f[4];        // 2^e / 2^f: what the 32-key groups of K / V were divided by
+  uint32_t miss[4];      // keys without a page
+  uint32_t bad[2][4];    // keys whose V (64-channel group) is not finite
+};
+
+// Which unpacked tile holds a sequence's key tile: only those that the call's
+// rows see are unpacked, the sinks' first.
+struct UnpackedTiles {
+  int sink, base;   // tiles [0, sink), then [base, end)
+  int end;
+  __device__ __forceinline__ int slot(int tile) const { return tile < sink ? tile : sink + (tile - base); }
+};
+__device__ __forceinline__ UnpackedTiles unpacked_tiles(const Visibility& v, int len, int nq) {
+  UnpackedTiles u{0, 0, 0};
+  if (nq <= 0) return u;
+  const KeyRanges a = visible_keys(v, len - nq, len), z = visible_keys(v, len - 1, len);
+  u.end = (z.hi + 127) >> 7;
+  if (v.window) {
+    u.base = a.lo >> 7;
+    u.sink = min((min(v.sinks, z.hi) + 127) >> 7, u.base);
+  }
+  return u;
+}
+
 struct TileParams {
   const void* q;
   void* out;
@@ -57,31 +107,10 @@ struct TileParams {
   float scale_log2;            // sm_scale * log2(e)
   const int32_t *lengths, *q_lengths;
   Kv4Pages pages;              // 4-bit cache only
+  const TileMeta* meta;        // unpacked tiles: [BH, slots]
+  int slots;
   float* part_o;
   float2* part_ml;
-};
-
-template <int D, bool KV4>
-struct TileCfg {
-  static constexpr int kThreads = KV4 ? 512 : 384;
-  static constexpr int kTile = 128 * D * 2;                  // bytes of a K, V or Q tile
-  static constexpr int kKS = KV4 ? 2 : D == 128 ? 3 : 4;     // K ring
-  static constexpr int kVS = KV4 ? 2 : D == 128 ? 2 : 4;     // V ring
-  static constexpr int kRS = KV4 ? 3 : 0;                    // ring of raw half tiles (64 keys)
-  static constexpr int kPoly = KV4 ? 0 : 2;   // of eight pairs of exponentials, on the FMA pipe
-  static constexpr int kRaw = 4 * Kv4Rec<D>::kBytes;
-  static constexpr int kOffQ = 0;
-  static constexpr int kOffK = kOffQ + 2 * kTile;
-  static constexpr int kOffV = kOffK + kKS * kTile;
-  static constexpr int kOffRaw = kOffV + kVS * kTile;
-  static constexpr int kOffCtl = kOffRaw + kRS * kRaw;
-};
-
-// What the dequantising warps found out about a key tile (4-bit cache).
-struct TileMeta {
-  int e[4], f[4];        // 2^e / 2^f: what the 32-key groups of K / V were divided by
-  uint32_t miss[4];      // keys without a page
-  uint32_t bad[2][4];    // keys whose V (64-channel group) is not finite
 };
 
 struct __align__(16) TileCtl {
@@ -190,10 +219,11 @@ __device__ __forceinline__ GroupKeys group_keys(const Visibility& v, int base, i
   return k;
 }
 
-template <int D, typename T, typename QT, bool KV4>
-__global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
+template <int D, typename T, typename QT, KvSource SRC>
+__global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
     tile_attention_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, TileParams p) {
-  using C = TileCfg<D, KV4>;
+  using C = TileCfg<D, SRC>;
+  constexpr bool KV4 = SRC != kTensors, kDequant = SRC == kRecords;
   constexpr int kSegs = D / 64;
   constexpr int kSeg = 128 * 128;   // bytes of a 64-channel segment of a tile
   extern __shared__ uint8_t smem_raw[];
@@ -212,12 +242,12 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
   }
   if (threadIdx.x == 256) {
     for (int s = 0; s < 4; ++s) {
-      mbar_init(&ctl->k_full[s], KV4 ? 64 : 1);
+      mbar_init(&ctl->k_full[s], kDequant ? 64 : 1);
       mbar_init(&ctl->step_done[s], 1);
-      mbar_init(&ctl->v_full[s], KV4 ? 64 : 1);
-      if constexpr (KV4) mbar_init(&ctl->meta_full[s], 128);
+      mbar_init(&ctl->v_full[s], kDequant ? 64 : 1);
+      if constexpr (kDequant) mbar_init(&ctl->meta_full[s], 128);
     }
-    if constexpr (KV4) {
+    if constexpr (kDequant) {
       for (int s = 0; s < 3; ++s) {
         mbar_init(&ctl->raw_full[s], 1);
         mbar_init(&ctl->raw_empty[s], 4);
@@ -263,7 +293,7 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
     return i < nsink ? i : main0 + (i - nsink);
   };
 
-  if constexpr (!KV4) {
+  if constexpr (!kDequant) {
     if (warp == 8 && lane == 0) tma_prefetch_desc(&tmk);
     if (warp == 10 && lane == 0) tma_prefetch_desc(&tmv);
   }
@@ -273,7 +303,7 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
   const uint32_t tmem = ctl->slot;
 
   if (warp >= 8) {
-    if constexpr (KV4) setmaxnreg_dec<64>();
+    if constexpr (kDequant) setmaxnreg_dec<64>();
     else setmaxnreg_dec<88>();
     if (warp == 9) {
       // ------------------------------------------------------------- MMA issuer
@@ -330,7 +360,11 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
           if (x == 1 && n + 1 < steps) ok = mbar_wait_warp(&ctl->k_full[(n + 1) % C::kKS], ((n + 1) / C::kKS) & 1, kErrTimeoutMma);
         }
       }
-    } else if constexpr (!KV4) {
+    } else if constexpr (!kDequant) {
+      // (unpacked tiles: the row that TMA reads a key tile from)
+      UnpackedTiles un{};
+      if constexpr (SRC == kUnpacked) un = unpacked_tiles(p.vis, len, nq);
+      auto first_row = [&](int n) -> int { return (SRC == kUnpacked ? un.slot(tile_of(n)) : tile_of(n)) * 128; };
       if (warp == 8 && lane == 0) {
         // ----------------------------------------------------------- K producer
         for (int n = 0; n < steps; ++n) {
@@ -339,7 +373,7 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
           mbar_expect_tx(&ctl->k_full[s], C::kTile);
           for (int g = 0; g < kSegs; ++g)
             tma_load_4d(smem + C::kOffK + s * C::kTile + g * kSeg, &tmk, &ctl->k_full[s], g * 64,
-                        tile_of(n) * 128, static_cast<int>(hk), static_cast<int>(b));
+                        first_row(n), hk, b);
         }
       } else if (warp == 10) {
         // ----------------------------------------------------------- V producer
@@ -351,12 +385,12 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
           uint8_t* dst = smem + C::kOffV + s * C::kTile;
           // rows at and past the sequence's end hold whatever the tensor does: 0 x NaN would reach
           // every row, so they are cleared before the MMA sees them (past Sk, TMA itself fills zeros)
-          const bool fix = k0 + 128 > len && len < p.Sk;
+          const bool fix = SRC == kTensors && k0 + 128 > len && len < p.Sk;
           uint64_t* bar = fix ? &ctl->v_fix : &ctl->v_full[s];
           if (lane == 0) {
             mbar_expect_tx(bar, C::kTile);
             for (int g = 0; g < kSegs; ++g)
-              tma_load_4d(dst + g * kSeg, &tmv, bar, g * 64, k0, static_cast<int>(hk), static_cast<int>(b));
+              tma_load_4d(dst + g * kSeg, &tmv, bar, g * 64, first_row(n), hk, b);
           }
           __syncwarp();
           if (fix) {
@@ -508,7 +542,7 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
       }
     }
   } else {
-    if constexpr (KV4) setmaxnreg_inc<192>();
+    if constexpr (kDequant) setmaxnreg_inc<192>();
     else setmaxnreg_inc<208>();
     // ------------------------------------------------------------ softmax group X
     const int x = warp >> 2, t = threadIdx.x & 127;
@@ -576,23 +610,52 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
     uint32_t nan_out = 0;      // 4-bit cache: 64-channel groups of this row that saw a value that is not finite
     uint32_t done = 0;
     bool ok = true;
+    UnpackedTiles un{};
+    int4 next_meta = make_int4(0, 0, 0, 0);
+    if constexpr (SRC == kUnpacked) {
+      un = unpacked_tiles(p.vis, len, nq);
+      if (steps > 0) next_meta = __ldg(reinterpret_cast<const int4*>(p.meta + int64_t(bh) * p.slots + un.slot(tile_of(0))));
+    }
     for (int n = 0; n < steps; ++n) {
       const int tile = tile_of(n), k0 = tile * 128;
-      if (!g.sees(tile)) continue;
+      if (!g.sees(tile)) {
+        if (SRC == kUnpacked && n + 1 < steps)
+          next_meta = __ldg(reinterpret_cast<const int4*>(p.meta + int64_t(bh) * p.slots + un.slot(tile_of(n + 1))));
+        continue;
+      }
       float cg[4] = {c_row, c_row, c_row, c_row};
       int fg[4] = {0, 0, 0, 0};
       uint32_t miss[4] = {0, 0, 0, 0}, bad[2][4] = {};   // 4-bit cache: see TileMeta
       if constexpr (KV4) {
         const TileMeta* meta = &ctl->meta[n & 3];
-        ok = mbar_wait_warp(&ctl->meta_full[n & 3], (n >> 2) & 1, kErrTimeoutSoftmax);
-        if (!ok) break;
+        bool any = true;
+        if constexpr (kDequant) {
+          ok = mbar_wait_warp(&ctl->meta_full[n & 3], (n >> 2) & 1, kErrTimeoutSoftmax);
+          if (!ok) break;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          cg[i] = c_row * __uint_as_float(uint32_t(127 + meta->e[i]) << 23);
-          fg[i] = meta->f[i];
-          miss[i] = meta->miss[i];
-          bad[0][i] = meta->bad[0][i];
-          bad[1][i] = meta->bad[1][i];
+          for (int i = 0; i < 4; ++i) {
+            cg[i] = c_row * __uint_as_float(uint32_t(127 + meta->e[i]) << 23);
+            fg[i] = meta->f[i];
+          }
+        } else {
+          meta = p.meta + int64_t(bh) * p.slots + un.slot(tile);
+          const int4 now = next_meta;   // exponents of K and V, and whether anything else is to know
+          if (n + 1 < steps) next_meta = __ldg(reinterpret_cast<const int4*>(p.meta + int64_t(bh) * p.slots + un.slot(tile_of(n + 1))));
+          any = now.z != 0;
+          const float c = c_row * __uint_as_float(uint32_t(127 + now.x) << 23);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            cg[i] = c;
+            fg[i] = now.y;
+          }
+        }
+        if (any) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            miss[i] = meta->miss[i];
+            bad[0][i] = meta->bad[0][i];
+            bad[1][i] = meta->bad[1][i];
+          }
         }
       }
       ok = mbar_wait_warp(&ctl->s_full[x], done & 1, kErrTimeoutSoftmax);
@@ -764,6 +827,35 @@ __global__ void __launch_bounds__(TileCfg<D, KV4>::kThreads, 1)
   }
 }
 
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn get_encode() {
+  static EncodeFn fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+                    q == cudaDriverEntryPointSuccess;
+    return ok ? reinterpret_cast<EncodeFn>(ptr) : nullptr;
+  }();
+  return fn;
+}
+
+// [B, H, S, D] 16-bit tensor through its strides; boxes of 64 channels x 128 tokens.
+bool make_map(CUtensorMap* m, const void* base, int dtype, int64_t B, int64_t H, int64_t S, int64_t D, int64_t sb,
+              int64_t sh, int64_t ss) {
+  EncodeFn enc = get_encode();
+  if (!enc) return false;
+  const cuuint64_t dims[4] = {cuuint64_t(D), cuuint64_t(S), cuuint64_t(H), cuuint64_t(B)};
+  const cuuint64_t strides[3] = {cuuint64_t(ss) * 2, cuuint64_t(sh) * 2, cuuint64_t(sb) * 2};
+  const cuuint32_t box[4] = {64, 128, 1, 1}, estr[4] = {1, 1, 1, 1};
+  return enc(m, dtype == VC_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+             const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Pairs of 128-row tiles, and splits of their keys where the pairs alone would
 // leave SMs idle.  ``keys``: the most keys that one row's CTA can see.
 struct TilePlan {
@@ -780,10 +872,10 @@ inline TilePlan tile_plan(int64_t BH, int64_t rows, int64_t G, int64_t keys, con
   return r;
 }
 
-template <int D, typename T, typename QT, bool KV4>
+template <int D, typename T, typename QT, KvSource SRC>
 int launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, const TileParams& p, cudaStream_t st) {
-  auto* k = tile_attention_kernel<D, T, QT, KV4>;
-  using C = TileCfg<D, KV4>;
+  auto* k = tile_attention_kernel<D, T, QT, SRC>;
+  using C = TileCfg<D, SRC>;
   constexpr int bytes = C::kOffCtl + int(sizeof(TileCtl)) + 1024;
   static_assert(bytes <= 227 * 1024, "shared memory");
   static std::atomic<uint64_t> ready{0};

@@ -497,8 +497,10 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor,
     (``causal`` implies j <= i) and (no ``window``, or j > i - window, or
     j < ``sinks``).  Rows that see nothing, and rows past ``q_lengths[b]``, are
     zeros.  ``max_length`` (an upper bound of ``lengths``; default the page
-    table's width) only steers how long sequences are split.  Returns a new
-    tensor like ``q``, or ``out``.
+    table's width) sizes the workspace and the split of long sequences: give it
+    where the table is much wider than the sequences are long.  A sequence that
+    is longer is cut there (bit 0x80 of ``error_word``).  Returns a new tensor
+    like ``q``, or ``out``.
     """
     name = "kv4_attention"
     _serving(name, tensor_layout, q)

@@ -212,7 +212,7 @@ int vc_attention_fwd_e4m3qk(const uint8_t* q8, const float* qs, const uint8_t* k
  *   t, 64-channel group g at (t*D/64 + g)*4), [17D, 18D) V pairs.
  * value = scale * code + minimum.  page_size is 16, 32, 64, 128 or 256, D 64
  * or 128.  A page table entry outside [0, pages) for a token that a call has
- * to write or read, or a length past the table's width, sets bit 0x80 of the
+ * to write or read, or a length past the table's width or max_length, sets bit 0x80 of the
  * device error word; that token is not written, reads as zeros, and is not
  * attended to.  No counterpart in the reference, which keeps no cache.
  *
@@ -247,8 +247,9 @@ int vc_kv4_read(const uint8_t* pool, int64_t pages, int64_t page_size, const int
  * Sq) are the queries: query t is at position i = lengths[b] - q_lengths[b] + t
  * and sees key j iff j < lengths[b], (not causal or j <= i) and (window = 0 or
  * j > i - window or j < sinks).  Rows that see nothing, and rows t >=
- * q_lengths[b], are zeros.  max_length (at least every length; 0: the table's
- * width) only sizes the split of long sequences and the workspace. */
+ * q_lengths[b], are zeros.  max_length (0: the table's width) bounds the
+ * lengths: it sizes the split of long sequences and the workspace (which must
+ * be 128-byte aligned), and a longer sequence is cut there (bit 0x80). */
 int64_t vc_kv4_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D, int causal,
                                          int64_t window, int64_t sinks, int64_t page_size, int64_t table_width,
                                          int64_t max_length);
