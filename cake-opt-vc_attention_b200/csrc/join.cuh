@@ -45,42 +45,71 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// One warp a row, D/32 channels a lane.
+// One CTA a row, a warp for every eighth split (at most eight warps), D/32
+// channels a lane; the warps' sums are added in order.  Launched while the
+// kernel before it still runs (programmatic dependent launch), so that its
+// launch costs nothing: it waits for that kernel's results itself.
 template <int D, typename T>
-__global__ void __launch_bounds__(128) join_splits_kernel(JoinParams p, int64_t total) {
-  const int64_t i = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (i >= total) return;
+__global__ void __launch_bounds__(256) join_splits_kernel(JoinParams p) {
+  constexpr int C = D / 32;
+  __shared__ float part[8][D];
+  __shared__ float sums[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int64_t i = blockIdx.x;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const float2* ml = p.part_ml + i * p.splits;
   float top = -INFINITY;
   for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, ml[s].x);
 #pragma unroll
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  constexpr int C = D / 32;
   float v[C], sum = 0.f;
 #pragma unroll
   for (int k = 0; k < C; ++k) v[k] = 0.f;
   const float* src = p.part_o + i * p.splits * D + lane * C;
-  for (int s = 0; s < p.splits; ++s) {
+#pragma unroll 4
+  for (int s = warp; s < p.splits; s += warps) {
     const float2 a = ml[s];
     const float f = a.x == -INFINITY ? 0.f : exp2_fast(a.x - top);
     sum += a.x == -INFINITY ? a.y : a.y * f;   // without a maximum: 0, or NaN where every logit is
+    float x[C];
+    if constexpr (C == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src + s * D);
+    else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(src + s * D);
 #pragma unroll
-    for (int k = 0; k < C; ++k) v[k] += src[s * D + k] * f;
+    for (int k = 0; k < C; ++k) v[k] = fmaf(x[k], f, v[k]);
   }
-  const int row = static_cast<int>(i % p.rows);
-  const int64_t bh = i / p.rows, b = bh / p.heads, hk = bh % p.heads;
-  T h[C];
 #pragma unroll
-  for (int k = 0; k < C; ++k) h[k] = from_f32<T>(sum == 0.f ? 0.f : v[k] / sum);
-  T* dst = static_cast<T*>(p.out) + b * p.osb + (hk * p.G + row % p.G) * p.osh + int64_t(row / p.G) * p.oss + lane * C;
-  if constexpr (C == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(h);
-  else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(h);
+  for (int k = 0; k < C; ++k) part[warp][lane * C + k] = v[k];
+  if (lane == 0) sums[warp] = sum;
+  __syncthreads();
+  const int row = static_cast<int>(i % p.rows), tok = row / p.G;
+  const int64_t bh = i / p.rows, b = bh / p.heads, hk = bh % p.heads;
+  T* dst = static_cast<T*>(p.out) + b * p.osb + (hk * p.G + (row - tok * p.G)) * p.osh + int64_t(tok) * p.oss;
+  for (int d = threadIdx.x; d < D; d += blockDim.x) {
+    float o = 0.f, l = 0.f;
+    for (int w = 0; w < warps; ++w) {
+      o += part[w][d];
+      l += sums[w];
+    }
+    dst[d] = from_f32<T>(l == 0.f ? 0.f : o / l);
+  }
 }
 
+// Tells that the next kernel on the stream may be launched; it still waits for
+// this one's results.
+__device__ __forceinline__ void allow_dependent_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 template <int D, typename T>
-inline void launch_join(const JoinParams& p, int64_t total, cudaStream_t st) {
-  join_splits_kernel<D, T><<<static_cast<unsigned>((total + 3) / 4), 128, 0, st>>>(p, total);
+inline cudaError_t launch_join(const JoinParams& p, int64_t total, cudaStream_t st) {
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(static_cast<unsigned>(total));
+  c.blockDim = dim3(32 * (p.splits >= 8 ? 8 : p.splits));
+  c.stream = st;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &early;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, join_splits_kernel<D, T>, p);
 }
 
 }  // namespace vcb

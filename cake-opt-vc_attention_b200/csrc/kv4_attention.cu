@@ -3,33 +3,37 @@
 //
 // One CTA takes up to 8*NT rows (query tokens x the query heads that share a
 // K/V head) of one sequence and K/V head, and a share of its keys; each of its
-// eight warps streams tiles of 32 keys on its own, with its own running
-// maximum, and the warps (then the splits, in a second kernel) are joined at
-// the end.
+// warps streams tiles of 32 keys on its own, with its own running maximum, and
+// the warps (then the splits, in a second kernel) are joined at the end.
 //
-// Memory-bound by design: a tile is two records of 18*D bytes (K and V codes
-// with their scales), each brought by one bulk copy into the warp's ring of
-// shared-memory stages, so page sizes and alignment do not matter and
-// 8 warps x 3 tiles a CTA keep about 200 KB an SM in flight.
-//
-// The codes go to the tensor core as integers; no value is dequantised:
+// A tile is two records of 18*D bytes (K and V codes with their scales), each
+// brought by one bulk copy into the warp's ring of shared-memory stages, so
+// page sizes and alignment do not matter and 16 warps x 3 tiles an SM keep
+// about 200 KB in flight.  What bounds it then is not memory but the integer
+// pipe that takes the nibbles apart (ALU_SHARE), so everything here saves such
+// instructions:
+//   The codes go to the tensor core as integers; no value is dequantised.  A
+//   nibble in the low byte of a 16-bit lane is the FP16 denormal u 2^-24 (16 u
+//   2^-24 in the high nibble), so one AND makes an operand register of two
+//   codes, exactly, and one shift serves two of them.
 //   S^T = K Q^T   A = K codes (m = key), B = Q (n = row).  x = s u + m gives
 //     q.k = sum_g s_g (q.u)_g + m_g (sum q)_g over the groups of 64 channels.
-//     A nibble in the low byte of a 16-bit lane is the FP16 denormal u 2^-24
-//     (or 16 u 2^-24 in the high nibble: that Q operand is divided by 16), so
-//     one AND makes an operand register, exactly.  Q is scaled by a power of
-//     two per row so that it fits FP16 whatever its range (BF16 has fewer
-//     significant bits, so this too is exact except for channels 2^-28 below
-//     the row's largest).  FP32 accumulation of exact products.
-//   O^T = V^T P^T  A = V codes (m = channel) as BF16 128 + u (exact), B = p s_g
-//     split into BF16 hi + lo (17 bits), so O is as good as FP32 arithmetic for
-//     both input types; sum_j p_j (m - 128 s)_jg is accumulated in FP32 beside
-//     it.  BF16 and not FP16 because p s has the range of the data.
+//     Q is scaled by a power of two per row so that it fits FP16 whatever its
+//     range (BF16 has fewer significant bits, so this is exact except for
+//     channels 2^-28 below the row's largest), and by 1/16 where it meets a
+//     high nibble.  Exact products, FP32 sums.
+//   O^T = V^T P^T  A = V codes (m = channel), two keys' words merged by byte
+//     permutes; B = p s_g 2^-e_g in FP16 (11 significant bits), where 2^e_g
+//     follows the largest scale met so far by steps (sum_j p_j m_jg is
+//     accumulated in FP32 beside it).
 //   S^T's accumulator layout becomes P^T's operand layout by one 8x8 transpose
 //   (movmatrix) a register.
 // The maximum that the exponents are taken against moves only when a logit
-// exceeds it by more than 8 (in powers of two): until then p <= 2^8, which
-// costs no precision, and the 32*NT accumulators are not rescaled.
+// exceeds it by more than 8 (in powers of two), and e_g only when a scale
+// exceeds 2^(e_g + 7): until then p s 2^-e < 2^15, which FP16 holds, and the
+// 32*NT accumulators are not rescaled.  One vote a tile finds out.
+// Keys that a row does not see are dealt with only in tiles that are partly
+// hidden, by a second copy of the code.
 #include <type_traits>
 #include "join.cuh"
 #include "kernels.h"
@@ -39,8 +43,6 @@
 namespace vcb {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;        // keys of a warp's tile: two records
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;
@@ -67,12 +69,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
@@ -80,10 +76,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 }
 __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t bf162_bits(float lo, float hi) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
@@ -117,50 +109,56 @@ __device__ __forceinline__ void load8(const T* p, float* x) {
 
 
 template <int D, int NT>
-struct DecodeSmem {
-  static constexpr int kStages = 3;
+struct DecodeCfg {
+  // 8 warps twice an SM, 12 or 8 once: what the accumulators leave of the registers
+  static constexpr int kWarps = NT == 2 ? 12 : 8, kThreads = kWarps * 32, kCtas = NT == 1 ? 2 : 1;
+  static constexpr int kStages = NT == 1 ? 3 : 4;
   static constexpr int kTileBytes = 2 * Kv4Rec<D>::kBytes;
   static constexpr int kRing = kWarps * kStages * kTileBytes;
   static constexpr int kMerge = kWarps * 8 * (D + 4) * 4;         // one n-tile's O of every warp (row stride D + 4)
-  static constexpr int kOffBar = kRing > kMerge ? kRing : kMerge;
+  static constexpr bool kQShared = NT > 2;                        // Q operands in shared memory, not registers
+  static constexpr int kOffQ = kRing > kMerge ? kRing : kMerge;
+  static constexpr int kQBytes = kQShared ? NT * (D / 32) * 32 * 16 : 0;
+  static constexpr int kOffBar = kOffQ + kQBytes;
   static constexpr int kOffStat = kOffBar + kWarps * kStages * 8; // float2 [warps][8 NT]
   static constexpr int kBytes = kOffStat + kWarps * 8 * NT * 8;
+  static_assert(kCtas * (kBytes + 1024) <= 228 * 1024, "shared memory");
 };
 
 template <int D, typename T, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv4_decode_kernel(DecodeParams p) {
+__global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::kCtas) kv4_decode_kernel(DecodeParams p) {
   using R = Kv4Rec<D>;
-  using L = DecodeSmem<D, NT>;
-  constexpr int NG = D / 64;
+  using L = DecodeCfg<D, NT>;
+  constexpr int kWarps = L::kWarps, NG = D / 64;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int split = blockIdx.x;
-  const int64_t bh = blockIdx.y, b = bh / p.pages.heads, hk = bh % p.pages.heads;
+  const int bh = blockIdx.y, b = bh / static_cast<int>(p.pages.heads), hk = bh - b * static_cast<int>(p.pages.heads);
   const int row0 = blockIdx.z * 8 * NT;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar) + warp * L::kStages;
+  if (lane < L::kStages) mbar_init(&bars[lane], 1);
+  fence_barrier_init();
+  if (p.splits > 1) allow_dependent_launch();
   int len, nq;
   kv4_sequence(p.pages, p.lengths, p.q_lengths, static_cast<int>(p.Sq), b, len, nq);
   const int live_rows = nq * p.G;
-
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar) + warp * L::kStages;
-  if (lane == 0)
-    for (int s = 0; s < L::kStages; ++s) mbar_init(&bars[s], 1);
-  fence_barrier_init();
   __syncwarp();
 
   // keys that some row of this CTA sees, in tiles of 32: sinks [0, nsink) and [main0, main0 + nmain)
   int nsink = 0, main0 = 0, ntiles = 0;
   const int last_row = min(row0 + 8 * NT, live_rows) - 1;
-  int pos_first = 0, pos_last = 0;
+  // rows see all of a tile iff it ends before the first row's last key and starts after the last row's first
+  int all_hi = 0, all_lo = 0;
   if (last_row >= row0) {
-    pos_first = len - nq + row0 / p.G;
-    pos_last = len - nq + last_row / p.G;
-    const KeyRanges a = visible_keys(p.vis, pos_first, len), z = visible_keys(p.vis, pos_last, len);
+    const KeyRanges a = visible_keys(p.vis, len - nq + row0 / p.G, len), z = visible_keys(p.vis, len - nq + last_row / p.G, len);
     const int lo = p.vis.window ? a.lo : 0, hi = z.hi;   // the last row reaches furthest, the first starts first
     const int sink_end = p.vis.window ? min(p.vis.sinks, hi) : 0;
     main0 = lo / kTile;
     const int end = (hi + kTile - 1) / kTile;
     nsink = min((sink_end + kTile - 1) / kTile, main0);
     ntiles = nsink + (end > main0 ? end - main0 : 0);
+    all_hi = a.hi;
+    all_lo = z.lo;
   }
   const int t_begin = static_cast<int>(int64_t(ntiles) * split / p.splits);
   const int t_end = static_cast<int>(int64_t(ntiles) * (split + 1) / p.splits);
@@ -181,8 +179,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv4_decode_kernel(D
     const int64_t rec = p.pages.record<D>(b, hk, blk);
     return rec < 0 ? -2 : rec;
   };
-  auto issue = [&](int i, int64_t rec) {
-    const int s = i % L::kStages;
+  auto issue = [&](int i, int s, int64_t rec) {
     if (rec == -2) raise_error(kErrBadIndex);
     const uint32_t n = __popc(__ballot_sync(0xffffffffu, rec >= 0));
     okbits = (okbits & ~(1u << s)) | (rec >= 0 ? 1u << s : 0u);
@@ -194,11 +191,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv4_decode_kernel(D
   for (int i = 0; i < L::kStages - 1 && i < mine; ++i) {
     const int64_t rec = next;
     next = locate(i + 1);
-    issue(i, rec);
+    issue(i, i, rec);
   }
 
-  // Q operands of this warp's (all) rows; row n = r of each n-tile
-  uint32_t qf[NT][NG][2][4];   // [word of 8 channels][b0 step 0, b1 step 0, b0 step 1, b1 step 1]
+  // Q operands; row n = r of each n-tile.  Word w of group g: channels 64g + 16c + 8w + {0,4} {1,5}/16 {2,6} {3,7}/16
+  uint32_t qf[L::kQShared ? 1 : NT][NG][2][4];
+  uint4* qs = reinterpret_cast<uint4*>(smem + L::kOffQ);
   float acol[NT][2], qsum[NT][NG][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -206,7 +204,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv4_decode_kernel(D
     float x[NG][16];
     float big = 0.f, sum[NG];
     const bool have = row < p.rows;
-    const T* src = static_cast<const T*>(p.q) + b * p.qsb + (hk * p.G + (have ? row % p.G : 0)) * p.qsh + (have ? row / p.G : 0) * p.qss;
+    const int tk = have ? row / p.G : 0, hd = have ? row - tk * p.G : 0;
+    const T* src = static_cast<const T*>(p.q) + b * p.qsb + (hk * p.G + hd) * p.qsh + tk * p.qss;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       load8(src + 64 * g + 16 * c, x[g]);
@@ -232,10 +231,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv4_decode_kernel(D
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const float* y = x[g] + 8 * w;
-        qf[nt][g][w][0] = half2_bits(y[0] * up, y[4] * up);
-        qf[nt][g][w][1] = half2_bits(y[1] * up16, y[5] * up16);
-        qf[nt][g][w][2] = half2_bits(y[2] * up, y[6] * up);
-        qf[nt][g][w][3] = half2_bits(y[3] * up16, y[7] * up16);
+        const uint32_t f[4] = {half2_bits(y[0] * up, y[4] * up), half2_bits(y[1] * up16, y[5] * up16),
+                               half2_bits(y[2] * up, y[6] * up), half2_bits(y[3] * up16, y[7] * up16)};
+        if constexpr (L::kQShared) {
+          if (warp == 0) qs[((nt * NG + g) * 2 + w) * 32 + lane] = make_uint4(f[0], f[1], f[2], f[3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) qf[nt][g][w][j] = f[j];
+        }
       }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {   // this thread's accumulator columns are rows 2c and 2c + 1
@@ -244,9 +247,16 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv4_decode_kernel(D
       for (int g = 0; g < NG; ++g) qsum[nt][g][k] = __shfl_sync(0xffffffffu, sum[g], (2 * c + k) * 4) * p.scale_log2;
     }
   }
+  if constexpr (L::kQShared) __syncthreads();
 
   float o[NT][NG][4][4];
   float m[NT][2], l[NT][2], vm[NT][NG][2];
+  float cap[NG], dn[NG];   // 2^(e_g + 7) and 2^-e_g; no scale met yet
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    cap[g] = -1.f;
+    dn[g] = 0.f;
+  }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -264,102 +274,160 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv4_decode_kernel(D
   // logical key row r of a record's m-tile is token pi(r) = r/2 + 4 (r%2) (and 8 + that for r + 8), so that
   // the V loads of the four c lanes, keys {c, c+4, c+8, c+12}, spread over the banks
   const int tok = (r >> 1) + 4 * (r & 1);
-  // rows see all of a tile iff it ends before every row's last key and starts after every row's first
-  const KeyRanges first = visible_keys(p.vis, pos_first, len);
-  const int last_lo = visible_keys(p.vis, pos_last, len).lo;
+  const uint32_t kat = tok * R::kCodeRow + c * 8, vat = R::kV + r * 4 + c * R::kCodeRow, pat = R::kKp + tok * R::kParRow;
+  const uint32_t ring_at = smem_u32(ring);
   bool ok = true;
-  for (int i = 0; i < mine; ++i) {
+  for (int i = 0, s = 0, phase = 0; i < mine; ++i) {
     {
       const int64_t rec = next;
       next = locate(i + L::kStages);
-      if (i + L::kStages - 1 < mine) issue(i + L::kStages - 1, rec);
+      const int fill = s == 0 ? L::kStages - 1 : s - 1;   // the stage read last
+      if (i + L::kStages - 1 < mine) issue(i + L::kStages - 1, fill, rec);
     }
-    const int s = i % L::kStages;
-    ok = __all_sync(0xffffffffu, mbar_wait(&bars[s], (i / L::kStages) & 1, kErrTimeoutTma));
+    ok = __all_sync(0xffffffffu, mbar_wait(&bars[s], phase, kErrTimeoutTma));
     if (!ok) break;
     const uint32_t have = __ballot_sync(0xffffffffu, (okbits >> s) & 1u) & 3u;
     const int key0 = tile_of(i) * kTile;
-    const bool whole = have == 3u && key0 + kTile <= first.hi &&
-                       (p.vis.window == 0 || key0 >= last_lo || key0 + kTile <= p.vis.sinks);
-    const uint32_t base = smem_u32(ring + s * L::kTileBytes);
+    const bool whole = have == 3u && key0 + kTile <= all_hi &&
+                       (p.vis.window == 0 || key0 >= all_lo || key0 + kTile <= p.vis.sinks);
+    const uint32_t base = ring_at + s * L::kTileBytes;
+    if (++s == L::kStages) {
+      s = 0;
+      phase ^= 1;
+    }
+    // logits of the tile: x[record][nt][.] of key rows r (0, 1: columns) and r + 8 (2, 3)
     float x[2][NT][4];
-    uint2 vpar[2][2];   // V (scale, minimum) of token rows r and r + 8; .y the second group
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {   // the two records
-      const uint32_t rec = base + k * R::kBytes;
-      float acc[NT][NG][4];
+    for (int g = 0; g < NG; ++g) {
+      float acc[2][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int g = 0; g < NG; ++g)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[nt][g][j] = 0.f;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const uint2 ca = lds64(rec + R::kK + tok * R::kCodeRow + g * 32 + c * 8);
-        const uint2 cb = lds64(rec + R::kK + (tok + 8) * R::kCodeRow + g * 32 + c * 8);
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const uint32_t a = w ? ca.y : ca.x, bq = w ? cb.y : cb.x;
-          const uint32_t a8 = a >> 8, b8 = bq >> 8;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma_f16(acc[nt][g], a & 0x000F000Fu, bq & 0x000F000Fu, a & 0x00F000F0u, bq & 0x00F000F0u, qf[nt][g][w][0], qf[nt][g][w][1]);
-            mma_f16(acc[nt][g], a8 & 0x000F000Fu, b8 & 0x000F000Fu, a8 & 0x00F000F0u, b8 & 0x00F000F0u, qf[nt][g][w][2], qf[nt][g][w][3]);
-          }
-        }
-      }
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int t = tok + 8 * half;
-        uint2 kp;
-        if constexpr (NG == 2) {
-          kp = lds64(rec + R::kKp + t * R::kParRow);
-          vpar[k][half] = lds64(rec + R::kVp + t * R::kParRow);
-        } else {
-          kp = make_uint2(lds32(rec + R::kKp + t * R::kParRow), 0u);
-          vpar[k][half] = make_uint2(lds32(rec + R::kVp + t * R::kParRow), 0u);
-        }
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float u = acc[nt][0][2 * half + j] * bf16_lo(kp.x), y = bf16_hi(kp.x) * qsum[nt][0][j];
-            if constexpr (NG == 2) {
-              u = fmaf(acc[nt][NG - 1][2 * half + j], bf16_lo(kp.y), u);
-              y = fmaf(bf16_hi(kp.y), qsum[nt][NG - 1][j], y);
-            }
-            x[k][nt][2 * half + j] = fmaf(u, acol[nt][j], y);
-          }
+          for (int j = 0; j < 4; ++j) acc[k][nt][j] = 0.f;
+      uint2 ca[2], cb[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        ca[k] = lds64(base + k * R::kBytes + kat + g * 32);
+        cb[k] = lds64(base + k * R::kBytes + kat + g * 32 + 8 * R::kCodeRow);
       }
-    }
-    if (!whole) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int w = 0; w < 2; ++w) {
+        uint32_t a[2][8];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int row = row0 + nt * 8 + 2 * c + j;
-          const KeyRanges v = visible_keys(p.vis, len - nq + row / p.G, len);
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t u = w ? ca[k].y : ca[k].x, v = w ? cb[k].y : cb[k].x, u8 = u >> 8, v8 = v >> 8;
+          a[k][0] = u & 0x000F000Fu;
+          a[k][1] = v & 0x000F000Fu;
+          a[k][2] = u & 0x00F000F0u;
+          a[k][3] = v & 0x00F000F0u;
+          a[k][4] = u8 & 0x000F000Fu;
+          a[k][5] = v8 & 0x000F000Fu;
+          a[k][6] = u8 & 0x00F000F0u;
+          a[k][7] = v8 & 0x00F000F0u;
+        }
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
+        for (int nt = 0; nt < NT; ++nt) {
+          uint32_t f[4];
+          if constexpr (L::kQShared) {
+            const uint4 q4 = qs[((nt * NG + g) * 2 + w) * 32 + lane];
+            f[0] = q4.x; f[1] = q4.y; f[2] = q4.z; f[3] = q4.w;
+          } else {
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const int key = key0 + 16 * k + tok + 8 * half;
-              const bool see = ((have >> k) & 1u) && key < v.hi && (key >= v.lo || key < v.sink_end);
-              if (!see) x[k][nt][2 * half + j] = -INFINITY;
+            for (int j = 0; j < 4; ++j) f[j] = qf[nt][g][w][j];
+          }
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            mma_f16(acc[k][nt], a[k][0], a[k][1], a[k][2], a[k][3], f[0], f[1]);
+            mma_f16(acc[k][nt], a[k][4], a[k][5], a[k][6], a[k][7], f[2], f[3]);
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t kp = lds32(base + k * R::kBytes + pat + 8 * half * R::kParRow + g * 4);
+          const float sk = bf16_lo(kp), mk = bf16_hi(kp);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float& t = x[k][nt][2 * half + j];
+              const float u = acc[k][nt][2 * half + j] * acol[nt][j];
+              t = fmaf(u, sk, g == 0 ? mk * qsum[nt][0][j] : fmaf(mk, qsum[nt][g][j], t));
             }
         }
     }
-    // move the maxima only if some logit is far above its own
+    // V (scale, minimum) of key rows r and r + 8 of both records
+    uint32_t vpar[2][2][NG];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t at = base + k * R::kBytes + pat + (R::kVp - R::kKp) + 8 * half * R::kParRow;
+        if constexpr (NG == 2) {
+          const uint2 u = lds64(at);
+          vpar[k][half][0] = u.x;
+          vpar[k][half][NG - 1] = u.y;
+        } else {
+          vpar[k][half][0] = lds32(at);
+        }
+      }
+    if (!whole) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int key = key0 + 16 * k + tok + 8 * half;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int row = row0 + nt * 8 + 2 * c + j;
+              const KeyRanges v = visible_keys(p.vis, len - nq + row / p.G, len);
+              if (!(((have >> k) & 1u) && key < v.hi && (key >= v.lo || key < v.sink_end))) x[k][nt][2 * half + j] = -INFINITY;
+            }
+          // past the end there is no scale (whatever was read)
+          if (!((have >> k) & 1u) || key >= len)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) vpar[k][half][g] = 0u;
+        }
+    }
+    // move the maxima and the scale exponents only if some logit or scale is far above them
     bool far = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float top = fmaxf(fmaxf(x[0][nt][j], x[0][nt][2 + j]), fmaxf(x[1][nt][j], x[1][nt][2 + j]));
-        far |= top > m[nt][j] + kLazy;
-      }
+      for (int j = 0; j < 2; ++j)
+        far |= fmaxf(fmaxf(x[0][nt][j], x[0][nt][2 + j]), fmaxf(x[1][nt][j], x[1][nt][2 + j])) > m[nt][j] + kLazy;
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+      far |= fmaxf(fmaxf(bf16_lo(vpar[0][0][g]), bf16_lo(vpar[0][1][g])), fmaxf(bf16_lo(vpar[1][0][g]), bf16_lo(vpar[1][1][g]))) > cap[g];
     if (__any_sync(0xffffffffu, far)) {
+      float up[NG];
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float top = 0.f;   // scales that are not finite count for nothing here: their products are not either
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const float sv = bf16_lo(vpar[k][half][g]);
+            if (sv < INFINITY) top = fmaxf(top, sv);
+          }
+        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+        up[g] = 1.f;
+        if (__uint_as_float(bits) > cap[g]) {
+          // 2^e: the largest scale's own power of two, within what its reciprocal and 2^(e + 7) can be
+          const int e = max(-100, min(100, static_cast<int>(bits >> 23) - 127));
+          const float now = __uint_as_float(uint32_t(127 - e) << 23);
+          up[g] = cap[g] < 0.f ? 0.f : now / dn[g];
+          dn[g] = now;
+          cap[g] = __uint_as_float(uint32_t(127 + e + 7) << 23);
+        }
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -375,69 +443,72 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv4_decode_kernel(D
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
             vm[nt][g][j] *= alpha;
+            const float f = alpha * up[g];
 #pragma unroll
             for (int i4 = 0; i4 < 4; ++i4) {
-              o[nt][g][i4][j] *= alpha;
-              o[nt][g][i4][2 + j] *= alpha;
+              o[nt][g][i4][j] *= f;
+              o[nt][g][i4][2 + j] *= f;
             }
           }
         }
     }
     // probabilities, then O^T += V^T P^T
+    auto product = [&](auto hidden) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const uint32_t rec = base + k * R::kBytes;
-      uint32_t bh_[NT][NG][2], bl_[NT][NG][2];
+      for (int k = 0; k < 2; ++k) {
+        uint32_t bp[NT][NG][2];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const float s0 = bf16_lo(vpar[k][half].x), s1 = bf16_lo(vpar[k][half].y);
-        const float m0 = fmaf(-128.f, s0, bf16_hi(vpar[k][half].x)), m1 = fmaf(-128.f, s1, bf16_hi(vpar[k][half].y));
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float e[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float v = x[k][nt][2 * half + j];
-            e[j] = v == -INFINITY ? 0.f : exp2_fast(v - m[nt][j]);
-            l[nt][j] += e[j];
-          }
+        for (int half = 0; half < 2; ++half) {
+          float sv[NG], mv[NG];
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
-            const float sg = g ? s1 : s0, mg = g ? m1 : m0;
-            float w[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              // a hidden key's scale may be anything: its weight is zero, not 0 * scale
-              const bool hid = x[k][nt][2 * half + j] == -INFINITY;
-              w[j] = hid ? 0.f : e[j] * sg;
-              vm[nt][g][j] += hid ? 0.f : e[j] * mg;
-            }
-            const uint32_t hi = bf162_bits(w[0], w[1]);
-            const uint32_t lo = bf162_bits(w[0] - bf16_lo(hi), w[1] - bf16_hi(hi));
-            bh_[nt][g][half] = transpose8x8(hi);
-            bl_[nt][g][half] = transpose8x8(lo);
+            sv[g] = bf16_lo(vpar[k][half][g]) * dn[g];
+            mv[g] = bf16_hi(vpar[k][half][g]);
           }
-        }
-      }
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const uint32_t at = rec + R::kV + g * 32 + r * 4;
-        const uint32_t w0 = lds32(at + c * R::kCodeRow), w1 = lds32(at + (c + 4) * R::kCodeRow);
-        const uint32_t w2 = lds32(at + (c + 8) * R::kCodeRow), w3 = lds32(at + (c + 12) * R::kCodeRow);
-        const uint32_t la = __byte_perm(w0, w1, 0x5410), ha = __byte_perm(w0, w1, 0x7632);
-        const uint32_t lb = __byte_perm(w2, w3, 0x5410), hb = __byte_perm(w2, w3, 0x7632);
-#pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-          const uint32_t a0 = ((la >> (4 * i4)) & 0x000F000Fu) | 0x43004300u, a1 = ((ha >> (4 * i4)) & 0x000F000Fu) | 0x43004300u;
-          const uint32_t a2 = ((lb >> (4 * i4)) & 0x000F000Fu) | 0x43004300u, a3 = ((hb >> (4 * i4)) & 0x000F000Fu) | 0x43004300u;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            mma_bf16(o[nt][g][i4], a0, a1, a2, a3, bh_[nt][g][0], bh_[nt][g][1]);
-            mma_bf16(o[nt][g][i4], a0, a1, a2, a3, bl_[nt][g][0], bl_[nt][g][1]);
+            float e[2];
+            bool hid[2] = {false, false};
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float t = x[k][nt][2 * half + j];
+              if constexpr (decltype(hidden)::value) hid[j] = t == -INFINITY;
+              // (no maximum yet: nothing is seen, and -inf - -inf would not be 0)
+              e[j] = hid[j] ? 0.f : exp2_fast(t - m[nt][j]);
+              l[nt][j] += e[j];
+            }
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              // a hidden key's scale may be anything: its weight is zero, not 0 * scale
+#pragma unroll
+              for (int j = 0; j < 2; ++j) vm[nt][g][j] = hid[j] ? vm[nt][g][j] : fmaf(e[j], mv[g], vm[nt][g][j]);
+              bp[nt][g][half] = transpose8x8(half2_bits(hid[0] ? 0.f : e[0] * sv[g], hid[1] ? 0.f : e[1] * sv[g]));
+            }
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const uint32_t at = base + k * R::kBytes + vat + g * 32;
+          const uint32_t w0 = lds32(at), w1 = lds32(at + 4 * R::kCodeRow), w2 = lds32(at + 8 * R::kCodeRow), w3 = lds32(at + 12 * R::kCodeRow);
+          // channels 8r + 0..3 (la, lb) and 8r + 4..7 (ha, hb) of keys 2c, 2c + 1 (a) and 2c + 8, 2c + 9 (b)
+          const uint32_t la = __byte_perm(w0, w1, 0x5410), ha = __byte_perm(w0, w1, 0x7632);
+          const uint32_t lb = __byte_perm(w2, w3, 0x5410), hb = __byte_perm(w2, w3, 0x7632);
+#pragma unroll
+          for (int i2 = 0; i2 < 2; ++i2) {
+            const uint32_t u = la >> (8 * i2), v = ha >> (8 * i2), y = lb >> (8 * i2), z = hb >> (8 * i2);
+#pragma unroll
+            for (int i1 = 0; i1 < 2; ++i1) {
+              const uint32_t mask = i1 ? 0x00F000F0u : 0x000F000Fu;
+              const uint32_t a0 = u & mask, a1 = v & mask, a2 = y & mask, a3 = z & mask;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][g][2 * i2 + i1], a0, a1, a2, a3, bp[nt][g][0], bp[nt][g][1]);
+            }
           }
         }
       }
-    }
+    };
+    if (whole) product(std::false_type());
+    else product(std::true_type());
     __syncwarp();   // every lane has read the stage that the next issue overwrites
   }
 
@@ -455,6 +526,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv4_decode_kernel(D
       }
       if (r == 0) stat[warp * 8 * NT + nt * 8 + 2 * c + j] = make_float2(m[nt][j], l[nt][j]);
     }
+  // O is in units of 2^e_g 2^-24 (codes in the low nibble) or 2^-20 (in the high one)
+  float unit[NG];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) unit[g] = dn[g] > 0.f ? 16777216.f / dn[g] : 0.f;
   __syncthreads();
   float* merge = reinterpret_cast<float*>(smem);
   constexpr int kRow = D + 4;
@@ -472,17 +547,18 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv4_decode_kernel(D
         float v[8];
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4) {
-          v[i4] = (o[nt][g][i4][j] + vm[nt][g][j]) * f;
-          v[4 + i4] = (o[nt][g][i4][2 + j] + vm[nt][g][j]) * f;
+          const float by = (i4 & 1) ? unit[g] * 0.0625f : unit[g];
+          v[i4] = fmaf(o[nt][g][i4][j], by, vm[nt][g][j]) * f;
+          v[4 + i4] = fmaf(o[nt][g][i4][2 + j], by, vm[nt][g][j]) * f;
         }
         *reinterpret_cast<float4*>(row + 64 * g + 8 * r) = make_float4(v[0], v[1], v[2], v[3]);
         *reinterpret_cast<float4*>(row + 64 * g + 8 * r + 4) = make_float4(v[4], v[5], v[6], v[7]);
       }
     }
     __syncthreads();
-    // warp w joins row w of this n-tile; lane: D/32 channels
+    // warp w < 8 joins row w of this n-tile; lane: D/32 channels
     const int row = row0 + nt * 8 + warp;
-    if (row < p.rows) {
+    if (warp < 8 && row < p.rows) {
       float top = -INFINITY, sum = 0.f;
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, stat[w * 8 * NT + nt * 8 + warp].x);
       for (int w = 0; w < kWarps; ++w) {
@@ -506,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) kv4_decode_kernel(D
         if constexpr (C == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(h);
         else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(h);
       } else {
-        const int64_t at = (bh * p.rows + row) * p.splits + split;
+        const int64_t at = (int64_t(bh) * p.rows + row) * p.splits + split;
         float* dst = p.part_o + at * D + lane * C;
 #pragma unroll
         for (int k = 0; k < C; ++k) dst[k] = dead ? 0.f : v[k];
@@ -521,19 +597,20 @@ struct Plan {
   int nt, blocks, splits;
 };
 
-// Rows a CTA (8, 16 or 32) and splits of the keys: enough CTAs to fill the
-// GPU twice over, at least one tile a warp each.
+// Rows a CTA (8, 16, 24 or 32) and splits of the keys: about one CTA for each
+// that fits the GPU, and at least one tile a warp each.
 Plan plan_of(const Kv4AttnArgs& a) {
   const int64_t rows = a.Sq * (a.Hq / a.cache.Hkv);
   Plan r;
-  r.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  r.nt = static_cast<int>(rows >= 25 ? 4 : (rows + 7) / 8);
   r.blocks = static_cast<int>((rows + 8 * r.nt - 1) / (8 * r.nt));
   int64_t keys = kv4_most(a.cache, a.max_length);
   if (a.window > 0) keys = min64(keys, a.window + a.Sq + a.sinks + 2 * kTile);
   const int64_t tiles = (keys + kTile - 1) / kTile, items = a.cache.B * a.cache.Hkv * r.blocks;
-  int64_t s = (4 * 148 + items - 1) / items;
-  s = min64(s, (tiles + kWarps - 1) / kWarps);
-  r.splits = static_cast<int>(s < 1 ? 1 : s > 256 ? 256 : s);
+  const int64_t fit = 148 * (r.nt == 1 ? 2 : 1), warps = r.nt == 2 ? 12 : 8;
+  int64_t s = items >= 8 * fit ? 1 : items >= fit ? 2 : fit / items;
+  s = min64(s, (tiles + warps - 1) / warps);
+  r.splits = static_cast<int>(s < 1 ? 1 : s);
   return r;
 }
 
@@ -546,13 +623,13 @@ int launched() { return cudaGetLastError() == cudaSuccess ? VC_OK : VC_ERR_LAUNC
 template <int D, typename T, int NT>
 int launch_decode(const DecodeParams& p, const Plan& plan, int64_t BH, cudaStream_t st) {
   auto* k = kv4_decode_kernel<D, T, NT>;
-  constexpr int bytes = DecodeSmem<D, NT>::kBytes;
+  constexpr int bytes = DecodeCfg<D, NT>::kBytes;
   static std::atomic<uint64_t> ready{0};
   if (!allow_smem(reinterpret_cast<const void*>(k), bytes, ready)) return VC_ERR_LAUNCH;
-  k<<<dim3(plan.splits, static_cast<unsigned>(BH), plan.blocks), kThreads, bytes, st>>>(p);
+  k<<<dim3(plan.splits, static_cast<unsigned>(BH), plan.blocks), DecodeCfg<D, NT>::kThreads, bytes, st>>>(p);
   if (plan.splits > 1) {
     const JoinParams j{p.part_o, p.part_ml, p.out, p.osb, p.osh, p.oss, p.pages.heads, p.rows, p.G, p.splits};
-    launch_join<D, T>(j, BH * p.rows, st);
+    if (launch_join<D, T>(j, BH * p.rows, st) != cudaSuccess) return VC_ERR_LAUNCH;
   }
   return launched();
 }
@@ -561,6 +638,7 @@ template <int D, typename T>
 int launch(const DecodeParams& p, const Plan& plan, int64_t BH, cudaStream_t st) {
   if (plan.nt == 1) return launch_decode<D, T, 1>(p, plan, BH, st);
   if (plan.nt == 2) return launch_decode<D, T, 2>(p, plan, BH, st);
+  if (plan.nt == 3) return launch_decode<D, T, 3>(p, plan, BH, st);
   return launch_decode<D, T, 4>(p, plan, BH, st);
 }
 

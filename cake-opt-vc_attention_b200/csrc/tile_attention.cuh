@@ -263,6 +263,7 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
     }
     fence_barrier_init();
   }
+  if (p.splits > 1) allow_dependent_launch();
   int len, nq, base;
   if constexpr (KV4) {
     kv4_sequence(p.pages, p.lengths, p.q_lengths, p.Sq, b, len, nq);
@@ -883,7 +884,7 @@ int launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, const TileParams&
   k<<<dim3(static_cast<unsigned>(p.BH) * static_cast<unsigned>(p.pairs), static_cast<unsigned>(p.splits)), C::kThreads, bytes, st>>>(mk, mv, p);
   if (p.splits > 1) {
     const JoinParams j{p.part_o, p.part_ml, p.out, p.osb, p.osh, p.oss, p.Hkv, p.rows, p.G, p.splits};
-    launch_join<D, QT>(j, int64_t(p.BH) * p.rows, st);
+    if (launch_join<D, QT>(j, int64_t(p.BH) * p.rows, st) != cudaSuccess) return VC_ERR_LAUNCH;
   }
   return cudaGetLastError() == cudaSuccess ? VC_OK : VC_ERR_LAUNCH;
 }
