@@ -536,8 +536,9 @@ int vc_kv4_append(const void* k, const void* v, const void* q, void* q_out, int 
     if (int rc = check_input(fn, "q", q, dtype, q_stride_b, q_stride_h, q_stride_s)) return rc;
     if (int rc = check_input(fn, "q_out", q_out, dtype, qo_stride_b, qo_stride_h, qo_stride_s)) return rc;
   }
-  if (rot_dim < 0 || rot_dim > D || rot_dim % 16 || (rot_dim > 0 && (!cos || !sin || rot_rows < 1))) {
-    set_last_error("%s: rot_dim must be a multiple of 16 in [0, D] with cos and sin of at least one row", fn);
+  if (rot_dim < 0 || rot_dim > D || rot_dim % 16 ||
+      (rot_dim > 0 && (!cos || !sin || !aligned16(cos) || !aligned16(sin) || rot_rows < 1))) {
+    set_last_error("%s: rot_dim must be a multiple of 16 in [0, D] with 16-byte aligned cos and sin of at least one row", fn);
     return VC_ERR_ARG;
   }
   if (!lengths) {

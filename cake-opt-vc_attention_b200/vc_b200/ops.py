@@ -431,6 +431,9 @@ def kv4_append(pool: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tens
                              f"most {D}")
         cos, sin = cos.contiguous(), sin.contiguous()
         cp, sp = cos.data_ptr(), sin.data_ptr()
+        if (cp | sp) & 15:
+            cos, sin = cos.clone(), sin.clone()
+            cp, sp = cos.data_ptr(), sin.data_ptr()
     lengths = _ints(name, "lengths", lengths, (B,), dev)
     positions = _ints(name, "positions", positions, (B, S), dev)
     counts = _ints(name, "counts", counts, (B,), dev)
