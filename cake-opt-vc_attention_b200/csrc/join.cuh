@@ -45,32 +45,51 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// One CTA a row, a warp for every eighth split (at most eight warps), D/32
-// channels a lane; the warps' sums are added in order.  Launched while the
-// kernel before it still runs (programmatic dependent launch), so that its
-// launch costs nothing: it waits for that kernel's results itself.
+// One CTA a row, at most eight warps that take every eighth split each, D/32
+// channels a lane; the warps' sums are added in order.  The factors 2^(m_s - m)
+// come first, so that the loads of the outputs depend on nothing and several
+// are in flight.  Launched while the kernel before it still runs (programmatic
+// dependent launch), so that its launch costs nothing: it waits for that
+// kernel's results itself.
+constexpr int kMostSplits = 1024;
+
 template <int D, typename T>
 __global__ void __launch_bounds__(256) join_splits_kernel(JoinParams p) {
   constexpr int C = D / 32;
   __shared__ float part[8][D];
-  __shared__ float sums[8];
+  __shared__ float factor[kMostSplits];
+  __shared__ float tops[8], sums[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int64_t i = blockIdx.x;
+  const int row = static_cast<int>(blockIdx.x % static_cast<unsigned>(p.rows)), tok = row / p.G;
+  const int bh = static_cast<int>(blockIdx.x / static_cast<unsigned>(p.rows)), b = bh / static_cast<int>(p.heads), hk = bh % static_cast<int>(p.heads);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const float2* ml = p.part_ml + i * p.splits;
   float top = -INFINITY;
-  for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, ml[s].x);
+  for (int s = threadIdx.x; s < p.splits; s += blockDim.x) top = fmaxf(top, ml[s].x);
 #pragma unroll
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float v[C], sum = 0.f;
-#pragma unroll
-  for (int k = 0; k < C; ++k) v[k] = 0.f;
-  const float* src = p.part_o + i * p.splits * D + lane * C;
-#pragma unroll 4
-  for (int s = warp; s < p.splits; s += warps) {
+  if (lane == 0) tops[warp] = top;
+  __syncthreads();
+  for (int w = 0; w < warps; ++w) top = fmaxf(top, tops[w]);
+  float sum = 0.f;
+  for (int s = threadIdx.x; s < p.splits; s += blockDim.x) {
     const float2 a = ml[s];
     const float f = a.x == -INFINITY ? 0.f : exp2_fast(a.x - top);
     sum += a.x == -INFINITY ? a.y : a.y * f;   // without a maximum: 0, or NaN where every logit is
+    factor[s] = f;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) sums[warp] = sum;
+  __syncthreads();
+  float v[C];
+#pragma unroll
+  for (int k = 0; k < C; ++k) v[k] = 0.f;
+  const float* src = p.part_o + i * p.splits * D + lane * C;
+#pragma unroll 8
+  for (int s = warp; s < p.splits; s += warps) {
+    const float f = factor[s];
     float x[C];
     if constexpr (C == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src + s * D);
     else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(src + s * D);
@@ -79,17 +98,13 @@ __global__ void __launch_bounds__(256) join_splits_kernel(JoinParams p) {
   }
 #pragma unroll
   for (int k = 0; k < C; ++k) part[warp][lane * C + k] = v[k];
-  if (lane == 0) sums[warp] = sum;
   __syncthreads();
-  const int row = static_cast<int>(i % p.rows), tok = row / p.G;
-  const int64_t bh = i / p.rows, b = bh / p.heads, hk = bh % p.heads;
   T* dst = static_cast<T*>(p.out) + b * p.osb + (hk * p.G + (row - tok * p.G)) * p.osh + int64_t(tok) * p.oss;
+  float l = 0.f;
+  for (int w = 0; w < warps; ++w) l += sums[w];
   for (int d = threadIdx.x; d < D; d += blockDim.x) {
-    float o = 0.f, l = 0.f;
-    for (int w = 0; w < warps; ++w) {
-      o += part[w][d];
-      l += sums[w];
-    }
+    float o = 0.f;
+    for (int w = 0; w < warps; ++w) o += part[w][d];
     dst[d] = from_f32<T>(l == 0.f ? 0.f : o / l);
   }
 }

@@ -24,8 +24,12 @@
 //     high nibble.  Exact products, FP32 sums.
 //   O^T = V^T P^T  A = V codes (m = channel), two keys' words merged by byte
 //     permutes; B = p s_g 2^-e_g in FP16 (11 significant bits), where 2^e_g
-//     follows the largest scale met so far by steps (sum_j p_j m_jg is
-//     accumulated in FP32 beside it).
+//     follows the largest scale met so far by steps; sum_j p_j m_jg is
+//     accumulated in FP32.  That rounding of p s counts against s u, a value's
+//     distance from the end of its group's range; where the results are FP16 it
+//     should count against the distance from the middle, so codes are then
+//     counted from 8: one more tile of constant codes 8 gives 8 sum_j P_j of the
+//     same rounded P_j to subtract, and m + 8 s takes the place of m.
 //   S^T's accumulator layout becomes P^T's operand layout by one 8x8 transpose
 //   (movmatrix) a register.
 // The maximum that the exponents are taken against moves only when a logit
@@ -110,19 +114,23 @@ __device__ __forceinline__ void load8(const T* p, float* x) {
 
 template <int D, int NT>
 struct DecodeCfg {
-  // 8 warps twice an SM, 12 or 8 once: what the accumulators leave of the registers
-  static constexpr int kWarps = NT == 2 ? 12 : 8, kThreads = kWarps * 32, kCtas = NT == 1 ? 2 : 1;
+  // What the accumulators leave of the registers: 16, 12 or 8 warps an SM, in CTAs small enough that
+  // some work while others wait for their first keys or join their warps.
+  static constexpr int kWarps = NT == 1 ? 4 : NT == 2 ? 6 : 4, kThreads = kWarps * 32, kCtas = NT == 1 ? 4 : 2;
   static constexpr int kStages = NT == 1 ? 3 : 4;
   static constexpr int kTileBytes = 2 * Kv4Rec<D>::kBytes;
   static constexpr int kRing = kWarps * kStages * kTileBytes;
   static constexpr int kMerge = kWarps * 8 * (D + 4) * 4;         // one n-tile's O of every warp (row stride D + 4)
-  static constexpr bool kQShared = NT > 2;                        // Q operands in shared memory, not registers
-  static constexpr int kOffQ = kRing > kMerge ? kRing : kMerge;
-  static constexpr int kQBytes = kQShared ? NT * (D / 32) * 32 * 16 : 0;
-  static constexpr int kOffBar = kOffQ + kQBytes;
+  static constexpr bool kQShared = NT > 2;                        // Q operands stay in shared memory, not registers
+  // Q operands: their own place, or (where they move on to registers) warp 0's last stage before it is first filled
+  static constexpr int kOffQ = kQShared ? (kRing > kMerge ? kRing : kMerge) : (kStages - 1) * kTileBytes;
+  static constexpr int kQBytes = NT * (D / 32) * 32 * 16;
+  static constexpr int kOffCol = (kRing > kMerge ? kRing : kMerge) + (kQShared ? kQBytes : 0);                 // float4 [8 NT]: a row's factor, sums of Q
+  static constexpr int kOffBar = kOffCol + 8 * NT * 4 * 4;
   static constexpr int kOffStat = kOffBar + kWarps * kStages * 8; // float2 [warps][8 NT]
   static constexpr int kBytes = kOffStat + kWarps * 8 * NT * 8;
   static_assert(kCtas * (kBytes + 1024) <= 228 * 1024, "shared memory");
+  static_assert(kQShared || kQBytes <= kTileBytes, "Q operands do not fit a stage");
 };
 
 template <int D, typename T, int NT>
@@ -194,13 +202,11 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
     issue(i, i, rec);
   }
 
-  // Q operands; row n = r of each n-tile.  Word w of group g: channels 64g + 16c + 8w + {0,4} {1,5}/16 {2,6} {3,7}/16
-  uint32_t qf[L::kQShared ? 1 : NT][NG][2][4];
+  // Q operands, an n-tile a warp; row n = r.  Word w of group g: channels 64g + 16c + 8w + {0,4} {1,5}/16 {2,6} {3,7}/16
   uint4* qs = reinterpret_cast<uint4*>(smem + L::kOffQ);
-  float acol[NT][2], qsum[NT][NG][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int row = row0 + nt * 8 + r;
+  float4* cols = reinterpret_cast<float4*>(smem + L::kOffCol);   // by row: factor, scaled sum of Q by group
+  if (warp < NT) {
+    const int nt = warp, row = row0 + nt * 8 + r;
     float x[NG][16];
     float big = 0.f, sum[NG];
     const bool have = row < p.rows;
@@ -210,6 +216,9 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
     for (int g = 0; g < NG; ++g) {
       load8(src + 64 * g + 16 * c, x[g]);
       load8(src + 64 * g + 16 * c + 8, x[g] + 8);
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
       sum[g] = 0.f;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -225,47 +234,70 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
     int e = big > 0.f ? 14 + 127 - static_cast<int>(__float_as_uint(big) >> 23) : 0;
     e = max(-100, min(126, e));
     const float up = __uint_as_float(uint32_t(127 + e) << 23), up16 = up * 0.0625f;
-    const float ac = __uint_as_float(uint32_t(127 - e) << 23) * 16777216.f * p.scale_log2;   // 2^(24 - e) scale
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const float* y = x[g] + 8 * w;
-        const uint32_t f[4] = {half2_bits(y[0] * up, y[4] * up), half2_bits(y[1] * up16, y[5] * up16),
-                               half2_bits(y[2] * up, y[6] * up), half2_bits(y[3] * up16, y[7] * up16)};
-        if constexpr (L::kQShared) {
-          if (warp == 0) qs[((nt * NG + g) * 2 + w) * 32 + lane] = make_uint4(f[0], f[1], f[2], f[3]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) qf[nt][g][w][j] = f[j];
-        }
+        qs[((nt * NG + g) * 2 + w) * 32 + lane] =
+            make_uint4(half2_bits(y[0] * up, y[4] * up), half2_bits(y[1] * up16, y[5] * up16),
+                       half2_bits(y[2] * up, y[6] * up), half2_bits(y[3] * up16, y[7] * up16));
       }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {   // this thread's accumulator columns are rows 2c and 2c + 1
-      acol[nt][k] = __shfl_sync(0xffffffffu, ac, (2 * c + k) * 4);
-#pragma unroll
-      for (int g = 0; g < NG; ++g) qsum[nt][g][k] = __shfl_sync(0xffffffffu, sum[g], (2 * c + k) * 4) * p.scale_log2;
+    if (c == 0)   // logits are kept in units of 2^(24 - e) scale, their column's factor
+    {
+      const float unit = __uint_as_float(uint32_t(127 - e) << 23) * 16777216.f;
+      cols[nt * 8 + r] = make_float4(fmaxf(unit * p.scale_log2, 1.1754943508222875e-38f), sum[0] / unit, sum[NG - 1] / unit, 0.f);
     }
   }
-  if constexpr (L::kQShared) __syncthreads();
+  __syncthreads();
+  uint32_t qf[L::kQShared ? 1 : NT][NG][2][4];
+  float acol[NT][2], qsum[NT][NG][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {   // this thread's accumulator columns are rows 2c and 2c + 1
+      const float4 v = cols[nt * 8 + 2 * c + k];
+      acol[nt][k] = v.x;
+      qsum[nt][0][k] = v.y;
+      qsum[nt][NG - 1][k] = v.z;
+    }
+    if constexpr (!L::kQShared) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const uint4 v = qs[((nt * NG + g) * 2 + w) * 32 + lane];
+          qf[nt][g][w][0] = v.x; qf[nt][g][w][1] = v.y; qf[nt][g][w][2] = v.z; qf[nt][g][w][3] = v.w;
+        }
+    }
+  }
 
-  float o[NT][NG][4][4];
-  float m[NT][2], l[NT][2], vm[NT][NG][2];
-  float cap[NG], dn[NG];   // 2^(e_g + 7) and 2^-e_g; no scale met yet
+  if constexpr (!L::kQShared) {
+    __syncthreads();   // the operands are read before the stage is filled
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  // (FP16 results show the difference, BF16 ones do not)
+  constexpr bool kMiddle = std::is_same<T, __half>::value;
+  float o[NT][NG][4][4], mid[kMiddle ? NT : 1][NG][4];   // mid: 8 sum_j P_j, the same in every row
+  float m[NT][2], lim[NT][2], l[NT][2], vm[NT][NG][2];   // lim: where a logit moves the maximum
+  // 2^(e_g + 7), 2^-e_g, and what O is in units of: 2^e_g 2^-24 (codes in the low nibble; 2^-20 in the high one).
+  // No scale met yet.
+  float cap[NG], dn[NG], unit[NG];
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
     cap[g] = -1.f;
-    dn[g] = 0.f;
+    dn[g] = unit[g] = 0.f;
   }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      m[nt][k] = -INFINITY;
+      m[nt][k] = lim[nt][k] = -INFINITY;
       l[nt][k] = 0.f;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         vm[nt][g][k] = 0.f;
+        if constexpr (kMiddle) mid[nt][g][2 * k] = mid[nt][g][2 * k + 1] = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[nt][g][i][2 * k] = o[nt][g][i][2 * k + 1] = 0.f;
       }
@@ -295,7 +327,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
       s = 0;
       phase ^= 1;
     }
-    // logits of the tile: x[record][nt][.] of key rows r (0, 1: columns) and r + 8 (2, 3)
+    // logits of the tile, in units of their column's factor: x[record][nt][.] of key rows r (0, 1: columns) and r + 8 (2, 3)
     float x[2][NT][4];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
@@ -355,8 +387,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               float& t = x[k][nt][2 * half + j];
-              const float u = acc[k][nt][2 * half + j] * acol[nt][j];
-              t = fmaf(u, sk, g == 0 ? mk * qsum[nt][0][j] : fmaf(mk, qsum[nt][g][j], t));
+              t = fmaf(acc[k][nt][2 * half + j], sk, g == 0 ? mk * qsum[nt][0][j] : fmaf(mk, qsum[nt][g][j], t));
             }
         }
     }
@@ -401,7 +432,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 2; ++j)
-        far |= fmaxf(fmaxf(x[0][nt][j], x[0][nt][2 + j]), fmaxf(x[1][nt][j], x[1][nt][2 + j])) > m[nt][j] + kLazy;
+        far |= fmaxf(fmaxf(x[0][nt][j], x[0][nt][2 + j]), fmaxf(x[1][nt][j], x[1][nt][2 + j])) > lim[nt][j];
 #pragma unroll
     for (int g = 0; g < NG; ++g)
       far |= fmaxf(fmaxf(bf16_lo(vpar[0][0][g]), bf16_lo(vpar[0][1][g])), fmaxf(bf16_lo(vpar[1][0][g]), bf16_lo(vpar[1][1][g]))) > cap[g];
@@ -425,6 +456,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
           const float now = __uint_as_float(uint32_t(127 - e) << 23);
           up[g] = cap[g] < 0.f ? 0.f : now / dn[g];
           dn[g] = now;
+          unit[g] = 16777216.f / now;
           cap[g] = __uint_as_float(uint32_t(127 + e + 7) << 23);
         }
       }
@@ -437,13 +469,18 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
           const float mn = fmaxf(m[nt][j], top);
-          const float alpha = mn == -INFINITY ? 1.f : exp2_fast(m[nt][j] - mn);
+          const float alpha = mn == -INFINITY ? 1.f : exp2_fast((m[nt][j] - mn) * acol[nt][j]);
           m[nt][j] = mn;
+          lim[nt][j] = mn + kLazy / acol[nt][j];
           l[nt][j] *= alpha;
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
             vm[nt][g][j] *= alpha;
             const float f = alpha * up[g];
+            if constexpr (kMiddle) {
+              mid[nt][g][j] *= f;
+              mid[nt][g][2 + j] *= f;
+            }
 #pragma unroll
             for (int i4 = 0; i4 < 4; ++i4) {
               o[nt][g][i4][j] *= f;
@@ -463,7 +500,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
             sv[g] = bf16_lo(vpar[k][half][g]) * dn[g];
-            mv[g] = bf16_hi(vpar[k][half][g]);
+            mv[g] = kMiddle ? fmaf(8.f, bf16_lo(vpar[k][half][g]), bf16_hi(vpar[k][half][g])) : bf16_hi(vpar[k][half][g]);
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
@@ -474,7 +511,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
               const float t = x[k][nt][2 * half + j];
               if constexpr (decltype(hidden)::value) hid[j] = t == -INFINITY;
               // (no maximum yet: nothing is seen, and -inf - -inf would not be 0)
-              e[j] = hid[j] ? 0.f : exp2_fast(t - m[nt][j]);
+              e[j] = hid[j] ? 0.f : exp2_fast((t - m[nt][j]) * acol[nt][j]);   // exactly 1 at the maximum
               l[nt][j] += e[j];
             }
 #pragma unroll
@@ -493,6 +530,9 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
           // channels 8r + 0..3 (la, lb) and 8r + 4..7 (ha, hb) of keys 2c, 2c + 1 (a) and 2c + 8, 2c + 9 (b)
           const uint32_t la = __byte_perm(w0, w1, 0x5410), ha = __byte_perm(w0, w1, 0x7632);
           const uint32_t lb = __byte_perm(w2, w3, 0x5410), hb = __byte_perm(w2, w3, 0x7632);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            if constexpr (kMiddle) mma_f16(mid[nt][g], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, bp[nt][g][0], bp[nt][g][1]);
 #pragma unroll
           for (int i2 = 0; i2 < 2; ++i2) {
             const uint32_t u = la >> (8 * i2), v = ha >> (8 * i2), y = lb >> (8 * i2), z = hb >> (8 * i2);
@@ -524,12 +564,9 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
 #pragma unroll
         for (int g = 0; g < NG; ++g) vm[nt][g][j] += __shfl_xor_sync(0xffffffffu, vm[nt][g][j], sh);
       }
+      m[nt][j] *= acol[nt][j];   // from here on a plain power of two
       if (r == 0) stat[warp * 8 * NT + nt * 8 + 2 * c + j] = make_float2(m[nt][j], l[nt][j]);
     }
-  // O is in units of 2^e_g 2^-24 (codes in the low nibble) or 2^-20 (in the high one)
-  float unit[NG];
-#pragma unroll
-  for (int g = 0; g < NG; ++g) unit[g] = dn[g] > 0.f ? 16777216.f / dn[g] : 0.f;
   __syncthreads();
   float* merge = reinterpret_cast<float*>(smem);
   constexpr int kRow = D + 4;
@@ -544,25 +581,27 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
       float* row = merge + (warp * 8 + 2 * c + j) * kRow;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        float v[8];
+        float v[8], base = vm[nt][g][j];
+        if constexpr (kMiddle) base = fmaf(mid[nt][g][j], -unit[g], base);
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4) {
           const float by = (i4 & 1) ? unit[g] * 0.0625f : unit[g];
-          v[i4] = fmaf(o[nt][g][i4][j], by, vm[nt][g][j]) * f;
-          v[4 + i4] = fmaf(o[nt][g][i4][2 + j], by, vm[nt][g][j]) * f;
+          v[i4] = fmaf(o[nt][g][i4][j], by, base) * f;
+          v[4 + i4] = fmaf(o[nt][g][i4][2 + j], by, base) * f;
         }
         *reinterpret_cast<float4*>(row + 64 * g + 8 * r) = make_float4(v[0], v[1], v[2], v[3]);
         *reinterpret_cast<float4*>(row + 64 * g + 8 * r + 4) = make_float4(v[4], v[5], v[6], v[7]);
       }
     }
     __syncthreads();
-    // warp w < 8 joins row w of this n-tile; lane: D/32 channels
-    const int row = row0 + nt * 8 + warp;
-    if (warp < 8 && row < p.rows) {
+    // a warp joins rows warp, warp + kWarps, ... of this n-tile; lane: D/32 channels
+    for (int wr = warp; wr < 8; wr += kWarps) {
+      const int row = row0 + nt * 8 + wr;
+      if (row >= p.rows) break;
       float top = -INFINITY, sum = 0.f;
-      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, stat[w * 8 * NT + nt * 8 + warp].x);
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, stat[w * 8 * NT + nt * 8 + wr].x);
       for (int w = 0; w < kWarps; ++w) {
-        const float2 ml = stat[w * 8 * NT + nt * 8 + warp];
+        const float2 ml = stat[w * 8 * NT + nt * 8 + wr];
         sum += ml.x == -INFINITY ? ml.y : ml.y * exp2_fast(ml.x - top);   // no maximum: 0, or NaN if all logits are
       }
       constexpr int C = D / 32;
@@ -572,7 +611,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
 #pragma unroll
       for (int w = 0; w < kWarps; ++w)
 #pragma unroll
-        for (int k = 0; k < C; ++k) v[k] += merge[(w * 8 + warp) * kRow + lane * C + k];
+        for (int k = 0; k < C; ++k) v[k] += merge[(w * 8 + wr) * kRow + lane * C + k];
       const bool dead = row >= live_rows || sum == 0.f;   // nothing seen
       if (p.splits == 1) {
         T h[C];
@@ -607,10 +646,15 @@ Plan plan_of(const Kv4AttnArgs& a) {
   int64_t keys = kv4_most(a.cache, a.max_length);
   if (a.window > 0) keys = min64(keys, a.window + a.Sq + a.sinks + 2 * kTile);
   const int64_t tiles = (keys + kTile - 1) / kTile, items = a.cache.B * a.cache.Hkv * r.blocks;
-  const int64_t fit = 148 * (r.nt == 1 ? 2 : 1), warps = r.nt == 2 ? 12 : 8;
-  int64_t s = items >= 8 * fit ? 1 : items >= fit ? 2 : fit / items;
-  s = min64(s, (tiles + warps - 1) / warps);
-  r.splits = static_cast<int>(s < 1 ? 1 : s);
+  const int64_t fit = 148 * (r.nt == 1 ? 4 : 2), warps = r.nt == 2 ? 6 : 4;
+  // One sequence: its heads' shares are alike, and half a wave of CTAs is enough (37741 keys of 4 heads: 14.6 us;
+  // a whole wave, whose results take longer to join, 17.9; a third 17.9).  Several: their lengths differ, so
+  // about 3.5 waves of CTAs to even them out, of at least twelve tiles a warp (a CTA costs about as much beside
+  // them) unless that leaves the GPU half empty (64 sequences up to 8192, 8 heads: 96 us; two waves 105, one 121).
+  const int64_t a_wave = (fit + items - 1) / items;
+  int64_t s = a.cache.B == 1 ? min64(fit / 2 / items, tiles / warps)
+                             : max64(min64(7 * fit / 2 / items, tiles / (12 * warps)), min64(2 * a_wave, (tiles + 3 * warps - 1) / (3 * warps)));
+  r.splits = static_cast<int>(s < 1 ? 1 : min64(s, kMostSplits));
   return r;
 }
 

@@ -3,7 +3,7 @@
 // append: K (and the call's Q) rotated by position, K and V quantised, K/V
 //   codes and (scale, minimum) pairs written to their pages, Q written out.
 //     rotation   y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin (FP32; each product and sum rounded)
-//     64 channels of a token and head: s = bf16((max - min) / 15), m = bf16(min),
+//     64 channels of a token and head: s = bf16((max - min) * (1/15)), m = bf16(min),
 //     code = clamp(rint((x - m) * (1 / s)), 0, 15), 0 where s is 0 or not finite
 //   A group that holds a NaN or an infinity reads back as NaN: its (s, m) are.
 //   The minimum and maximum propagate NaN for that reason.
@@ -23,6 +23,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr float kLeastNormal = 1.1754943508222875e-38f;
+constexpr float kFifteenth = 1.f / 15.f;
 
 struct AppendParams {
   const void *k, *v, *q;
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, HEADS > 1 ? 4 : 1) kv4_append_kernel
         continue;
       }
       const __nv_bfloat16 m16 = __float2bfloat16_rn(lo);
-      __nv_bfloat16 s16 = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
+      __nv_bfloat16 s16 = __float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, lo), kFifteenth));
       const float m = __bfloat162float(m16);
       float s = __bfloat162float(s16);
       if (s < kLeastNormal) {

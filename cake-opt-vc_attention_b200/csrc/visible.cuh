@@ -12,6 +12,8 @@ namespace vcb {
 // clamped to 2^30 (which is then no limit), so 32-bit arithmetic holds.
 constexpr int64_t kMostTokens = int64_t(1) << 30;
 
+inline int64_t max64(int64_t a, int64_t b) { return a > b ? a : b; }
+
 struct Visibility {
   int window;   // 0: unlimited
   int sinks;

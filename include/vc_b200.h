@@ -223,7 +223,7 @@ int vc_attention_fwd_e4m3qk(const uint8_t* q8, const float* qs, const uint8_t* k
  * [0, rot_rows): bit 0x80 and row 0), pairs (i, i + rot_dim/2), or
  * (2i, 2i + 1) when interleaved, of the first rot_dim channels (a multiple of
  * 16, at most D):  y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin.  Each group of
- * 64 channels is then quantised: scale = bf16((max - min)/15), minimum =
+ * 64 channels is then quantised: scale = bf16((max - min) * (1/15), FP32), minimum =
  * bf16(min), code = clamp(rint((x - minimum) * (1/scale)), 0, 15).  A group
  * with a NaN or an infinity reads back as NaN.  dtype F16 or BF16. */
 int vc_kv4_append(const void* k, const void* v, const void* q, void* q_out, int dtype, int64_t B, int64_t Hq,

@@ -16,7 +16,7 @@ def quantise(x):
     """(codes [.., D], scale [.., D/64], minimum) with the FP32 arithmetic of the definition."""
     y = x.float().unflatten(-1, (-1, GROUP))
     lo, hi = y.amin(-1), y.amax(-1)
-    s, m = ((hi - lo) / 15.0).to(torch.bfloat16).float(), lo.to(torch.bfloat16).float()
+    s, m = ((hi - lo) * torch.tensor(1.0 / 15.0)).to(torch.bfloat16).float(), lo.to(torch.bfloat16).float()
     s = torch.where(s < TINY, torch.zeros_like(s), s)
     inv = torch.where(s == 0, torch.zeros_like(s), 1.0 / s)
     u = ((y - m[..., None]) * inv[..., None]).round().clamp(0, 15).nan_to_num(nan=0.0)
