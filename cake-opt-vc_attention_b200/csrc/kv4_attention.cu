@@ -156,11 +156,12 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
   int nsink = 0, main0 = 0, ntiles = 0;
   const int last_row = min(row0 + 8 * NT, live_rows) - 1;
   // rows see all of a tile iff it ends before the first row's last key and starts after the last row's first
-  int all_hi = 0, all_lo = 0;
+  int all_hi = 0, all_lo = 0, lo = 0, sink_end = 0;
   if (last_row >= row0) {
     const KeyRanges a = visible_keys(p.vis, len - nq + row0 / p.G, len), z = visible_keys(p.vis, len - nq + last_row / p.G, len);
-    const int lo = p.vis.window ? a.lo : 0, hi = z.hi;   // the last row reaches furthest, the first starts first
-    const int sink_end = p.vis.window ? min(p.vis.sinks, hi) : 0;
+    const int hi = z.hi;   // the last row reaches furthest, the first starts first
+    lo = p.vis.window ? a.lo : 0;
+    sink_end = p.vis.window ? min(p.vis.sinks, hi) : 0;
     main0 = lo / kTile;
     const int end = (hi + kTile - 1) / kTile;
     nsink = min((sink_end + kTile - 1) / kTile, main0);
@@ -180,10 +181,11 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
     const int t = i0 + i * kWarps;
     return t < nsink ? t : main0 + (t - nsink);
   };
-  auto locate = [&](int i) -> int64_t {   // lanes 0 and 1: the record's offset, -1 past the end, -2 without a page
+  auto locate = [&](int i) -> int64_t {   // lanes 0 and 1: the record's offset, -1 where no row sees it, -2 without a page
     if (lane > 1 || i >= mine) return -1;
     const int blk = tile_of(i) * 2 + lane;
-    if (blk * kKv4Block >= len) return -1;
+    const int first = blk * kKv4Block;
+    if (first >= len || (first + kKv4Block <= lo && first >= sink_end)) return -1;
     const int64_t rec = p.pages.record<D>(b, hk, blk);
     return rec < 0 ? -2 : rec;
   };
@@ -420,7 +422,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
               const KeyRanges v = visible_keys(p.vis, len - nq + row / p.G, len);
               if (!(((have >> k) & 1u) && key < v.hi && (key >= v.lo || key < v.sink_end))) x[k][nt][2 * half + j] = -INFINITY;
             }
-          // past the end there is no scale (whatever was read)
+          // what was not brought, or lies past the end, has no scale (whatever was read)
           if (!((have >> k) & 1u) || key >= len)
 #pragma unroll
             for (int g = 0; g < NG; ++g) vpar[k][half][g] = 0u;

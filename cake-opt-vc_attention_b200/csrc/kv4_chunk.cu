@@ -69,9 +69,9 @@ __global__ void __launch_bounds__(256) kv4_unpack_kernel(UnpackParams p) {
   if (tile >= un.end) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x < 8) {
-    const int blk = tile * 8 + threadIdx.x;
-    int64_t at = -1;   // past the end
-    if (int64_t(blk) * kKv4Block < len) {
+    const int blk = tile * 8 + threadIdx.x, first = blk * kKv4Block;
+    int64_t at = -1;   // seen by no row
+    if (first < len && !(p.vis.window && first + kKv4Block <= un.lo && first >= un.sink_end)) {
       at = p.pages.record<D>(b, hk, blk);
       if (at < 0) {
         raise_error(kErrBadIndex);

@@ -80,18 +80,21 @@ struct __align__(16) TileMeta {
 // Which unpacked tile holds a sequence's key tile: only those that the call's
 // rows see are unpacked, the sinks' first.
 struct UnpackedTiles {
-  int sink, base;   // tiles [0, sink), then [base, end)
+  int sink, base;      // tiles [0, sink), then [base, end)
   int end;
+  int lo, sink_end;    // keys [0, sink_end) and from lo on are seen by some row
   __device__ __forceinline__ int slot(int tile) const { return tile < sink ? tile : sink + (tile - base); }
 };
 __device__ __forceinline__ UnpackedTiles unpacked_tiles(const Visibility& v, int len, int nq) {
-  UnpackedTiles u{0, 0, 0};
+  UnpackedTiles u{0, 0, 0, 0, 0};
   if (nq <= 0) return u;
   const KeyRanges a = visible_keys(v, len - nq, len), z = visible_keys(v, len - 1, len);
   u.end = (z.hi + 127) >> 7;
   if (v.window) {
+    u.lo = a.lo;
+    u.sink_end = min(v.sinks, z.hi);
     u.base = a.lo >> 7;
-    u.sink = min((min(v.sinks, z.hi) + 127) >> 7, u.base);
+    u.sink = min((u.sink_end + 127) >> 7, u.base);
   }
   return u;
 }
@@ -411,10 +414,11 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
     } else {
       if (warp == 8) {
         // ------------------------------------- records of a half tile (64 keys), four lanes
-        auto locate = [&](int u) -> int64_t {   // offset, -1 past the end, -2 without a page
+        const int lo = gb.any ? min(ga.lo, gb.lo) : ga.lo, sink_end = gb.any ? max(ga.sink_end, gb.sink_end) : ga.sink_end;
+        auto locate = [&](int u) -> int64_t {   // offset, -1 where no row sees it, -2 without a page
           if (lane > 3 || u >= 2 * steps) return -1;
-          const int blk = tile_of(u >> 1) * 8 + (u & 1) * 4 + lane;
-          if (int64_t(blk) * kKv4Block >= len) return -1;
+          const int blk = tile_of(u >> 1) * 8 + (u & 1) * 4 + lane, first = blk * kKv4Block;
+          if (first >= len || (p.vis.window && first + kKv4Block <= lo && first >= sink_end)) return -1;
           const int64_t rec = p.pages.record<D>(b, hk, blk);
           return rec < 0 ? -2 : rec;
         };

@@ -1,0 +1,109 @@
+"""A paged 4-bit K/V cache for a batch of sequences: pages, page table and
+lengths around ``ops.kv4_append`` and ``ops.kv4_attention``.
+
+The device holds the pool, the page table and the lengths; the host mirrors
+the lengths and hands out pages, so no call waits for the device.  With a
+window, pages that no later query can see go back to the pool (``trim``): a
+rolling cache of ``sinks + window`` tokens a sequence.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import ops
+
+
+class KV4Cache:
+    """``batch`` sequences of at most ``max_tokens`` tokens that share
+    ``pages`` pages of ``page_size`` tokens.
+
+    ``cos``/``sin`` (FP32 [positions, R/2], optional): the rotation that
+    ``append`` applies to keys and queries.  ``window``/``sinks``/``causal``:
+    what ``attend`` lets a query see (see ``ops.kv4_attention``).
+    """
+
+    def __init__(self, batch: int, kv_heads: int, head_dim: int, *, pages: int, max_tokens: int, page_size: int = 64,
+                 cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, interleaved: bool = False,
+                 window: int | None = None, sinks: int = 0, causal: bool = True, device=None):
+        if batch < 1 or max_tokens < 1:
+            raise ValueError("KV4Cache: batch and max_tokens must be positive")
+        self.pool = ops.kv4_pool(pages, kv_heads, head_dim, page_size, device=device)
+        dev = self.pool.device
+        self.page_size, self.cos, self.sin, self.interleaved = page_size, cos, sin, interleaved
+        self.window, self.sinks, self.causal = window, sinks, causal
+        width = -(-max_tokens // page_size)
+        self.page_table = torch.full((batch, width), -1, dtype=torch.int32, device=dev)
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=dev)
+        self._table = [[-1] * width for _ in range(batch)]   # host mirrors
+        self._lengths = [0] * batch
+        self._free = list(range(pages - 1, -1, -1))
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _rows_to_device(self, rows):
+        for b in rows:
+            self.page_table[b].copy_(torch.tensor(self._table[b], dtype=torch.int32))
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None, *, counts=None,
+               tensor_layout: str = "HND") -> torch.Tensor | None:
+        """Append the call's tokens (``counts``: how many of them, by
+        sequence, host integers; default all) and return the rotated ``q``.
+        Raises RuntimeError, changing nothing, when pages or table run out."""
+        S = k.shape[2] if tensor_layout == "HND" else k.shape[1]
+        counts = [S] * len(self._lengths) if counts is None else [int(c) for c in counts]
+        if len(counts) != len(self._lengths) or any(not 0 <= c <= S for c in counts):
+            raise ValueError("KV4Cache.append: counts must be one number in [0, S] a sequence")
+        need = []
+        for b, c in enumerate(counts):
+            last = -(-(self._lengths[b] + c) // self.page_size)
+            if last > len(self._table[b]):
+                raise RuntimeError(f"KV4Cache: sequence {b} would pass max_tokens")
+            need += [(b, i) for i in range(self._lengths[b] // self.page_size, last) if c and self._table[b][i] < 0]
+        if len(need) > len(self._free):
+            raise RuntimeError(f"KV4Cache: {len(need)} pages needed, {len(self._free)} free")
+        for b, i in need:
+            self._table[b][i] = self._free.pop()
+        self._rows_to_device(sorted({b for b, _ in need}))
+        even = all(c == S for c in counts)
+        dcounts = None if even else torch.tensor(counts, dtype=torch.int32).to(self.pool.device)
+        out = ops.kv4_append(self.pool, self.page_table, self.lengths, k, v, q=q, cos=self.cos, sin=self.sin,
+                             counts=dcounts, interleaved=self.interleaved, tensor_layout=tensor_layout)
+        self.lengths.add_(S if even else dcounts)
+        self._lengths = [n + c for n, c in zip(self._lengths, counts)]
+        return out
+
+    def attend(self, q: torch.Tensor, *, q_lengths: torch.Tensor | None = None, sm_scale: float | None = None,
+               tensor_layout: str = "HND", out: torch.Tensor | None = None) -> torch.Tensor:
+        """``ops.kv4_attention`` of the newest tokens over this cache."""
+        return ops.kv4_attention(q, self.pool, self.page_table, self.lengths, q_lengths=q_lengths, causal=self.causal,
+                                 window=self.window, sinks=self.sinks, sm_scale=sm_scale,
+                                 max_length=max(1, max(self._lengths)), tensor_layout=tensor_layout, out=out)
+
+    def trim(self) -> int:
+        """Return the pages that no query at or after the end of its sequence
+        can see (all tokens behind the window and past the sinks) to the pool;
+        how many they were.  Without a window there are none."""
+        if self.window is None:
+            return 0
+        freed = 0
+        for b, n in enumerate(self._lengths):
+            first = -(-min(self.sinks, n) // self.page_size)            # pages with sinks stay
+            last = max(0, n - self.window + 1) // self.page_size        # as does the first that the next token sees
+            gone = [i for i in range(first, min(last, len(self._table[b]))) if self._table[b][i] >= 0]
+            for i in gone:
+                self._free.append(self._table[b][i])
+                self._table[b][i] = -1
+            if gone:
+                self._rows_to_device([b])
+            freed += len(gone)
+        return freed
+
+    def drop(self, sequence: int) -> None:
+        """Forget a sequence and return its pages."""
+        self._free += [p for p in self._table[sequence] if p >= 0]
+        self._table[sequence] = [-1] * len(self._table[sequence])
+        self._lengths[sequence] = 0
+        self._rows_to_device([sequence])
+        self.lengths[sequence] = 0

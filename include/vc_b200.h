@@ -25,8 +25,9 @@
  *   pool        uint8 [pages, Hkv, page_size/16, 18*D]: the paged 4-bit K/V
  *               cache (vc_kv4_*)
  *   page_table  int32 [B, table_width]: the page that holds tokens
- *               [i*page_size, (i+1)*page_size) of a sequence; entries past a
- *               sequence's end are never read
+ *               [i*page_size, (i+1)*page_size) of a sequence; entries of
+ *               pages that a call neither writes nor lets a query see (past a
+ *               sequence's end, hidden by the window) are not used
  */
 #ifndef VC_B200_H
 #define VC_B200_H

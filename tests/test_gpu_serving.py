@@ -512,3 +512,59 @@ def test_refusals_on_the_device(ops):
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+@pytest.mark.parametrize("Sq,page", [(1, 16), (5, 16), (40, 32), (300, 16), (1, 128)])
+def test_pages_that_no_query_sees_may_be_missing(ops, Sq, page):
+    """Behind the window and past the sinks the table may say anything."""
+    g = _gen(Sq + page)
+    D, L, window, sinks = 128, 900, 200, 20
+    pool, table, n = _filled(ops, g, 1, 2, D, page, [L])
+    q = _randn(g, 1, 8, Sq, D)
+    full = ops.kv4_attention(q.cuda(), pool, table.cuda(), n.cuda(), window=window, sinks=sinks)
+    holes = table.clone()
+    lo = L - Sq - window + 1
+    holes[0, -(-sinks // page): lo // page] = -1
+    assert (holes != table).sum() > 1
+    assert torch.equal(ops.kv4_attention(q.cuda(), pool, holes.cuda(), n.cuda(), window=window, sinks=sinks), full)
+
+
+def test_rolling_cache(ops):
+    """KV4Cache: pages come and go, ragged appends, and the results are those of a cache that keeps everything."""
+    from vc_b200.kv_cache import KV4Cache
+    g = _gen(41)
+    B, H, Hq, D, window, sinks = 2, 2, 4, 64, 48, 10
+    kw = dict(page_size=16, window=window, sinks=sinks)
+    small = KV4Cache(B, H, D, pages=16, max_tokens=400, **kw)
+    large = KV4Cache(B, H, D, pages=60, max_tokens=400, **kw)
+    freed, lengths = 0, [0, 0]
+    for step, counts in ((40, None), (20, [20, 3]), (1, None), (33, [0, 33]), (1, None), (30, None), (30, [30, 29])):
+        k, v, q = (_randn(g, B, h, step, D).cuda() for h in (H, H, Hq))
+        for c in (small, large):
+            assert c.append(k, v, q, counts=counts) is not None
+        counts = counts or [step] * B
+        lengths = [a + b for a, b in zip(lengths, counts)]
+        assert small.lengths.tolist() == lengths
+        ql = torch.tensor(counts, device="cuda")
+        assert torch.equal(small.attend(q, q_lengths=ql), large.attend(q, q_lengths=ql))
+        freed += small.trim()
+    assert freed > 0 and small.free_pages + freed > 0
+    before = small.free_pages
+    with pytest.raises(RuntimeError, match="pages needed"):
+        small.append(*(_randn(g, B, H, 270, D).cuda() for _ in range(2)))
+    assert small.free_pages == before and small.lengths.tolist() == lengths
+    with pytest.raises(RuntimeError, match="max_tokens"):
+        large.append(*(_randn(g, B, H, 390, D).cuda() for _ in range(2)))
+    small.drop(0)
+    assert small.lengths.tolist() == [0, lengths[1]] and small.free_pages > before
+    with pytest.raises(ValueError, match="counts"):
+        small.append(k, v, counts=[1])
+
+
+def test_streaming_example_runs(ops):
+    """The example's stages are near exact attention: the prompt to BF16 rounding, the cache to 4 bits."""
+    from vc_attention.streaming import run
+    reports = run(400, (130, 8, 1), heads=8, kv_heads=2, window=200, sinks=6)
+    assert [r["tokens"] for r in reports] == [400, 130, 8, 1]
+    assert reports[0]["rel_l2"] < 2.0 ** -6
+    assert all(r["rel_l2"] < 0.25 for r in reports[1:]) and sum(r["pages_freed"] for r in reports) > 0
