@@ -551,7 +551,7 @@ def test_rolling_cache(ops):
     assert freed > 0 and small.free_pages + freed > 0
     before = small.free_pages
     with pytest.raises(RuntimeError, match="pages needed"):
-        small.append(*(_randn(g, B, H, 270, D).cuda() for _ in range(2)))
+        small.append(*(_randn(g, B, H, 250, D).cuda() for _ in range(2)))
     assert small.free_pages == before and small.lengths.tolist() == lengths
     with pytest.raises(RuntimeError, match="max_tokens"):
         large.append(*(_randn(g, B, H, 390, D).cuda() for _ in range(2)))
