@@ -24,12 +24,28 @@ inline bool allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& rea
 }
 
 struct JoinParams {
-  const float* part_o;    // [rows of all heads, splits, D]
-  const float2* part_ml;  // [rows of all heads, splits]
+  const float* part_o;    // [partial rows, splits, D]
+  const float2* part_ml;  // [partial rows, splits]
   void* out;
   int64_t osb, osh, oss;
   int64_t heads;          // K/V heads
   int rows, G, splits;    // rows a K/V head: token r / G, query head hk * G + r % G
+  // pairs = 0: the partial rows are all rows, head after head.  Else they are
+  // those of the tile kernel's items from ``whole`` on, 256 each.
+  int whole, pairs, BH;
+
+  // Which row partial row i is; false: past the head's rows.
+  __device__ __forceinline__ bool locate(int64_t i, int& bh, int& row) const {
+    if (pairs == 0) {
+      row = static_cast<int>(static_cast<unsigned>(i) % static_cast<unsigned>(rows));
+      bh = static_cast<int>(static_cast<unsigned>(i) / static_cast<unsigned>(rows));
+      return true;
+    }
+    const int item = whole + static_cast<int>(i >> 8);
+    bh = item % BH;
+    row = (pairs - 1 - item / BH) * 256 + static_cast<int>(i & 255);
+    return row < rows;
+  }
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -45,8 +61,8 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// One CTA a row, at most eight warps that take every eighth split each, D/32
-// channels a lane; the warps' sums are added in order.  The factors 2^(m_s - m)
+// One CTA a row, eight warps that take every eighth split each, D/32 channels
+// a lane; the warps' sums are added in order.  The factors 2^(m_s - m)
 // come first, so that the loads of the outputs depend on nothing and several
 // are in flight.  Launched while the kernel before it still runs (programmatic
 // dependent launch), so that its launch costs nothing: it waits for that
@@ -61,9 +77,11 @@ __global__ void __launch_bounds__(256) join_splits_kernel(JoinParams p) {
   __shared__ float tops[8], sums[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int64_t i = blockIdx.x;
-  const int row = static_cast<int>(blockIdx.x % static_cast<unsigned>(p.rows)), tok = row / p.G;
-  const int bh = static_cast<int>(blockIdx.x / static_cast<unsigned>(p.rows)), b = bh / static_cast<int>(p.heads), hk = bh % static_cast<int>(p.heads);
+  int bh, row;
+  const bool mine = p.locate(i, bh, row);
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!mine) return;
+  const int tok = row / p.G, b = bh / static_cast<int>(p.heads), hk = bh % static_cast<int>(p.heads);
   const float2* ml = p.part_ml + i * p.splits;
   float top = -INFINITY;
   for (int s = threadIdx.x; s < p.splits; s += blockDim.x) top = fmaxf(top, ml[s].x);
@@ -109,6 +127,57 @@ __global__ void __launch_bounds__(256) join_splits_kernel(JoinParams p) {
   }
 }
 
+// The same for few splits: a warp a row, eight rows a CTA, a split's maximum and
+// sum in the lane of its number, all outputs in flight at once.
+constexpr int kFewSplits = 8;
+
+template <int D, typename T>
+__global__ void __launch_bounds__(256) join_few_kernel(JoinParams p, int64_t total) {
+  constexpr int C = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t i = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  int bh, row;
+  const bool mine = i < total && p.locate(i, bh, row);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!mine) return;
+  const int tok = row / p.G, b = bh / static_cast<int>(p.heads), hk = bh % static_cast<int>(p.heads);
+  T* dst = static_cast<T*>(p.out) + b * p.osb + (hk * p.G + (row - tok * p.G)) * p.osh + int64_t(tok) * p.oss + lane * C;
+  const float2 a = lane < p.splits ? p.part_ml[i * p.splits + lane] : make_float2(-INFINITY, 0.f);
+  const float* src = p.part_o + i * p.splits * D + lane * C;
+  float x[kFewSplits][C];
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    if (s < p.splits) {
+      if constexpr (C == 4) *reinterpret_cast<float4*>(x[s]) = *reinterpret_cast<const float4*>(src + s * D);
+      else *reinterpret_cast<float2*>(x[s]) = *reinterpret_cast<const float2*>(src + s * D);
+    }
+  }
+  float top = a.x;
+#pragma unroll
+  for (int o = 4; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float f = a.x == -INFINITY ? 0.f : exp2_fast(a.x - top);
+  float l = a.x == -INFINITY ? a.y : a.y * f;   // without a maximum: 0, or NaN where every logit is
+#pragma unroll
+  for (int o = 4; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  l = __shfl_sync(0xffffffffu, l, 0);
+  float v[C];
+#pragma unroll
+  for (int k = 0; k < C; ++k) v[k] = 0.f;
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    const float fs = __shfl_sync(0xffffffffu, f, s);
+    if (s < p.splits) {
+#pragma unroll
+      for (int k = 0; k < C; ++k) v[k] = fmaf(x[s][k], fs, v[k]);
+    }
+  }
+  T r[C];
+#pragma unroll
+  for (int k = 0; k < C; ++k) r[k] = from_f32<T>(l == 0.f ? 0.f : v[k] / l);
+  if constexpr (C == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(r);
+  else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(r);
+}
+
 // Tells that the next kernel on the stream may be launched; it still waits for
 // this one's results.
 __device__ __forceinline__ void allow_dependent_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
@@ -116,14 +185,16 @@ __device__ __forceinline__ void allow_dependent_launch() { asm volatile("griddep
 template <int D, typename T>
 inline cudaError_t launch_join(const JoinParams& p, int64_t total, cudaStream_t st) {
   cudaLaunchConfig_t c{};
-  c.gridDim = dim3(static_cast<unsigned>(total));
-  c.blockDim = dim3(32 * (p.splits >= 8 ? 8 : p.splits));
+  const bool few = p.splits <= kFewSplits;
+  c.gridDim = dim3(static_cast<unsigned>(few ? (total + 7) / 8 : total));
+  c.blockDim = dim3(256);
   c.stream = st;
   cudaLaunchAttribute early{};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   c.attrs = &early;
   c.numAttrs = 1;
+  if (few) return cudaLaunchKernelEx(&c, join_few_kernel<D, T>, p, total);
   return cudaLaunchKernelEx(&c, join_splits_kernel<D, T>, p);
 }
 

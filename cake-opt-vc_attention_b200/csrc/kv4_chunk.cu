@@ -5,8 +5,8 @@
 // Every CTA (256 rows) reads all keys of its head, so with several CTAs a head
 // the dequantising warps of each do the same work again, and they take issue
 // slots from the softmax: the chunk of 1024 tokens over 16384 (28/4 heads,
-// D 128; 28 CTAs a head) takes 396 us that way and KUNPACKED us unpacked first,
-// of which the unpacking is KUNPACK.  So: unpack when a head has two CTAs or
+// D 128; 28 CTAs a head) takes 396 us that way and 251 us unpacked first,
+// of which the unpacking is about 12.  So: unpack when a head has two CTAs or
 // more and the FP16 tiles fit kMostUnpacked bytes; the workspace is otherwise
 // only needed for split keys.
 #include "tile_attention.cuh"
@@ -39,7 +39,7 @@ ChunkPlan plan_of(const Kv4AttnArgs& a) {
     r.meta_bytes = (BH * slots * int64_t(sizeof(TileMeta)) + 127) / 128 * 128;
   }
   r.bytes = 2 * r.tile_bytes + r.meta_bytes;
-  if (r.tiles.splits > 1) r.bytes += a.cache.B * a.Hq * a.Sq * r.tiles.splits * (a.D + 2) * 4;
+  r.bytes += r.tiles.part_rows() * (a.D + 2) * 4;
   return r;
 }
 
@@ -52,17 +52,21 @@ struct UnpackParams {
   TileMeta* meta;      // [BH, slots]
 };
 
-// One CTA unpacks one tile of 128 keys: first a thread a key finds the tile's
-// largest magnitudes and the keys that are missing or not finite, then 16 bytes
-// of codes (32 channels, 64 bytes of FP16) a thread and turn.
+// One CTA unpacks one tile of 128 keys.  A thread a key (K: warps 0-3, V: 4-7)
+// takes the parameters: the tile's largest magnitudes, the keys that are
+// missing or not finite, scale and minimum as FP16.  Then four bytes of codes
+// (eight channels, 16 bytes of FP16) a thread and turn, so that both sides of a
+// warp are contiguous; those loads are in flight from the start.
 template <int D>
 __global__ void __launch_bounds__(256) kv4_unpack_kernel(UnpackParams p) {
   using R = Kv4Rec<D>;
-  constexpr int kPer = D / 32;   // threads a key
+  constexpr int kChunks = D / 8, kTurns = 2 * 128 * kChunks / 256;
   __shared__ int64_t rec[8];
-  __shared__ uint32_t top[2][8], state[3][4];   // largest magnitude by warp; cleared K, V group 0, V group 1
+  __shared__ uint32_t top[2][8];        // largest magnitude by warp; whether anything is missing or not finite
+  __shared__ uint2 par[2][D / 64][128];   // scale and minimum twice, FP16
   const int bh = blockIdx.y, b = bh / static_cast<int>(p.pages.heads), hk = bh % static_cast<int>(p.pages.heads);
   int len, nq;
+  allow_dependent_launch();
   kv4_sequence(p.pages, p.lengths, p.q_lengths, p.Sq, b, len, nq);
   const UnpackedTiles un = unpacked_tiles(p.vis, len, nq);
   const int slot = blockIdx.x, tile = slot < un.sink ? slot : un.base + (slot - un.sink);
@@ -81,18 +85,24 @@ __global__ void __launch_bounds__(256) kv4_unpack_kernel(UnpackParams p) {
     rec[threadIdx.x] = at;
   }
   __syncthreads();
-  TileMeta* meta = p.meta + int64_t(bh) * p.slots + slot;
-  // warps 0-3: K of 32 keys each, warps 4-7: V
   const int key = threadIdx.x & 127, is_v = threadIdx.x >> 7;
   const int64_t at = rec[key >> 4];
   uint32_t sm[2] = {0, 0};
   const bool ended = at == -1 || tile * 128 + key >= len, lost = at == -2 && !ended;
   if (at >= 0) {
-    const uint8_t* par = p.pages.pool + at + (is_v ? R::kVp : R::kKp) + (key & 15) * R::kParRow;
+    const uint8_t* src = p.pages.pool + at + (is_v ? R::kVp : R::kKp) + (key & 15) * R::kParRow;
 #pragma unroll
-    for (int g = 0; g < D / 64; ++g) sm[g] = __ldg(reinterpret_cast<const uint32_t*>(par) + g);
+    for (int g = 0; g < D / 64; ++g) sm[g] = __ldg(reinterpret_cast<const uint32_t*>(src) + g);
     if constexpr (D == 64) sm[1] = sm[0];
   }
+  uint32_t codes[kTurns];
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i) {
+    const int u = i * 256 + threadIdx.x, w = i >= kTurns / 2, k = u / kChunks & 127, c = u % kChunks;
+    const int64_t r = rec[k >> 4];
+    codes[i] = r < 0 ? 0 : __ldg(reinterpret_cast<const uint32_t*>(p.pages.pool + r + (w ? R::kV : R::kK) + (k & 15) * R::kCodeRow) + c);
+  }
+  TileMeta* meta = p.meta + int64_t(bh) * p.slots + slot;
   const bool gone = ended || lost;
   bool fine[2];
   float big = 0.f;
@@ -103,30 +113,27 @@ __global__ void __launch_bounds__(256) kv4_unpack_kernel(UnpackParams p) {
     if (!gone && m < INFINITY) big = fmaxf(big, m);
   }
   const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
-  const uint32_t clear = __ballot_sync(0xffffffffu, gone), miss = __ballot_sync(0xffffffffu, lost);
+  const uint32_t miss = __ballot_sync(0xffffffffu, lost);
   const uint32_t bad0 = __ballot_sync(0xffffffffu, !gone && !fine[0]), bad1 = __ballot_sync(0xffffffffu, !gone && !fine[1]);
   if (lane == 0) {
     top[is_v][warp & 3] = most;
     if (is_v) {
-      state[1][warp & 3] = clear | bad0;
-      state[2][warp & 3] = clear | bad1;
       meta->bad[0][warp & 3] = bad0;
       meta->bad[1][warp & 3] = bad1;
       top[1][4 + (warp & 3)] = bad0 | bad1;
     } else {
-      state[0][warp & 3] = clear;
       meta->miss[warp & 3] = miss;
       top[0][4 + (warp & 3)] = miss;
     }
   }
   __syncthreads();
-  float down[2];
+  float down = 1.f;
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
     const uint32_t bits = max(max(top[w][0], top[w][1]), max(top[w][2], top[w][3]));
     const int te = static_cast<int>(bits >> 23) - 127;   // the maximum lies in [2^te, 2^(te+1))
     const int e = bits == 0u || (te >= -8 && te <= 14) ? 0 : te > 14 ? te - 14 : max(te, -60);
-    down[w] = __uint_as_float(uint32_t(127 - e) << 23);
+    if (w == is_v) down = __uint_as_float(uint32_t(127 - e) << 23);
     if (threadIdx.x == 0) meta->e[w] = e;
   }
   if (threadIdx.x == 0) {
@@ -135,37 +142,32 @@ __global__ void __launch_bounds__(256) kv4_unpack_kernel(UnpackParams p) {
       for (int i = 4; i < 8; ++i) any |= top[w][i];
     meta->e[2] = any != 0;
   }
+#pragma unroll
+  for (int g = 0; g < D / 64; ++g) {
+    // hidden keys, and V that is not finite (its row's results are set to NaN later), become zeros
+    const uint32_t x = gone || (is_v && !fine[g]) ? 0 : sm[g];
+    const __half2 s2 = __float2half2_rn(bf16_lo(x) * down), m2 = __float2half2_rn(bf16_hi(x) * down);
+    par[is_v][g][key] = make_uint2(*reinterpret_cast<const uint32_t*>(&s2), *reinterpret_cast<const uint32_t*>(&m2));
+  }
+  __syncthreads();
   const __half2 minus1024 = __float2half2_rn(-1024.f), sixteenth = __float2half2_rn(0.0625f), minus64 = __float2half2_rn(-64.f);
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int u = i * 256 + threadIdx.x, w = u / (128 * kPer), k = u / kPer & 127, q = u % kPer;
-    const int64_t r = rec[k >> 4];
-    uint4 codes = make_uint4(0, 0, 0, 0);
-    uint32_t ms = 0;
-    const bool hide = (state[w == 0 ? 0 : 1 + (D == 128 ? q >> 1 : 0)][k >> 5] >> (k & 31)) & 1u;
-    if (r >= 0 && !hide) {
-      const uint8_t* base = p.pages.pool + r;
-      codes = __ldg(reinterpret_cast<const uint4*>(base + (w ? R::kV : R::kK) + (k & 15) * R::kCodeRow + q * 16));
-      ms = __ldg(reinterpret_cast<const uint32_t*>(base + (w ? R::kVp : R::kKp) + (k & 15) * R::kParRow + (D == 128 ? (q >> 1) * 4 : 0)));
-    }
-    const __half2 s2 = __float2half2_rn(bf16_lo(ms) * down[w]), m2 = __float2half2_rn(bf16_hi(ms) * down[w]);
-    uint8_t* dst = (w ? p.v : p.k) + ((int64_t(bh) * p.slots + slot) * 128 + k) * (D * 2) + q * 64;
-    const uint32_t cw[4] = {codes.x, codes.y, codes.z, codes.w};
+  for (int i = 0; i < kTurns; ++i) {
+    const int u = i * 256 + threadIdx.x, w = i >= kTurns / 2, k = u / kChunks & 127, c = u % kChunks;
+    const uint2 sm2 = par[w][c / 8][k];
+    const __half2 s2 = *reinterpret_cast<const __half2*>(&sm2.x), m2 = *reinterpret_cast<const __half2*>(&sm2.y);
+    const uint32_t c0 = codes[i], c8 = c0 >> 8;
+    uint32_t x[4] = {(c0 & 0x000F000Fu) | 0x64006400u, (c0 & 0x00F000F0u) | 0x64006400u,
+                     (c8 & 0x000F000Fu) | 0x64006400u, (c8 & 0x00F000F0u) | 0x64006400u};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t c0 = cw[j], c8 = c0 >> 8;
-      uint32_t x[4] = {(c0 & 0x000F000Fu) | 0x64006400u, (c0 & 0x00F000F0u) | 0x64006400u,
-                       (c8 & 0x000F000Fu) | 0x64006400u, (c8 & 0x00F000F0u) | 0x64006400u};
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        __half2 v = *reinterpret_cast<__half2*>(&x[h]);
-        v = (h & 1) ? __hfma2(v, sixteenth, minus64) : __hadd2(v, minus1024);   // the code, exactly
-        v = __hfma2(v, s2, m2);
-        x[h] = *reinterpret_cast<uint32_t*>(&v);
-      }
-      // channels 8a + {0,4,1,5,2,6,3,7}, as the tile kernel stores Q and writes O
-      reinterpret_cast<uint4*>(dst)[j] = make_uint4(x[0], x[1], x[2], x[3]);
+    for (int h = 0; h < 4; ++h) {
+      __half2 v = *reinterpret_cast<__half2*>(&x[h]);
+      v = (h & 1) ? __hfma2(v, sixteenth, minus64) : __hadd2(v, minus1024);   // the code, exactly
+      v = __hfma2(v, s2, m2);
+      x[h] = *reinterpret_cast<uint32_t*>(&v);
     }
+    // channels 8a + {0,4,1,5,2,6,3,7}, as the tile kernel stores Q and writes O
+    *(reinterpret_cast<uint4*>((w ? p.v : p.k) + ((int64_t(bh) * p.slots + slot) * 128 + k) * (D * 2)) + c) = make_uint4(x[0], x[1], x[2], x[3]);
   }
 }
 
@@ -209,15 +211,12 @@ int kv4_chunk_attention(const Kv4AttnArgs& a, cudaStream_t st) {
   p.Sq = static_cast<int>(a.Sq);
   p.G = static_cast<int>(a.Hq / a.cache.Hkv);
   p.rows = p.Sq * p.G;
-  p.pairs = static_cast<int>(plan.tiles.pairs);
-  p.splits = static_cast<int>(plan.tiles.splits);
   p.vis = visibility(a.window, a.sinks, a.causal);
   p.scale_log2 = a.sm_scale * kLog2e;
   p.lengths = a.lengths;
   p.q_lengths = a.q_lengths;
   p.pages = kv4_pages(a.cache, a.max_length);
-  p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + 2 * plan.tile_bytes + plan.meta_bytes);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + int64_t(p.BH) * p.rows * p.splits * a.D);
+  set_plan(p, plan.tiles, static_cast<uint8_t*>(a.workspace) + 2 * plan.tile_bytes + plan.meta_bytes, a.D);
   if (a.dtype == VC_DTYPE_BF16) return a.D == 128 ? run<128, __nv_bfloat16>(a, plan, p, st) : run<64, __nv_bfloat16>(a, plan, p, st);
   return a.D == 128 ? run<128, __half>(a, plan, p, st) : run<64, __half>(a, plan, p, st);
 }

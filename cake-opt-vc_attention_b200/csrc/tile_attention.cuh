@@ -105,7 +105,8 @@ struct TileParams {
   int64_t qsb, qsh, qss, osb, osh, oss;
   int Sq, Sk;
   int Hkv, BH;                 // BH = B * Hkv
-  int G, rows, pairs, splits;  // rows = Sq * G
+  int G, rows, pairs;          // rows = Sq * G
+  int whole, cut, splits, first;   // TilePlan
   Visibility vis;
   float scale_log2;            // sm_scale * log2(e)
   const int32_t *lengths, *q_lengths;
@@ -227,6 +228,7 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
     tile_attention_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, TileParams p) {
   using C = TileCfg<D, SRC>;
   constexpr bool KV4 = SRC != kTensors, kDequant = SRC == kRecords;
+  constexpr int kGroups = kDequant ? 4 : 1;   // keys of a tile that share one pair of exponents: 32 or all
   constexpr int kSegs = D / 64;
   constexpr int kSeg = 128 * 128;   // bytes of a 64-channel segment of a tile
   extern __shared__ uint8_t smem_raw[];
@@ -235,9 +237,14 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   // the pairs with the most keys come first: under causal order those are the last ones
-  const int split = blockIdx.y;
-  const int pair = p.pairs - 1 - static_cast<int>(blockIdx.x) / p.BH;
-  const int bh = static_cast<int>(blockIdx.x) % p.BH, b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  int item = blockIdx.x, split = 0;
+  const bool cut = item >= p.whole;
+  if (cut) {
+    split = (item - p.whole) / p.cut;
+    item -= split * p.cut;
+  }
+  const int pair = p.pairs - 1 - item / p.BH;
+  const int bh = item % p.BH, b = bh / p.Hkv, hk = bh - b * p.Hkv;
 
   if (warp == 9) {
     tmem_alloc(&ctl->slot, 512);
@@ -266,7 +273,7 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
     }
     fence_barrier_init();
   }
-  if (p.splits > 1) allow_dependent_launch();
+  if (p.cut > 0) allow_dependent_launch();
   int len, nq, base;
   if constexpr (KV4) {
     kv4_sequence(p.pages, p.lengths, p.q_lengths, p.Sq, b, len, nq);
@@ -289,9 +296,13 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
     const int end = (hi + 127) >> 7;
     total = nsink + (end > main0 ? end - main0 : 0);
   }
-  // (at most 2^24 tiles times 148 splits: 32 unsigned bits)
-  const int i0 = p.splits == 1 ? 0 : static_cast<int>(unsigned(total) * unsigned(split) / unsigned(p.splits));
-  const int steps = (p.splits == 1 ? total : static_cast<int>(unsigned(total) * unsigned(split + 1) / unsigned(p.splits))) - i0;
+  // (at most 2^23 tiles times 295 parts: 32 unsigned bits)
+  int i0 = 0, steps = total;
+  if (cut) {
+    const unsigned parts = p.first + p.splits - 1, until = p.first + split;
+    i0 = split == 0 ? 0 : static_cast<int>(unsigned(total) * (until - 1) / parts);
+    steps = static_cast<int>(unsigned(total) * until / parts) - i0;
+  }
   auto tile_of = [&](int n) -> int {
     const int i = i0 + n;
     return i < nsink ? i : main0 + (i - nsink);
@@ -305,6 +316,8 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ctl->slot;
+  // launched while the cache is still being unpacked; nothing above reads what that kernel writes
+  if constexpr (SRC == kUnpacked) asm volatile("griddepcontrol.wait;" ::: "memory");
 
   if (warp >= 8) {
     if constexpr (kDequant) setmaxnreg_dec<64>();
@@ -628,8 +641,8 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
           next_meta = __ldg(reinterpret_cast<const int4*>(p.meta + int64_t(bh) * p.slots + un.slot(tile_of(n + 1))));
         continue;
       }
-      float cg[4] = {c_row, c_row, c_row, c_row};
-      int fg[4] = {0, 0, 0, 0};
+      float cg[kGroups] = {c_row};   // records: by 32 keys
+      int fg[kGroups] = {0};
       uint32_t miss[4] = {0, 0, 0, 0}, bad[2][4] = {};   // 4-bit cache: see TileMeta
       if constexpr (KV4) {
         const TileMeta* meta = &ctl->meta[n & 3];
@@ -647,12 +660,8 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
           const int4 now = next_meta;   // exponents of K and V, and whether anything else is to know
           if (n + 1 < steps) next_meta = __ldg(reinterpret_cast<const int4*>(p.meta + int64_t(bh) * p.slots + un.slot(tile_of(n + 1))));
           any = now.z != 0;
-          const float c = c_row * __uint_as_float(uint32_t(127 + now.x) << 23);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            cg[i] = c;
-            fg[i] = now.y;
-          }
+          cg[0] = c_row * __uint_as_float(uint32_t(127 + now.x) << 23);
+          fg[0] = now.y;
         }
         if (any) {
 #pragma unroll
@@ -706,16 +715,18 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
           top4[q4][1] = max3f(top4[q4][1], __uint_as_float(raw[32 * q4 + c + 2]), __uint_as_float(raw[32 * q4 + c + 3]));
         }
       float top;
-      if constexpr (KV4) {
+      if constexpr (kDequant) {
         top = fmaxf(fmaxf(fmaxf(top4[0][0], top4[0][1]) * cg[0], fmaxf(top4[1][0], top4[1][1]) * cg[1]),
                     fmaxf(fmaxf(top4[2][0], top4[2][1]) * cg[2], fmaxf(top4[3][0], top4[3][1]) * cg[3]));
       } else {
         top = max3f(max3f(top4[0][0], top4[0][1], top4[1][0]), max3f(top4[1][1], top4[2][0], top4[2][1]),
-                    fmaxf(top4[3][0], top4[3][1])) * c_row;
+                    fmaxf(top4[3][0], top4[3][1])) * cg[0];
       }
       float by = 1.f;   // what O has to be multiplied by
       if constexpr (KV4) {
-        int fnew = max(max(fg[0], fg[1]), max(fg[2], fg[3]));
+        int fnew = fg[0];
+#pragma unroll
+        for (int i = 1; i < kGroups; ++i) fnew = max(fnew, fg[i]);
         if (done > 0) fnew = max(fnew, frun);
         if (fnew != frun) by = __uint_as_float(uint32_t(127 + max(-126, frun - fnew)) << 23);
         frun = fnew;
@@ -739,12 +750,17 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
         }
       }
       const float mneg = m == -INFINITY ? 0.f : -m;
+      float shift = KV4 ? static_cast<float>(max(-126, fg[0] - frun)) : 0.f, sum = 0.f;
+      uint64_t c2 = pk2f(cg[0], cg[0]), n2 = pk2f(mneg + shift, mneg + shift);
       uint32_t pw[64];
       auto half = [&](int h) {
 #pragma unroll
         for (int q4 = 2 * h; q4 < 2 * h + 2; ++q4) {
-          const float shift = KV4 ? static_cast<float>(max(-126, fg[q4] - frun)) : 0.f;
-          const uint64_t c2 = pk2f(cg[q4], cg[q4]), n2 = pk2f(mneg + shift, mneg + shift);
+          if constexpr (kDequant) {
+            shift = static_cast<float>(max(-126, fg[q4] - frun));
+            c2 = pk2f(cg[q4], cg[q4]);
+            n2 = pk2f(mneg + shift, mneg + shift);
+          }
           uint64_t sum2[2] = {0, 0};   // bits of (0.f, 0.f)
 #pragma unroll
           for (int i8 = 0; i8 < 16; i8 += 8) {   // eight pairs: kPoly of them by polynomial, side by side
@@ -764,11 +780,12 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
           uint32_t a, d;
           up2(f2_add(sum2[0], sum2[1]), a, d);
           const float s = __uint_as_float(a) + __uint_as_float(d);
-          l += KV4 ? s * exp2_fast(-shift) : s;
+          sum += kDequant ? s * exp2_fast(-shift) : s;
         }
       };
       half(0);
       half(1);
+      l += SRC == kUnpacked ? sum * exp2_fast(-shift) : sum;
       tmem_st32(scol, *reinterpret_cast<uint32_t(*)[32]>(pw));
       tmem_st32(scol + 32, *reinterpret_cast<uint32_t(*)[32]>(pw + 32));
       tmem_wait_st();
@@ -783,8 +800,8 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
       // (hidden keys leave traces of 2^-125 in l, so the maximum tells whether a row saw any; NaN logits leave it alone)
       const bool seen = row < live && done > 0 && (m > -INFINITY || l != l);
       const float unit = KV4 ? __uint_as_float(uint32_t(127 + max(-126, frun)) << 23) : 1.f;
-      const float inv = seen ? (p.splits == 1 ? unit / l : unit) : 0.f;
-      const int64_t at = (int64_t(bh) * p.rows + row) * p.splits + split;
+      const float inv = seen ? (cut ? unit : unit / l) : 0.f;
+      const int64_t at = (int64_t(item - p.whole) * 256 + (row - pair * 256)) * p.splits + split;
 #pragma unroll 1
       for (int cc = 0; cc < D / 32; ++cc) {
         uint32_t o[32];
@@ -798,7 +815,7 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
           v[i] = seen ? __uint_as_float(o[from]) * inv : 0.f;
           if (KV4 && seen && ((nan_out >> (cc >> 1)) & 1u)) v[i] = NAN;
         }
-        if (p.splits == 1) {
+        if (!cut) {
           // all MMAs are done: the Q tile's memory stages the output
 #pragma unroll
           for (int i = 0; i < 4; ++i)
@@ -811,7 +828,7 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
           for (int i = 0; i < 8; ++i) dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
         }
       }
-      if (p.splits == 1) {
+      if (!cut) {
         __syncwarp();
 #pragma unroll 2
         for (int i = 0; i < 32 / kRowsAt; ++i) {
@@ -820,7 +837,7 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
           if (r < p.rows) *reinterpret_cast<uint4*>(static_cast<QT*>(p.out) + int64_t(b) * p.osb + rh * p.osh + rt * p.oss + ch * 8) = u;
         }
       }
-      if (p.splits > 1 && row < p.rows) p.part_ml[at] = seen ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+      if (cut && row < p.rows) p.part_ml[at] = seen ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
     }
   }
   tc_fence_before();
@@ -861,20 +878,64 @@ bool make_map(CUtensorMap* m, const void* base, int dtype, int64_t B, int64_t H,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Pairs of 128-row tiles, and splits of their keys where the pairs alone would
-// leave SMs idle.  ``keys``: the most keys that one row's CTA can see.
+// The CTAs' work.  An item is a pair of 128-row tiles; the first ``whole`` items
+// get a CTA each, the keys of the other ``cut`` are shared by ``splits`` CTAs
+// (join.cuh), of which the first takes ``first`` shares and the others one.
 struct TilePlan {
-  int64_t pairs = 0, splits = 1;
+  int64_t pairs = 0, whole = 0, cut = 0, splits = 1, first = 1;
+  int64_t ctas() const { return whole + cut * splits; }
+  int64_t part_rows() const { return cut * splits * 256; }
 };
+
+// ``keys``: the most keys of a sequence.  One CTA fills an SM, so the items that
+// are left after full waves of 148 (all of them, where there are fewer) leave
+// SMs idle for the time of an item.  Up to half a wave of them is cut into equal
+// shares (2048 x 2048 keys all visible, D 128: 160 items 76 -> 62 us, 200 items
+// 75 -> 70 us); more into two, such that the SMs without a long share take
+// ``first`` short ones each in the same time (16384 keys: 80 items 254 -> 204 us,
+// 96 items 254 -> 206 us, 104 items 254 -> 240 us).  With four short ones the
+// additional CTAs and the join take what the cut gives, and more busy SMs have a
+// lower clock under the power limit (112 items 254 -> 267 us), so three is the
+// most; and a CTA costs about four tiles (8 us), so a short share has eight.
+// Items of very different lengths, as under causal order, fill the SMs by
+// themselves, since the long ones start first.
 inline TilePlan tile_plan(int64_t BH, int64_t rows, int64_t G, int64_t keys, const Visibility& v) {
   TilePlan r;
   r.pairs = (rows + 255) / 256;
-  if (v.window > 0) keys = min64(keys, v.window + (255 + G) / G + v.sinks + 256);
+  int64_t least = v.causal ? max64(keys - rows / G, 0) + 255 / G + 1 : keys;
+  if (v.window > 0) {
+    const int64_t most = v.window + (255 + G) / G + v.sinks + 256;
+    keys = min64(keys, most);
+    least = min64(least, most);
+  }
   const int64_t tiles = (keys + 127) / 128, items = BH * r.pairs;
-  int64_t s = 148 / items;
-  s = min64(s, tiles / 4);
-  r.splits = s < 1 ? 1 : s;
+  r.whole = items;
+  const int64_t tail = items % 148;
+  if (tail == 0 || (items > 148 && 4 * least < 3 * keys)) return r;
+  int64_t s, first = 1;
+  if (tail <= 74) {
+    s = min64(148 / tail, tiles / 4);
+  } else {
+    s = 2;
+    first = (tail + (148 - tail) - 1) / (148 - tail);
+    if (first > 3 || tiles / (first + 1) < 8) s = 1;
+  }
+  if (s < 2) return r;
+  r.whole = items - tail;
+  r.cut = tail;
+  r.splits = s;
+  r.first = first;
   return r;
+}
+
+inline void set_plan(TileParams& p, const TilePlan& t, void* partials, int64_t D) {
+  p.pairs = static_cast<int>(t.pairs);
+  p.whole = static_cast<int>(t.whole);
+  p.cut = static_cast<int>(t.cut);
+  p.splits = static_cast<int>(t.splits);
+  p.first = static_cast<int>(t.first);
+  p.part_o = static_cast<float*>(partials);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + t.part_rows() * D);
 }
 
 template <int D, typename T, typename QT, KvSource SRC>
@@ -885,10 +946,20 @@ int launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, const TileParams&
   static_assert(bytes <= 227 * 1024, "shared memory");
   static std::atomic<uint64_t> ready{0};
   if (!allow_smem(reinterpret_cast<const void*>(k), bytes, ready)) return VC_ERR_LAUNCH;
-  k<<<dim3(static_cast<unsigned>(p.BH) * static_cast<unsigned>(p.pairs), static_cast<unsigned>(p.splits)), C::kThreads, bytes, st>>>(mk, mv, p);
-  if (p.splits > 1) {
-    const JoinParams j{p.part_o, p.part_ml, p.out, p.osb, p.osh, p.oss, p.Hkv, p.rows, p.G, p.splits};
-    if (launch_join<D, QT>(j, int64_t(p.BH) * p.rows, st) != cudaSuccess) return VC_ERR_LAUNCH;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(static_cast<unsigned>(p.whole) + static_cast<unsigned>(p.cut) * static_cast<unsigned>(p.splits));
+  c.blockDim = dim3(C::kThreads);
+  c.dynamicSmemBytes = bytes;
+  c.stream = st;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &early;
+  c.numAttrs = SRC == kUnpacked ? 1 : 0;
+  if (cudaLaunchKernelEx(&c, k, mk, mv, p) != cudaSuccess) return VC_ERR_LAUNCH;
+  if (p.cut > 0) {
+    const JoinParams j{p.part_o, p.part_ml, p.out, p.osb, p.osh, p.oss, p.Hkv, p.rows, p.G, p.splits, p.whole, p.pairs, p.BH};
+    if (launch_join<D, QT>(j, int64_t(p.cut) * 256, st) != cudaSuccess) return VC_ERR_LAUNCH;
   }
   return cudaGetLastError() == cudaSuccess ? VC_OK : VC_ERR_LAUNCH;
 }

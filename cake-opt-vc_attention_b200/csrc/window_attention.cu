@@ -13,8 +13,7 @@ TilePlan plan_of(const WindowAttnArgs& a) {
 }  // namespace
 
 int64_t window_attention_workspace(const WindowAttnArgs& a) {
-  const TilePlan t = plan_of(a);
-  return t.splits == 1 ? 0 : a.B * a.Hq * a.Sq * t.splits * (a.D + 2) * 4;
+  return plan_of(a).part_rows() * (a.D + 2) * 4;
 }
 
 int window_attention(const WindowAttnArgs& a, cudaStream_t st) {
@@ -39,13 +38,10 @@ int window_attention(const WindowAttnArgs& a, cudaStream_t st) {
   p.Sk = a.Sk;
   p.G = static_cast<int>(a.Hq / a.Hkv);
   p.rows = static_cast<int>(a.Sq * p.G);
-  p.pairs = static_cast<int>(t.pairs);
-  p.splits = static_cast<int>(t.splits);
   p.vis = visibility(a.window, a.sinks, a.causal);
   p.scale_log2 = a.sm_scale * kLog2e;
   p.lengths = a.kv_lengths;
-  p.part_o = static_cast<float*>(a.workspace);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + int64_t(p.BH) * p.rows * t.splits * a.D);
+  set_plan(p, t, a.workspace, a.D);
   if (a.dtype == VC_DTYPE_BF16)
     return a.D == 128 ? launch_tiles<128, __nv_bfloat16, __nv_bfloat16, kTensors>(mk, mv, p, st)
                       : launch_tiles<64, __nv_bfloat16, __nv_bfloat16, kTensors>(mk, mv, p, st);
