@@ -61,52 +61,68 @@ __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Eight 16-bit values as four pairs of FP32.
 template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& u, float (&x)[8]) {
+__device__ __forceinline__ void unpack8(const uint4& u, uint64_t (&x)[4]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if constexpr (sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value) {
-      x[2 * i] = bf16_lo(w[i]);
-      x[2 * i + 1] = bf16_hi(w[i]);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      x[i] = pk2f(bf16_lo(w[i]), bf16_hi(w[i]));
     } else {
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
+      x[i] = pk2f(f.x, f.y);
     }
   }
 }
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
-// One chunk of heads a blockIdx.y: HEADS heads of Q, K, V counted through, the
-// same ones in the whole block, D/8 threads a token.  The HEADS loads of a
-// thread are in flight together, and cos and sin are read once for them.
+// i / n, by 32 bits where all i < total allow it.
+__device__ __forceinline__ int sequence_of(int64_t i, int64_t total, int64_t n) {
+  return total <= INT32_MAX ? static_cast<int>(static_cast<unsigned>(i) / static_cast<unsigned>(n)) : static_cast<int>(i / n);
+}
+
+// HEADS heads of Q, of K or of V a blockIdx.y, D/8 threads a token.  The HEADS
+// loads of a thread are in flight together, and cos and sin are read once for
+// them.
 template <int D, typename T, int HEADS>
 __global__ void __launch_bounds__(kThreads, HEADS > 1 ? 4 : 1) kv4_append_kernel(AppendParams p) {
   constexpr int L = D / 8;   // threads a token
   const int64_t token = (int64_t(blockIdx.x) * kThreads + threadIdx.x) / L;
   const int l = threadIdx.x % L, Hkv = static_cast<int>(p.pages.heads), Hq = static_cast<int>(p.Hq);
   const bool live = token < p.B * p.S;
-  const int b = live ? static_cast<int>(token / p.S) : 0;
+  const int b = live ? sequence_of(token, p.B * p.S, p.S) : 0;
   const int64_t t = live ? token - b * p.S : 0;
   const bool write = live && (!p.counts || t < __ldg(p.counts + b));
-  const int c0 = l * 8, first = blockIdx.y * HEADS;
+  const int c0 = l * 8;
+  // the block's heads; everything about them is the same in the whole block
+  const int q_chunks = (Hq + HEADS - 1) / HEADS, kv_chunks = (Hkv + HEADS - 1) / HEADS;
+  int chunk = blockIdx.y;
+  const bool is_q = chunk < q_chunks, is_v = !is_q && chunk >= q_chunks + kv_chunks;
+  chunk -= is_q ? 0 : is_v ? q_chunks + kv_chunks : q_chunks;
+  const int first = chunk * HEADS, count = min(HEADS, (is_q ? Hq : Hkv) - first);
+  const int64_t step = is_q ? p.qsh : is_v ? p.vsh : p.ksh;
+  const T* src = (is_q   ? static_cast<const T*>(p.q) + b * p.qsb + t * p.qss
+                  : is_v ? static_cast<const T*>(p.v) + b * p.vsb + t * p.vss
+                         : static_cast<const T*>(p.k) + b * p.ksb + t * p.kss) + first * step + c0;
   uint4 u[HEADS];
 #pragma unroll
-  for (int i = 0; i < HEADS; ++i) {
-    const int head = first + i;
-    u[i] = make_uint4(0, 0, 0, 0);
-    if (live && head < Hq + 2 * Hkv) {
-      const T* src = head < Hq         ? static_cast<const T*>(p.q) + b * p.qsb + head * p.qsh + t * p.qss
-                     : head < Hq + Hkv ? static_cast<const T*>(p.k) + b * p.ksb + (head - Hq) * p.ksh + t * p.kss
-                                       : static_cast<const T*>(p.v) + b * p.vsb + (head - Hq - Hkv) * p.vsh + t * p.vss;
-      u[i] = __ldg(reinterpret_cast<const uint4*>(src + c0));
-    }
-  }
+  for (int i = 0; i < HEADS; ++i) u[i] = live && i < count ? __ldg(reinterpret_cast<const uint4*>(src + i * step)) : make_uint4(0, 0, 0, 0);
   const int64_t at = int64_t(__ldg(p.lengths + b)) + t;   // index in the sequence
-  // cos and sin of this lane's channels (half style: pair index = channel mod R/2)
+  // cos and sin of this lane's channels (half style: pair index = channel mod R/2).  Every channel becomes
+  // x cos + y s with its partner y and s = -sin (first of the pair) or sin, so that no lanes diverge.
   const int R = p.rot_dim, half = R / 2;
-  float cs[8], sn[8];
-  const bool rotated = c0 < R && first < Hq + Hkv;
+  uint64_t cs[4], sn[4];
+  const bool rotated = c0 < R && !is_v;
   if (rotated) {
     int64_t pos = p.positions ? int64_t(__ldg(p.positions + b * p.S + t)) : at;
     if (pos < 0 || pos >= p.rot_rows) {
@@ -116,79 +132,80 @@ __global__ void __launch_bounds__(kThreads, HEADS > 1 ? 4 : 1) kv4_append_kernel
     const float *cr = p.cos + pos * half, *sr = p.sin + pos * half;
     if (p.interleaved) {
       const float4 a = __ldg(reinterpret_cast<const float4*>(cr + c0 / 2)), d = __ldg(reinterpret_cast<const float4*>(sr + c0 / 2));
-      cs[0] = cs[1] = a.x; cs[2] = cs[3] = a.y; cs[4] = cs[5] = a.z; cs[6] = cs[7] = a.w;
-      sn[0] = sn[1] = d.x; sn[2] = sn[3] = d.y; sn[4] = sn[5] = d.z; sn[6] = sn[7] = d.w;
+      cs[0] = pk2f(a.x, a.x); cs[1] = pk2f(a.y, a.y); cs[2] = pk2f(a.z, a.z); cs[3] = pk2f(a.w, a.w);
+      sn[0] = pk2f(-d.x, d.x); sn[1] = pk2f(-d.y, d.y); sn[2] = pk2f(-d.z, d.z); sn[3] = pk2f(-d.w, d.w);
     } else {
-      const int i0 = c0 < half ? c0 : c0 - half;
+      const bool low = c0 < half;
+      const int i0 = low ? c0 : c0 - half;
 #pragma unroll
-      for (int i = 0; i < 8; i += 4) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(cr + i0 + i)), d = __ldg(reinterpret_cast<const float4*>(sr + i0 + i));
-        cs[i] = a.x; cs[i + 1] = a.y; cs[i + 2] = a.z; cs[i + 3] = a.w;
-        sn[i] = d.x; sn[i + 1] = d.y; sn[i + 2] = d.z; sn[i + 3] = d.w;
+      for (int i = 0; i < 2; ++i) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(cr + i0) + i), d = __ldg(reinterpret_cast<const float4*>(sr + i0) + i);
+        cs[2 * i] = pk2f(a.x, a.y);
+        cs[2 * i + 1] = pk2f(a.z, a.w);
+        sn[2 * i] = low ? pk2f(-d.x, -d.y) : pk2f(d.x, d.y);
+        sn[2 * i + 1] = low ? pk2f(-d.z, -d.w) : pk2f(d.z, d.w);
       }
     }
   }
+  const int64_t record0 = !is_q && write && at >= 0 ? p.pages.record<D>(b, first, at >> 4) : -1;
   const int lane = threadIdx.x & 31;
   const int partner = (lane & ~(L - 1)) | (rotated ? (c0 < half ? l + half / 8 : l - half / 8) : l);
 #pragma unroll
   for (int i = 0; i < HEADS; ++i) {
-    const int head = first + i;
-    if (head >= Hq + 2 * Hkv) break;   // (the same in every thread: the shuffles below are warp-wide)
-    float x[8];
-    unpack8<T>(u[i], x);
-    if (R > 0 && head < Hq + Hkv) {
-      if (p.interleaved) {
-        if (rotated) {
+    if (i >= count) break;   // (the same in every thread: the shuffles below are warp-wide)
+    uint64_t x2[4];
+    unpack8<T>(u[i], x2);
+    if (R > 0 && !is_v) {
+      uint4 w = u[i];
+      if (!p.interleaved) {   // the partner's sixteen bytes in the input type: four shuffles
+        w.x = __shfl_sync(0xffffffffu, w.x, partner);
+        w.y = __shfl_sync(0xffffffffu, w.y, partner);
+        w.z = __shfl_sync(0xffffffffu, w.z, partner);
+        w.w = __shfl_sync(0xffffffffu, w.w, partner);
+      } else {                // the partner is the pair's other half
+        w.x = __funnelshift_l(w.x, w.x, 16);
+        w.y = __funnelshift_l(w.y, w.y, 16);
+        w.z = __funnelshift_l(w.z, w.z, 16);
+        w.w = __funnelshift_l(w.w, w.w, 16);
+      }
+      if (rotated) {
+        uint64_t y2[4];
+        unpack8<T>(w, y2);
 #pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            const float a = x[j], c = x[j + 1];
-            x[j] = __fsub_rn(__fmul_rn(a, cs[j]), __fmul_rn(c, sn[j]));
-            x[j + 1] = __fadd_rn(__fmul_rn(c, cs[j]), __fmul_rn(a, sn[j]));
-          }
-        }
-      } else {
-        // the partner's sixteen bytes in the input type: four shuffles
-        uint4 w;
-        w.x = __shfl_sync(0xffffffffu, u[i].x, partner);
-        w.y = __shfl_sync(0xffffffffu, u[i].y, partner);
-        w.z = __shfl_sync(0xffffffffu, u[i].z, partner);
-        w.w = __shfl_sync(0xffffffffu, u[i].w, partner);
-        if (rotated) {
-          float y[8];
-          unpack8<T>(w, y);
-          if (c0 < half) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = __fsub_rn(__fmul_rn(x[j], cs[j]), __fmul_rn(y[j], sn[j]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = __fadd_rn(__fmul_rn(x[j], cs[j]), __fmul_rn(y[j], sn[j]));
-          }
+        for (int j = 0; j < 4; ++j) {
+          // (scalar additions: the packed ones were contracted with a product, which then is not rounded)
+          uint32_t a, d, e, f;
+          up2(f2_mul(x2[j], cs[j]), a, d);
+          up2(f2_mul(y2[j], sn[j]), e, f);
+          x2[j] = pk2f(__fadd_rn(__uint_as_float(a), __uint_as_float(e)), __fadd_rn(__uint_as_float(d), __uint_as_float(f)));
         }
       }
     }
-    if (head < Hq) {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t a, d;
+      up2(x2[j], a, d);
+      x[2 * j] = __uint_as_float(a);
+      x[2 * j + 1] = __uint_as_float(d);
+    }
+    if (is_q) {
       if (live) {
-        T* dst = static_cast<T*>(p.q_out) + b * p.osb + head * p.osh + t * p.oss + c0;
+        T* dst = static_cast<T*>(p.q_out) + b * p.osb + t * p.oss + (first + i) * p.osh + c0;
         *reinterpret_cast<uint4*>(dst) =
             make_uint4(pack16<T>(x[0], x[1]), pack16<T>(x[2], x[3]), pack16<T>(x[4], x[5]), pack16<T>(x[6], x[7]));
       }
       continue;
     }
-    float lo = x[0], hi = x[0];
-#pragma unroll
-    for (int j = 1; j < 8; ++j) {
-      lo = min_nan(lo, x[j]);
-      hi = max_nan(hi, x[j]);
-    }
+    float lo = min3_nan(min3_nan(x[0], x[1], x[2]), min3_nan(x[3], x[4], x[5]), min_nan(x[6], x[7]));
+    float hi = max3_nan(max3_nan(x[0], x[1], x[2]), max3_nan(x[3], x[4], x[5]), max_nan(x[6], x[7]));
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) {
       lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
       hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
     if (write) {
-      const bool is_v = head >= Hq + Hkv;
-      const int64_t rec = at < 0 ? -1 : p.pages.record<D>(b, head - Hq - (is_v ? Hkv : 0), at >> 4);
-      if (rec < 0) {
+      if (record0 < 0) {
         raise_error(kErrBadIndex);
         continue;
       }
@@ -200,15 +217,22 @@ __global__ void __launch_bounds__(kThreads, HEADS > 1 ? 4 : 1) kv4_append_kernel
         s = 0.f;
         s16 = __float2bfloat16_rn(0.f);
       }
-      const float inv = s == 0.f ? 0.f : __fdiv_rn(1.f, s);
+      const float inv = s == 0.f ? 0.f : __frcp_rn(s);
+      // clamped to [0, 15] (NaN -> 0) before it is rounded, which gives the same: adding 1.5 * 2^23 rounds to
+      // the nearest integer, ties to even, and leaves it in the low bits; 16^j times the sum's other bits,
+      // 0x4B400000, only reaches bits from 22 on and is taken off at the end
+      const uint64_t m2 = pk2f(m, m), inv2 = pk2f(inv, inv), magic = pk2f(12582912.f, 12582912.f);
       uint32_t w = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float c = rintf(__fmul_rn(__fsub_rn(x[j], m), inv));
-        w |= static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f)) << (4 * j);   // NaN -> 0
+      for (int j = 0; j < 4; ++j) {
+        uint32_t a, d;
+        up2(f2_mul(f2_sub(x2[j], m2), inv2), a, d);
+        up2(f2_add(pk2f(fminf(fmaxf(__uint_as_float(a), 0.f), 15.f), fminf(fmaxf(__uint_as_float(d), 0.f), 15.f)), magic), a, d);
+        w += (a << (8 * j)) + (d << (8 * j + 4));
       }
+      w -= 0x4B400000u * 0x11111111u;
       const int slot = static_cast<int>(at & 15);
-      uint8_t* r = p.pages.pool + rec;
+      uint8_t* r = p.pages.pool + record0 + (int64_t(i) << (p.pages.page_shift - 4)) * Kv4Rec<D>::kBytes;
       *reinterpret_cast<uint32_t*>(r + (is_v ? Kv4Rec<D>::kV : Kv4Rec<D>::kK) + slot * Kv4Rec<D>::kCodeRow + l * 4) = w;
       if ((l & 7) == 0) {
         const uint32_t sm = uint32_t(__bfloat16_as_ushort(s16)) | (uint32_t(__bfloat16_as_ushort(m16)) << 16);
@@ -236,7 +260,7 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(ReadParams p) {
   const int h = blockIdx.y, n = static_cast<int>(p.N);
   const int64_t row = i / L;
   if (row >= p.B * p.N) return;
-  const int b = static_cast<int>(row / n), t = static_cast<int>(row - int64_t(b) * n);
+  const int b = sequence_of(row, p.B * n, n), t = static_cast<int>(row - int64_t(b) * n);
   const int64_t at = (p.start ? int64_t(__ldg(p.start + b)) : 0) + t;
   const int64_t rec = at < 0 ? -1 : p.pages.record<D>(b, h, at >> 4);
   uint4 codes = make_uint4(0, 0, 0, 0);
@@ -275,11 +299,12 @@ int kv4_append(const Kv4AppendArgs& a, cudaStream_t st) {
   AppendParams p{a.k, a.v, a.q, a.q_out, a.ksb, a.ksh, a.kss, a.vsb, a.vsh, a.vss, a.qsb, a.qsh, a.qss, a.osb, a.osh,
                  a.oss, a.cos, a.sin, a.rot_rows, static_cast<int>(a.rot_dim), a.interleaved, a.positions, a.lengths,
                  a.counts, kv4_pages(a.cache), a.cache.B, a.S, a.q ? a.Hq : 0};
-  const int64_t heads = p.Hq + 2 * a.cache.Hkv, threads = a.cache.B * a.S * (a.D / 8);
+  const int64_t threads = a.cache.B * a.S * (a.D / 8);
   const unsigned blocks = static_cast<unsigned>((threads + kThreads - 1) / kThreads);
+  auto chunks = [&](int64_t n) { return static_cast<unsigned>((p.Hq + n - 1) / n + 2 * ((a.cache.Hkv + n - 1) / n)); };
   // four heads a thread where that still fills the GPU several times, else one (few tokens: latency)
-  const bool many = blocks * ((heads + 3) / 4) >= 4 * 148;
-  const dim3 grid(blocks, static_cast<unsigned>(many ? (heads + 3) / 4 : heads));
+  const bool many = blocks * chunks(4) >= 4 * 148;
+  const dim3 grid(blocks, chunks(many ? 4 : 1));
   auto go = [&](auto tag, auto dim) {
     using T = decltype(tag);
     constexpr int D = decltype(dim)::value;
