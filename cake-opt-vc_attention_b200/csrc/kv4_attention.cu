@@ -1,7 +1,7 @@
 // Attention of a few rows per K/V head over the paged 4-bit cache: decoding
 // (one token a sequence) and drafts.
 //
-// One CTA takes up to 8*NT rows (query tokens x the query heads that share a
+// One CTA takes the 8*NT rows at most (query tokens x the query heads that share a
 // K/V head) of one sequence and K/V head, and a share of its keys; each of its
 // warps streams tiles of 32 keys on its own, with its own running maximum, and
 // the warps (then the splits, in a second kernel) are joined at the end.
@@ -142,7 +142,6 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int split = blockIdx.x;
   const int bh = blockIdx.y, b = bh / static_cast<int>(p.pages.heads), hk = bh - b * static_cast<int>(p.pages.heads);
-  const int row0 = blockIdx.z * 8 * NT;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar) + warp * L::kStages;
   if (lane < L::kStages) mbar_init(&bars[lane], 1);
   fence_barrier_init();
@@ -154,11 +153,11 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
 
   // keys that some row of this CTA sees, in tiles of 32: sinks [0, nsink) and [main0, main0 + nmain)
   int nsink = 0, main0 = 0, ntiles = 0;
-  const int last_row = min(row0 + 8 * NT, live_rows) - 1;
+  const int last_row = live_rows - 1;
   // rows see all of a tile iff it ends before the first row's last key and starts after the last row's first
   int all_hi = 0, all_lo = 0, lo = 0, sink_end = 0;
-  if (last_row >= row0) {
-    const KeyRanges a = visible_keys(p.vis, len - nq + row0 / p.G, len), z = visible_keys(p.vis, len - nq + last_row / p.G, len);
+  if (last_row >= 0) {
+    const KeyRanges a = visible_keys(p.vis, len - nq, len), z = visible_keys(p.vis, len - nq + last_row / p.G, len);
     const int hi = z.hi;   // the last row reaches furthest, the first starts first
     lo = p.vis.window ? a.lo : 0;
     sink_end = p.vis.window ? min(p.vis.sinks, hi) : 0;
@@ -208,7 +207,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
   uint4* qs = reinterpret_cast<uint4*>(smem + L::kOffQ);
   float4* cols = reinterpret_cast<float4*>(smem + L::kOffCol);   // by row: factor, scaled sum of Q by group
   if (warp < NT) {
-    const int nt = warp, row = row0 + nt * 8 + r;
+    const int nt = warp, row = nt * 8 + r;
     float x[NG][16];
     float big = 0.f, sum[NG];
     const bool have = row < p.rows;
@@ -418,7 +417,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const int row = row0 + nt * 8 + 2 * c + j;
+              const int row = nt * 8 + 2 * c + j;
               const KeyRanges v = visible_keys(p.vis, len - nq + row / p.G, len);
               if (!(((have >> k) & 1u) && key < v.hi && (key >= v.lo || key < v.sink_end))) x[k][nt][2 * half + j] = -INFINITY;
             }
@@ -598,7 +597,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
     __syncthreads();
     // a warp joins rows warp, warp + kWarps, ... of this n-tile; lane: D/32 channels
     for (int wr = warp; wr < 8; wr += kWarps) {
-      const int row = row0 + nt * 8 + wr;
+      const int row = nt * 8 + wr;
       if (row >= p.rows) break;
       float top = -INFINITY, sum = 0.f;
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, stat[w * 8 * NT + nt * 8 + wr].x);
@@ -635,19 +634,17 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
 }
 
 struct Plan {
-  int nt, blocks, splits;
+  int nt, splits;
 };
 
-// Rows a CTA (8, 16, 24 or 32) and splits of the keys: about one CTA for each
-// that fits the GPU, and at least one tile a warp each.
+// Tiles of eight rows (one to four) and splits of the keys.
 Plan plan_of(const Kv4AttnArgs& a) {
   const int64_t rows = a.Sq * (a.Hq / a.cache.Hkv);
   Plan r;
-  r.nt = static_cast<int>(rows >= 25 ? 4 : (rows + 7) / 8);
-  r.blocks = static_cast<int>((rows + 8 * r.nt - 1) / (8 * r.nt));
+  r.nt = static_cast<int>((rows + 7) / 8);
   int64_t keys = kv4_most(a.cache, a.max_length);
   if (a.window > 0) keys = min64(keys, a.window + a.Sq + a.sinks + 2 * kTile);
-  const int64_t tiles = (keys + kTile - 1) / kTile, items = a.cache.B * a.cache.Hkv * r.blocks;
+  const int64_t tiles = (keys + kTile - 1) / kTile, items = a.cache.B * a.cache.Hkv;
   const int64_t fit = 148 * (r.nt == 1 ? 4 : 2), warps = r.nt == 2 ? 6 : 4;
   // One sequence: its heads' shares are alike, and half a wave of CTAs is enough (37741 keys of 4 heads: 14.6 us;
   // a whole wave, whose results take longer to join, 17.9; a third 17.9).  Several: their lengths differ, so
@@ -660,9 +657,13 @@ Plan plan_of(const Kv4AttnArgs& a) {
   return r;
 }
 
-// From this many rows a K/V head on, the tile kernel.
-constexpr int64_t kTileRows = 64;
-bool use_tiles(const Kv4AttnArgs& a) { return a.Sq * (a.Hq / a.cache.Hkv) >= kTileRows; }
+// More rows a K/V head than this kernel's accumulators hold go to the tile
+// kernel: a second CTA would read the keys again.  D 128, one sequence of 16384
+// (28/4 heads): 28 rows 20 us here, 22 there; 49 rows 30 in two CTAs, 24 there.
+// 16 sequences up to 8192 (32/8 heads): 32 rows 122 and 146, 48 rows 203 and
+// 147.  D 64, 8 up to 4096 (24/24 heads): 32 rows 49 and 75, 48 rows 81 and 75.
+constexpr int64_t kMostRows = 32;
+bool use_tiles(const Kv4AttnArgs& a) { return a.Sq * (a.Hq / a.cache.Hkv) > kMostRows; }
 
 int launched() { return cudaGetLastError() == cudaSuccess ? VC_OK : VC_ERR_LAUNCH; }
 
@@ -672,7 +673,7 @@ int launch_decode(const DecodeParams& p, const Plan& plan, int64_t BH, cudaStrea
   constexpr int bytes = DecodeCfg<D, NT>::kBytes;
   static std::atomic<uint64_t> ready{0};
   if (!allow_smem(reinterpret_cast<const void*>(k), bytes, ready)) return VC_ERR_LAUNCH;
-  k<<<dim3(plan.splits, static_cast<unsigned>(BH), plan.blocks), DecodeCfg<D, NT>::kThreads, bytes, st>>>(p);
+  k<<<dim3(plan.splits, static_cast<unsigned>(BH)), DecodeCfg<D, NT>::kThreads, bytes, st>>>(p);
   if (plan.splits > 1) {
     const JoinParams j{p.part_o, p.part_ml, p.out, p.osb, p.osh, p.oss, p.pages.heads, p.rows, p.G, p.splits};
     if (launch_join<D, T>(j, BH * p.rows, st) != cudaSuccess) return VC_ERR_LAUNCH;

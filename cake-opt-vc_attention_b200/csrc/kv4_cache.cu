@@ -302,8 +302,9 @@ int kv4_append(const Kv4AppendArgs& a, cudaStream_t st) {
   const int64_t threads = a.cache.B * a.S * (a.D / 8);
   const unsigned blocks = static_cast<unsigned>((threads + kThreads - 1) / kThreads);
   auto chunks = [&](int64_t n) { return static_cast<unsigned>((p.Hq + n - 1) / n + 2 * ((a.cache.Hkv + n - 1) / n)); };
-  // four heads a thread where that still fills the GPU several times, else one (few tokens: latency)
-  const bool many = blocks * chunks(4) >= 4 * 148;
+  // four heads a thread where that still fills the SMs, else one: 28/4 heads, D 128, 256 tokens (144 blocks of
+  // four heads) 3.6 us with four and 2.8 with one, 512 tokens (288) 3.8 and 4.2, 2048 tokens 7.2 and 10.3
+  const bool many = blocks * chunks(4) >= 3 * 148 / 2;
   const dim3 grid(blocks, chunks(many ? 4 : 1));
   auto go = [&](auto tag, auto dim) {
     using T = decltype(tag);

@@ -6,9 +6,10 @@
 // the dequantising warps of each do the same work again, and they take issue
 // slots from the softmax: the chunk of 1024 tokens over 16384 (28/4 heads,
 // D 128; 28 CTAs a head) takes 396 us that way and 251 us unpacked first,
-// of which the unpacking is about 12.  So: unpack when a head has two CTAs or
-// more and the FP16 tiles fit kMostUnpacked bytes; the workspace is otherwise
-// only needed for split keys.
+// of which the unpacking is about 12.  With one CTA a head it is 32 us fused and
+// 34 unpacked, with two 49 and 45, with four 74 and 63.  So: unpack when a head
+// has two CTAs or more.  The FP16 tiles take 3.6 times the cache's bytes, so
+// that only up to kMostUnpacked bytes of them (262144 tokens of 8 heads, D 128).
 #include "tile_attention.cuh"
 
 namespace vcb {
