@@ -1,0 +1,326 @@
+// The serving operators' calls from Python without the interpreter's share.
+//
+// A decoding step for one sequence takes the GPU a few microseconds, and the
+// wrappers in ops.py take the host 13 to 19 us a call: some sixty attribute
+// reads, an allocation or two and forty converted arguments.  This extension
+// does the same in C++ for arguments that need no conversion (5 to 8 us).
+// What it does not take, it leaves to the wrapper by returning NotImplemented
+// before anything is allocated or launched: copies of odd strides, conversions,
+// ``out``, another current device, and every refusal with its message.  A
+// library call that fails returns its status (an int) for the wrapper to raise.
+//
+// The library's functions are the ones the Python side has loaded (bind()), so
+// that there is one library and one set of error words.
+#include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
+#include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <cmath>
+
+#include "vc_b200.h"
+
+namespace {
+
+decltype(&vc_kv4_append) kv4_append_fn;
+decltype(&vc_kv4_read) kv4_read_fn;
+decltype(&vc_kv4_attention_workspace_bytes) kv4_workspace_fn;
+decltype(&vc_kv4_attention_fwd) kv4_attention_fn;
+decltype(&vc_window_attention_workspace_bytes) window_workspace_fn;
+decltype(&vc_window_attention_fwd) window_fn;
+
+PyObject* not_here() { Py_RETURN_NOTIMPLEMENTED; }
+
+int dtype_code(at::ScalarType t) {
+  return t == at::kHalf ? int(VC_DTYPE_F16) : t == at::kBFloat16 ? int(VC_DTYPE_BF16) : t == at::kFloat ? int(VC_DTYPE_F32) : -1;
+}
+
+// A plain CUDA tensor that no gradient is asked for; nullptr: not one.
+const at::Tensor* cuda_tensor(PyObject* o) {
+  if (!THPVariable_CheckExact(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda() || t.layout() != at::kStrided || (t.requires_grad() && c10::GradMode::is_enabled())) return nullptr;
+  return &t;
+}
+
+bool layout_of(PyObject* o, bool& hnd) {
+  if (!PyUnicode_Check(o)) return false;
+  if (PyUnicode_CompareWithASCIIString(o, "HND") == 0) return hnd = true;
+  hnd = false;
+  return PyUnicode_CompareWithASCIIString(o, "NHD") == 0;
+}
+
+// [B,H,S,D] of a tensor in either layout, with strides and address as the
+// library takes them (axes of one element address nothing: a row's stride).
+struct View {
+  void* p;
+  int64_t B, H, S, D, sb, sh, ss;
+};
+bool view_of(PyObject* o, bool hnd, at::ScalarType type, at::Device dev, View& v) {
+  const at::Tensor* t = cuda_tensor(o);
+  if (!t || t->scalar_type() != type || t->device() != dev || t->dim() != 4) return false;
+  const auto n = t->sizes(), s = t->strides();
+  const int h = hnd ? 1 : 2, q = hnd ? 2 : 1;
+  v = {t->data_ptr(), n[0], n[h], n[q], n[3], s[0], s[h], s[q]};
+  if (v.B < 2) v.sb = v.D;
+  if (v.H < 2) v.sh = v.D;
+  if (v.S < 2) v.ss = v.D;
+  return v.B > 0 && v.H > 0 && v.S > 0 && v.D > 0 && s[3] == 1 && v.ss > 0 && ((v.sb | v.sh | v.ss) & 7) == 0 &&
+         (reinterpret_cast<uintptr_t>(v.p) & 15) == 0;
+}
+
+// An int32 tensor of B (or B x S) elements, contiguous; None: null.
+bool ints_of(PyObject* o, at::Device dev, int64_t B, int64_t S, const int32_t*& p) {
+  p = nullptr;
+  if (o == Py_None) return true;
+  const at::Tensor* t = cuda_tensor(o);
+  if (!t || t->scalar_type() != at::kInt || t->device() != dev || !t->is_contiguous()) return false;
+  const auto n = t->sizes();
+  if (S < 0 ? n.size() != 1 || n[0] != B : n.size() != 2 || n[0] != B || n[1] != S) return false;
+  p = static_cast<const int32_t*>(t->data_ptr());
+  return true;
+}
+
+struct Cache {
+  uint8_t* pool;
+  const int32_t* table;
+  int64_t pages, H, D, page, B, width;
+};
+bool cache_of(PyObject* pool, PyObject* table, Cache& c, at::Device& dev) {
+  const at::Tensor *p = cuda_tensor(pool), *t = cuda_tensor(table);
+  if (!p || !t || p->scalar_type() != at::kByte || p->dim() != 4 || !p->is_contiguous() || t->scalar_type() != at::kInt ||
+      t->dim() != 2 || !t->is_contiguous() || p->device() != t->device())
+    return false;
+  const auto n = p->sizes();
+  if (n[3] != 18 * 64 && n[3] != 18 * 128) return false;
+  dev = p->device();
+  c = {static_cast<uint8_t*>(p->data_ptr()), static_cast<const int32_t*>(t->data_ptr()), n[0], n[1], n[3] / 18, n[2] * 16,
+       t->size(0), t->size(1)};
+  return c.B > 0 && dev.index() == c10::cuda::current_device();
+}
+
+// None -> absent (0); else an int of at least ``least``.
+bool count_of(PyObject* o, int64_t least, int64_t& v) {
+  v = 0;
+  if (o == Py_None) return true;
+  if (!PyLong_CheckExact(o)) return false;
+  int over = 0;
+  v = PyLong_AsLongLongAndOverflow(o, &over);
+  return !over && v >= least && v <= INT32_MAX;
+}
+bool flag_of(PyObject* o, int& v) {
+  v = o == Py_True;
+  return v || o == Py_False;
+}
+bool scale_of(PyObject* o, int64_t D, float& v) {
+  const double s = o == Py_None ? 1.0 / std::sqrt(double(D)) : PyFloat_CheckExact(o) ? PyFloat_AS_DOUBLE(o) : 0.0;
+  v = float(s);
+  return s > 0 && s <= 3.4028234663852886e38;
+}
+
+template <typename F>
+PyObject* finish(F&& call, PyObject* out) {
+  if (!out) return nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS;
+  rc = call();
+  Py_END_ALLOW_THREADS;
+  if (rc == VC_OK) return out;
+  Py_DECREF(out);
+  return PyLong_FromLong(rc);
+}
+
+void* stream_of(at::Device dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
+
+// pool, page_table, lengths, k, v, q, cos, sin, positions, counts, interleaved, layout
+PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Cache c;
+  at::Device dev(at::kCUDA);
+  bool hnd;
+  View k, v, q{};
+  int interleaved;
+  const int32_t *lengths, *positions, *counts;
+  if (n != 12 || !cache_of(a[0], a[1], c, dev) || !layout_of(a[11], hnd) || !flag_of(a[10], interleaved)) return not_here();
+  const at::Tensor* first = cuda_tensor(a[3]);
+  if (!first) return not_here();
+  const at::ScalarType type = first->scalar_type();
+  if ((type != at::kHalf && type != at::kBFloat16) || !view_of(a[3], hnd, type, dev, k) || !view_of(a[4], hnd, type, dev, v)) return not_here();
+  if (k.B != c.B || k.H != c.H || k.D != c.D || v.B != c.B || v.H != c.H || v.D != c.D || v.S != k.S) return not_here();
+  if (a[2] == Py_None || !ints_of(a[2], dev, c.B, -1, lengths) || !ints_of(a[8], dev, c.B, k.S, positions) ||
+      !ints_of(a[9], dev, c.B, -1, counts))
+    return not_here();
+  const float *cos = nullptr, *sin = nullptr;
+  int64_t rows = 0, rot = 0;
+  if (a[6] != Py_None || a[7] != Py_None) {
+    const at::Tensor *x = cuda_tensor(a[6]), *y = cuda_tensor(a[7]);
+    if (!x || !y || x->dim() != 2 || x->sizes() != y->sizes() || x->scalar_type() != at::kFloat || y->scalar_type() != at::kFloat ||
+        x->device() != dev || y->device() != dev || !x->is_contiguous() || !y->is_contiguous())
+      return not_here();
+    cos = static_cast<const float*>(x->data_ptr());
+    sin = static_cast<const float*>(y->data_ptr());
+    rows = x->size(0);
+    rot = 2 * x->size(1);
+    if (rot % 16 || rot > c.D || rot < 16 || rows < 1 || ((reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) & 15)) return not_here();
+  }
+  PyObject* out = Py_None;
+  void* op = nullptr;
+  int64_t osb = c.D, osh = c.D, oss = c.D;
+  if (a[5] != Py_None) {
+    if (!view_of(a[5], hnd, type, dev, q) || q.B != c.B || q.S != k.S || q.D != c.D || q.H % c.H) return not_here();
+    const at::Tensor& t = THPVariable_Unpack(a[5]);
+    at::Tensor o = at::empty(t.sizes(), t.options());
+    op = o.data_ptr();
+    osb = q.H * q.S * q.D;
+    osh = hnd ? q.S * q.D : q.D;
+    oss = hnd ? q.D : q.H * q.D;
+    out = THPVariable_Wrap(std::move(o));
+  } else {
+    q.sb = q.sh = q.ss = c.D;
+    Py_INCREF(out);
+  }
+  void* st = stream_of(dev);
+  return finish([&] {
+    return kv4_append_fn(k.p, v.p, q.p, op, dtype_code(type), c.B, q.H, c.H, k.S, c.D, k.sb, k.sh, k.ss, v.sb, v.sh, v.ss, q.sb, q.sh,
+                         q.ss, osb, osh, oss, cos, sin, rows, rot, interleaved, positions, lengths, counts, c.pool, c.pages, c.page,
+                         c.table, c.width, st);
+  }, out);
+  END_HANDLE_TH_ERRORS
+}
+
+// pool, page_table, start, count, dtype, layout
+PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Cache c;
+  at::Device dev(at::kCUDA);
+  bool hnd;
+  int64_t N;
+  const int32_t* start;
+  if (n != 6 || !cache_of(a[0], a[1], c, dev) || !layout_of(a[5], hnd) || !THPDtype_Check(a[4]) || a[3] == Py_None ||
+      !count_of(a[3], 1, N) || !ints_of(a[2], dev, c.B, -1, start))
+    return not_here();
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(a[4])->scalar_type;
+  const int code = dtype_code(type);
+  if (code < 0) return not_here();
+  const auto o = at::TensorOptions().dtype(type).device(dev);
+  const int64_t shape[4] = {c.B, hnd ? c.H : N, hnd ? N : c.H, c.D};
+  at::Tensor k = at::empty(shape, o), v = at::empty(shape, o);
+  void *kp = k.data_ptr(), *vp = v.data_ptr(), *st = stream_of(dev);
+  const int64_t sb = c.H * N * c.D, sh = hnd ? N * c.D : c.D, ss = hnd ? c.D : c.H * c.D;
+  PyObject* out = PyTuple_New(2);
+  if (!out) return nullptr;
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(k)));
+  PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(v)));
+  return finish([&] {
+    return kv4_read_fn(c.pool, c.pages, c.page, c.table, c.width, start, c.B, c.H, N, c.D, kp, vp, code, sb, sh, ss, sb, sh, ss, st);
+  }, out);
+  END_HANDLE_TH_ERRORS
+}
+
+at::Tensor workspace(int64_t bytes, at::Device dev) {
+  return bytes > 0 ? at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(dev)) : at::Tensor();
+}
+
+// q, pool, page_table, lengths, q_lengths, causal, window, sinks, sm_scale, max_length, layout
+PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Cache c;
+  at::Device dev(at::kCUDA);
+  bool hnd;
+  View q;
+  int causal;
+  int64_t window, sinks, most;
+  float scale;
+  const int32_t *lengths, *q_lengths;
+  if (n != 11 || !cache_of(a[1], a[2], c, dev) || !layout_of(a[10], hnd)) return not_here();
+  const at::Tensor* t = cuda_tensor(a[0]);
+  if (!t) return not_here();
+  const at::ScalarType type = t->scalar_type();
+  if ((type != at::kHalf && type != at::kBFloat16) || !view_of(a[0], hnd, type, dev, q) || q.B != c.B || q.D != c.D || c.H < 1 || q.H % c.H)
+    return not_here();
+  if (a[3] == Py_None || !ints_of(a[3], dev, c.B, -1, lengths) || !ints_of(a[4], dev, c.B, -1, q_lengths) || !flag_of(a[5], causal) ||
+      !count_of(a[6], 1, window) || a[7] == Py_None || !count_of(a[7], 0, sinks) || !scale_of(a[8], c.D, scale) || !count_of(a[9], 0, most))
+    return not_here();
+  const int64_t held = c.width * c.page;
+  if (a[9] == Py_None || most > held) most = held;
+  const int64_t bytes = kv4_workspace_fn(c.B, q.H, c.H, q.S, c.D, causal, window, sinks, c.page, c.width, most);
+  at::Tensor ws = workspace(bytes, dev), o = at::empty(t->sizes(), t->options());
+  void *wp = bytes > 0 ? ws.data_ptr() : nullptr, *op = o.data_ptr(), *st = stream_of(dev);
+  const int64_t osb = q.H * q.S * q.D, osh = hnd ? q.S * q.D : q.D, oss = hnd ? q.D : q.H * q.D;
+  return finish([&] {
+    return kv4_attention_fn(q.p, dtype_code(type), c.B, q.H, c.H, q.S, c.D, q.sb, q.sh, q.ss, c.pool, c.pages, c.page, c.table, c.width,
+                            lengths, q_lengths, causal, window, sinks, most, scale, op, osb, osh, oss, wp, bytes, st);
+  }, THPVariable_Wrap(std::move(o)));
+  END_HANDLE_TH_ERRORS
+}
+
+// q, k, v, window, sinks, causal, kv_lengths, sm_scale, layout
+PyObject* window_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  bool hnd;
+  View q, k, v;
+  int causal;
+  int64_t window, sinks;
+  float scale;
+  const int32_t* lengths;
+  const at::Tensor* t = n == 9 ? cuda_tensor(a[0]) : nullptr;
+  if (!t || !layout_of(a[8], hnd)) return not_here();
+  const at::ScalarType type = t->scalar_type();
+  const at::Device dev = t->device();
+  if ((type != at::kHalf && type != at::kBFloat16) || dev.index() != c10::cuda::current_device() || !view_of(a[0], hnd, type, dev, q) ||
+      !view_of(a[1], hnd, type, dev, k) || !view_of(a[2], hnd, type, dev, v))
+    return not_here();
+  if ((q.D != 64 && q.D != 128) || k.B != q.B || k.D != q.D || v.B != q.B || v.H != k.H || v.S != k.S || v.D != q.D || q.H % k.H)
+    return not_here();
+  if (!count_of(a[3], 1, window) || a[4] == Py_None || !count_of(a[4], 0, sinks) || !flag_of(a[5], causal) ||
+      !ints_of(a[6], dev, q.B, -1, lengths) || !scale_of(a[7], q.D, scale))
+    return not_here();
+  const int64_t bytes = window_workspace_fn(q.B, q.H, k.H, q.S, k.S, q.D, causal, window, sinks);
+  at::Tensor ws = workspace(bytes, dev), o = at::empty(t->sizes(), t->options());
+  void *wp = bytes > 0 ? ws.data_ptr() : nullptr, *op = o.data_ptr(), *st = stream_of(dev);
+  const int64_t osb = q.H * q.S * q.D, osh = hnd ? q.S * q.D : q.D, oss = hnd ? q.D : q.H * q.D;
+  return finish([&] {
+    return window_fn(q.p, k.p, v.p, dtype_code(type), q.B, q.H, k.H, q.S, k.S, q.D, q.sb, q.sh, q.ss, k.sb, k.sh, k.ss, v.sb, v.sh, v.ss,
+                     lengths, causal, window, sinks, scale, op, osb, osh, oss, wp, bytes, st);
+  }, THPVariable_Wrap(std::move(o)));
+  END_HANDLE_TH_ERRORS
+}
+
+// The addresses of the six library functions, in the order below.
+PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 6) {
+    PyErr_SetString(PyExc_TypeError, "bind takes six addresses");
+    return nullptr;
+  }
+  void* p[6];
+  for (int i = 0; i < 6; ++i) {
+    p[i] = PyLong_AsVoidPtr(a[i]);
+    if (!p[i]) {
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: null address");
+      return nullptr;
+    }
+  }
+  kv4_append_fn = reinterpret_cast<decltype(kv4_append_fn)>(p[0]);
+  kv4_read_fn = reinterpret_cast<decltype(kv4_read_fn)>(p[1]);
+  kv4_workspace_fn = reinterpret_cast<decltype(kv4_workspace_fn)>(p[2]);
+  kv4_attention_fn = reinterpret_cast<decltype(kv4_attention_fn)>(p[3]);
+  window_workspace_fn = reinterpret_cast<decltype(window_workspace_fn)>(p[4]);
+  window_fn = reinterpret_cast<decltype(window_fn)>(p[5]);
+  Py_RETURN_NONE;
+}
+
+PyMethodDef kMethods[] = {
+    {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(bind)), METH_FASTCALL, nullptr},
+    {"kv4_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(append)), METH_FASTCALL, nullptr},
+    {"kv4_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(read)), METH_FASTCALL, nullptr},
+    {"kv4_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(attention)), METH_FASTCALL, nullptr},
+    {"window_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(window_attention)), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_serving_calls", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__serving_calls() { return PyModule_Create(&kModule); }

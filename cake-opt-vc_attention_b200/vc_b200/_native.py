@@ -7,10 +7,12 @@ VC_ERR_ARG / VC_ERR_WORKSPACE -> ValueError, others -> RuntimeError.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libvc_b200.so"
+CALLS_PATH = LIB_PATH.with_name("_serving_calls.so")
 
 VC_OK, VC_ERR_ARG, VC_ERR_LAUNCH, VC_ERR_UNSUPPORTED, VC_ERR_WORKSPACE = 0, 1, 2, 3, 4
 VC_DTYPE_F16, VC_DTYPE_BF16, VC_DTYPE_F32 = 0, 1, 2
@@ -59,6 +61,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_calls = None
 _lock = threading.Lock()
 
 
@@ -90,6 +93,27 @@ def load(build_if_missing: bool = False):
             raise NativeLibraryMissing("libvc_b200.so API version mismatch; rebuild it")
         _lib = lib
         return lib
+
+
+def calls():
+    """The extension ``_serving_calls``, bound to the loaded library; raise if unavailable."""
+    global _calls
+    if _calls is not None:
+        return _calls
+    lib = load()
+    with _lock:
+        if _calls is not None:
+            return _calls
+        if not CALLS_PATH.exists():
+            raise NativeLibraryMissing(f"{CALLS_PATH} is missing. Build it with `python -m vc_b200.build`.")
+        spec = importlib.util.spec_from_file_location("_serving_calls", CALLS_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(*(C.cast(getattr(lib, name), C.c_void_p).value for name in (
+            "vc_kv4_append", "vc_kv4_read", "vc_kv4_attention_workspace_bytes", "vc_kv4_attention_fwd",
+            "vc_window_attention_workspace_bytes", "vc_window_attention_fwd")))
+        _calls = module
+        return module
 
 
 def last_error() -> str:

@@ -2,7 +2,9 @@
 
 The library is a plain C-ABI shared object (see include/vc_b200.h); Python
 loads it with ctypes.  Objects are compiled in parallel and relinked only when
-a source or header is newer than the library.
+a source or header is newer than the library.  ``_serving_calls.so`` beside it
+is a small CPython extension (host code, g++ with torch's headers) through
+which the serving operators are called.
 
     python -m vc_b200.build [--force] [--verbose]
 """
@@ -14,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -22,6 +25,7 @@ REPO = ROOT.parent
 CSRC = ROOT / "csrc"
 INCLUDE = REPO / "include"
 LIB = PKG / "libvc_b200.so"
+CALLS = PKG / "_serving_calls.so"
 OBJ_DIR = ROOT / "_build"
 SOURCES = ["capi.cu", "prep_qk.cu", "prep_hadamard.cu", "prep_v.cu", "cluster.cu", "attention.cu", "tensor_peak.cu",
            "kv4_cache.cu", "kv4_attention.cu", "kv4_chunk.cu",
@@ -42,13 +46,13 @@ def nvcc() -> str:
 
 def _deps() -> list[Path]:
     return sorted(list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) +
-                  list(INCLUDE.glob("*.h")))
+                  list(CSRC.glob("*.cpp")) + list(INCLUDE.glob("*.h")))
 
 
 def needs_build() -> bool:
-    if not LIB.exists():
+    if not LIB.exists() or not CALLS.exists():
         return True
-    t = LIB.stat().st_mtime
+    t = min(LIB.stat().st_mtime, CALLS.stat().st_mtime)
     return any(p.stat().st_mtime > t for p in _deps())
 
 
@@ -61,12 +65,30 @@ def _compile(src: str, verbose: bool) -> tuple[str, str]:
     return str(obj), (r.stderr if verbose else "")
 
 
+def _build_calls() -> None:
+    import torch
+    home = Path(torch.__file__).resolve().parent
+    include = [home / "include", home / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"],
+               Path(nvcc()).resolve().parent.parent / "include"]
+    tmp = CALLS.with_suffix(".so.tmp")
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-I", str(INCLUDE),
+           *(x for i in include for x in ("-isystem", str(i))), str(CSRC / "serving_calls.cpp"), "-o", str(tmp),
+           "-L", str(home / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for serving_calls.cpp:\n{r.stderr[-8000:]}")
+    os.replace(tmp, CALLS)
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     if not force and not needs_build():
         return LIB
     OBJ_DIR.mkdir(exist_ok=True)
-    with cf.ThreadPoolExecutor(max_workers=len(SOURCES)) as ex:
+    with cf.ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
+        calls = ex.submit(_build_calls)
         results = list(ex.map(lambda s: _compile(s, verbose), SOURCES))
+    calls.result()
     objs = [o for o, _ in results]
     if verbose:
         for _, log in results:

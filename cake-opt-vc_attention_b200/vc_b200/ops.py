@@ -270,13 +270,23 @@ def attention_fwd(q8, qs, k8, ks, v8, vs, means, *, out_dtype=torch.bfloat16, sm
 # Paged 4-bit K/V cache and window attention (inference only).
 #
 # A decoding step makes several of these calls, and for one sequence their GPU
-# time is a few microseconds each: the wrappers therefore read each tensor's
-# shape and strides once and make no views (NHD is a matter of the order in
-# which the axes are read).
+# time is a few microseconds each.  Arguments that need no conversion therefore
+# go through the extension ``_serving_calls``, which leaves everything else,
+# refusals included, to the code here by returning NotImplemented; that code
+# reads each tensor's shape and strides once and makes no views (NHD is a matter
+# of the order in which the axes are read).
 # ---------------------------------------------------------------------------
 KV4_RECORD_TOKENS = 16
 _F16, _BF16, _I32, _U8, _F32 = torch.float16, torch.bfloat16, torch.int32, torch.uint8, torch.float32
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # current_stream(i).cuda_stream without the object
+
+
+def _direct(name, *args):
+    """The call through the extension; NotImplemented where it does not take the arguments."""
+    r = getattr(N.calls(), name)(*args)
+    if type(r) is int:   # the library's status
+        N.check(r, name)
+    return r
 
 
 def _bhsd(name, what, t, layout, dtype, device):
@@ -403,6 +413,9 @@ def kv4_append(pool: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tens
     index has no page is not written and bit 0x80 of ``error_word`` is set.
     """
     name = "kv4_append"
+    r = _direct(name, pool, page_table, lengths, k, v, q, cos, sin, positions, counts, interleaved, tensor_layout)
+    if r is not NotImplemented:
+        return r
     _serving(name, tensor_layout, k)
     dev, dt = k.device, k.dtype
     H, D, page, B, width, pages = _cache(name, pool, page_table, dev)
@@ -451,6 +464,9 @@ def kv4_read(pool: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor |
     0) to ``start[b] + count - 1`` of every sequence: (K, V) in ``dtype``
     (FP16, BF16 or FP32), [B,Hkv,count,D] or [B,count,Hkv,D] for NHD."""
     name = "kv4_read"
+    r = _direct(name, pool, page_table, start, count, dtype, tensor_layout)
+    if r is not NotImplemented:
+        return r
     if tensor_layout != "HND" and tensor_layout != "NHD":
         raise ValueError(f"{name}: tensor_layout must be HND or NHD")
     if dtype not in _DT:
@@ -506,6 +522,10 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor,
     like ``q``, or ``out``.
     """
     name = "kv4_attention"
+    if out is None:
+        r = _direct(name, q, pool, page_table, lengths, q_lengths, causal, window, sinks, sm_scale, max_length, tensor_layout)
+        if r is not NotImplemented:
+            return r
     _serving(name, tensor_layout, q)
     dev, dt, q0 = q.device, q.dtype, q
     H, D, page, B, width, pages = _cache(name, pool, page_table, dev)
@@ -551,6 +571,10 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     or ``out``.
     """
     name = "window_attention"
+    if out is None:
+        r = _direct(name, q, k, v, window, sinks, causal, kv_lengths, sm_scale, tensor_layout)
+        if r is not NotImplemented:
+            return r
     _serving(name, tensor_layout, q)
     dev, dt, q0 = q.device, q.dtype, q
     view = q, qp, B, Hq, Sq, D, qsb, qsh, qss = _bhsd(name, "q", q, tensor_layout, dt, dev)

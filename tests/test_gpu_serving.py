@@ -470,6 +470,80 @@ def test_prompt_then_tokens_matches_one_long_call(ops):
     _check(torch.cat(outs, 2), want, BF, D, 11)
 
 
+@pytest.mark.parametrize("H,Sq,Sk,causal", [(160, 20, 1100, True), (80, 130, 3200, False), (100, 40, 4100, True)])
+def test_items_cut_after_the_full_waves(ops, H, Sq, Sk, causal):
+    """One item a head: 12 of 160 in equal shares; 80 and 100 in a long and a short share each."""
+    g = _gen(H)
+    q, k, v = _randn(g, 1, H, Sq, 64), _randn(g, 1, H, Sk, 64), _randn(g, 1, H, Sk, 64)
+    got = ops.window_attention(q.cuda(), k.cuda(), v.cuda(), causal=causal)
+    assert torch.equal(got, ops.window_attention(q.cuda(), k.cuda(), v.cuda(), causal=causal))
+    _check(got, O.window_attention(q, k, v, causal=causal), BF, 64, 8)
+
+
+def test_items_cut_over_the_cache(ops):
+    g = _gen(5)
+    lengths = [3300, 3111]
+    pool, table, n = _filled(ops, g, 2, 40, 64, 64, lengths, dtype=HF)
+    q = _randn(g, 2, 40, 40, 64, dtype=HF)
+    got = ops.kv4_attention(q.cuda(), pool, table.cuda(), n.cuda())
+    _check(got, O.paged_attention(q, pool.cpu(), table, n), HF, 64, 11)
+
+
+def test_direct_calls_equal_the_wrappers(ops, monkeypatch):
+    """Arguments that the extension takes give the same through the wrappers' own code."""
+    from vc_b200 import _native as N
+    g = _gen(8)
+    B, Hq, H, S, D = 2, 6, 2, 70, 128
+    table = torch.randperm(8, generator=g).to(torch.int32).view(2, 4).cuda()
+    n = torch.tensor([3, 40], dtype=torch.int32, device="cuda")
+    cos, sin = torch.rand((256, 32), generator=g).cuda(), torch.rand((256, 32), generator=g).cuda()
+    counts = torch.tensor([70, 9], dtype=torch.int32, device="cuda")
+    pos = torch.randint(0, 256, (B, S), generator=g, dtype=torch.int32).cuda()
+    taken = []
+
+    def run(layout):
+        shape = (lambda h: (B, h, S, D)) if layout == "HND" else (lambda h: (B, S, h, D))
+        g2 = _gen(9)
+        q, k, v = (_randn(g2, *shape(h)).cuda() for h in (Hq, H, H))
+        pool = ops.kv4_pool(8, H, D, 64)
+        out = [ops.kv4_append(pool, table, n, k, v, q=q, cos=cos, sin=sin, tensor_layout=layout, interleaved=True),
+               ops.kv4_append(pool, table, n, k, v, positions=pos, counts=counts, cos=cos, sin=sin, tensor_layout=layout),
+               *ops.kv4_read(pool, table, n, 60, dtype=torch.float16, tensor_layout=layout),
+               *ops.kv4_read(pool, table, None, 60, tensor_layout=layout),
+               ops.kv4_attention(q, pool, table, n + S, tensor_layout=layout),
+               ops.kv4_attention(q, pool, table, n + S, q_lengths=counts, causal=False, window=30, sinks=5, sm_scale=0.05,
+                                 max_length=120, tensor_layout=layout),
+               ops.window_attention(q, k, v, tensor_layout=layout),
+               ops.window_attention(q, k, v, window=20, sinks=3, causal=False, kv_lengths=counts, sm_scale=0.2,
+                                    tensor_layout=layout), pool]
+        return out
+
+    class Counting:
+        def __getattr__(self, name):
+            fn = getattr(real, name)
+
+            def call(*a):
+                r = fn(*a)
+                taken.append(r is not NotImplemented)
+                return r
+            return call
+
+    class Refusing:
+        def __getattr__(self, name):
+            return lambda *a: NotImplemented
+
+    real = N.calls()
+    for layout in ("HND", "NHD"):
+        monkeypatch.setattr(N, "calls", Counting)
+        a = run(layout)
+        monkeypatch.setattr(N, "calls", Refusing)
+        b = run(layout)
+        for x, y in zip(a, b):
+            assert (x is None and y is None) or (x.dtype == y.dtype and x.shape == y.shape and torch.equal(x, y))
+    assert len(taken) == 16 and all(taken)
+    ops.error_word(0, clear=True)   # (the 120-token bound cut a sequence)
+
+
 def test_refusals_on_the_device(ops):
     g = _gen(1)
     pool = ops.kv4_pool(4, 2, 64, 16)

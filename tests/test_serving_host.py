@@ -156,3 +156,21 @@ def test_oracle_round_trips_its_own_records():
         rec[2048 + t * 8:2048 + t * 8 + 8] = torch.stack((s[0, t], m[0, t]), -1).to(torch.bfloat16).view(torch.uint8).flatten()
     k, _ = O.decode(pool, torch.zeros(1, dtype=torch.int32), 0, 5)
     assert torch.equal(k, y[0])
+
+
+def test_direct_calls_leave_what_they_do_not_take_to_the_wrappers():
+    from vc_b200 import _native as N
+    from vc_b200 import build as B
+    if not N.CALLS_PATH.exists():
+        B.build()
+    f = N.calls()
+    x = torch.zeros((1, 2, 4, 64), dtype=torch.bfloat16)
+    pool, table, n = torch.zeros((2, 2, 1, 1152), dtype=torch.uint8), torch.zeros((1, 2), dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    assert f.kv4_append(pool, table, n, x, x, None, None, None, None, None, False, "HND") is NotImplemented
+    assert f.kv4_read(pool, table, n, 1, torch.float16, "HND") is NotImplemented
+    assert f.kv4_attention(x, pool, table, n, None, True, None, 0, None, None, "HND") is NotImplemented
+    assert f.window_attention(x, x, x, None, 0, True, None, None, "HND") is NotImplemented
+    for name in ("kv4_append", "kv4_read", "kv4_attention", "window_attention"):
+        assert getattr(f, name)() is NotImplemented and getattr(f, name)(1, "a", None) is NotImplemented
+    with pytest.raises(TypeError):
+        f.bind(1)
