@@ -27,6 +27,15 @@
 // all is skipped for that group, and only tiles that are partly visible are
 // masked (by selection, so hidden scores may be anything).
 //
+// What bounds it.  The MMAs of a step (256 rows x 128 keys, D 128: 32 of 64
+// cycles) are 2048 cycles; the step takes about 3400, because a group's chain
+// (scores read, maximum, 128 exponentials a row, probabilities written) is
+// longer than the other group's MMAs.  2 x 4096 tokens, 28/4 heads, BF16, causal:
+// 247 us, 973 TFLOP/s or 59% of the measured GEMM rate, tensor pipe 48% (counters),
+// at 1.65 to 1.75 GHz under the power limit.  D 64 has half the MMA work and the
+// same chain: 1 x 4096 107 us against 129.  A CTA's start and end take about
+// 5 us in all, as long as two to three steps.
+//
 // K and V stages both hold [64-channel segment][key][128 bytes] with the
 // 128-byte swizzle: K is the K-major B operand of QK^T, V the MN-major B
 // operand of P.V, no transposition anywhere.
@@ -59,7 +68,9 @@ struct TileCfg {
   static constexpr int kKS = KV4 ? 2 : D == 128 ? 3 : 4;     // K ring
   static constexpr int kVS = KV4 ? 2 : D == 128 ? 2 : 4;     // V ring
   static constexpr int kRS = KV4 ? 3 : 0;                    // ring of raw half tiles (64 keys)
-  static constexpr int kPoly = SRC == kRecords ? 0 : 2;   // of eight pairs of exponentials, on the FMA pipe
+  // Of eight pairs of exponentials, on the FMA pipe: 2 x 4096 causal, D 128, 253 us with none, 247 with two, more is
+  // slower.  With the dequantising warps, which use that pipe themselves, none is best.
+  static constexpr int kPoly = SRC == kRecords ? 0 : 2;
   static constexpr int kRaw = 4 * Kv4Rec<D>::kBytes;
   static constexpr int kOffQ = 0;
   static constexpr int kOffK = kOffQ + 2 * kTile;
