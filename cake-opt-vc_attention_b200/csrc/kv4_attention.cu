@@ -647,14 +647,32 @@ Plan plan_of(const Kv4AttnArgs& a) {
   int64_t keys = kv4_most(a.cache, a.max_length);
   if (a.window > 0) keys = min64(keys, a.window + a.Sq + a.sinks + 2 * kTile);
   const int64_t tiles = (keys + kTile - 1) / kTile, items = a.cache.B * a.cache.Hkv;
-  const int64_t fit = 148 * (r.nt == 1 ? 4 : 2), warps = r.nt == 2 ? 6 : 4;
+  const int64_t fit = 148 * (r.nt == 1 ? 4 : 2), warps = r.nt == 2 ? 6 : 4;   // DecodeCfg's
   // One sequence: its heads' shares are alike, and half a wave of CTAs is enough (37741 keys of 4 heads: 14.6 us;
-  // a whole wave, whose results take longer to join, 17.9; a third 17.9).  Several: their lengths differ, so
-  // about 3.5 waves of CTAs to even them out, of at least twelve tiles a warp (a CTA costs about as much beside
-  // them) unless that leaves the GPU half empty (64 sequences up to 8192, 8 heads: 96 us; two waves 105, one 121).
-  const int64_t a_wave = (fit + items - 1) / items;
-  int64_t s = a.cache.B == 1 ? min64(fit / 2 / items, tiles / warps)
-                             : max64(min64(7 * fit / 2 / items, tiles / (12 * warps)), min64(2 * a_wave, (tiles + 3 * warps - 1) / (3 * warps)));
+  // a whole wave, whose results take longer to join, 17.9; a third 17.9).
+  int64_t s = min64(fit / 2 / items, tiles / warps);
+  if (a.cache.B > 1) {
+    // Several: the least of an estimate over 1 and the splits that fill half a wave, one, two, three or four, in
+    // units of a warp's tile on a full SM.  A CTA costs about 3 tiles beside its own (4.5 with more rows), a tile
+    // 0.3 + 0.7 y on an SM that is filled to y, and several waves even out the sequences' lengths.  D 128, 32/8
+    // heads, lengths from half to the whole: 16 sequences up to 4096 tokens 4 splits 22 us, 7 29 us; 32 up to 2048 2
+    // splits 24 us, 1 26, 4 26; 64 up to 1024 1 split 21 us, 2 26, 4 31; 64 up to 8192 4 splits 97 us, 2 105, 1 121.
+    const double each = r.nt == 1 ? 3.0 : 4.5;
+    double best = 0.0;
+    s = 0;
+    for (int half_waves : {0, 1, 2, 4, 6, 8}) {
+      const int64_t t = max64(1, min64(min64(half_waves * fit / 2 / items, (tiles + warps - 1) / warps), kMostSplits));
+      if (t == s) continue;
+      const double x = double(t * items) / double(fit), y = x - double(t * items / fit), n = double((tiles + t * warps - 1) / (t * warps));
+      double cost = (x - y) * (each + n) + (y > 0.0 ? each + n * (0.3 + 0.7 * y) : 0.0);
+      if (x > 1.0) cost *= 0.62 + 0.38 / x;
+      if (t > 1) cost += 1.0 + double(t) / 40.0;   // the join
+      if (best == 0.0 || cost < best) {
+        best = cost;
+        s = t;
+      }
+    }
+  }
   r.splits = static_cast<int>(s < 1 ? 1 : min64(s, kMostSplits));
   return r;
 }
