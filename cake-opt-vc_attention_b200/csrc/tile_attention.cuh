@@ -110,6 +110,21 @@ __device__ __forceinline__ UnpackedTiles unpacked_tiles(const Visibility& v, int
   return u;
 }
 
+// n / d for n < 2^31 by a multiplication: a CTA's start has six divisions in a
+// row, 1000 cycles of it in all.
+struct Divisor {
+  uint32_t d, mul, shift;
+  __device__ __forceinline__ int of(int n) const {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), mul) + static_cast<uint32_t>(n)) >> shift);
+  }
+};
+inline Divisor divisor(int64_t d) {
+  Divisor r{static_cast<uint32_t>(d), 0, 0};
+  while ((int64_t(1) << r.shift) < d) ++r.shift;
+  r.mul = static_cast<uint32_t>(((uint64_t(1) << 32) * ((uint64_t(1) << r.shift) - r.d)) / r.d + 1);
+  return r;
+}
+
 struct TileParams {
   const void* q;
   void* out;
@@ -118,6 +133,7 @@ struct TileParams {
   int Hkv, BH;                 // BH = B * Hkv
   int G, rows, pairs;          // rows = Sq * G
   int whole, cut, splits, first;   // TilePlan
+  Divisor by_G, by_Hkv, by_BH, by_cut;
   Visibility vis;
   float scale_log2;            // sm_scale * log2(e)
   const int32_t *lengths, *q_lengths;
@@ -220,12 +236,12 @@ __device__ __forceinline__ uint32_t visible_bits(int lo, int hi, int sink, int k
   return (bits_below(hi - k) & ~bits_below(lo - k)) | bits_below(sink - k);
 }
 
-__device__ __forceinline__ GroupKeys group_keys(const Visibility& v, int base, int r0, int live, int G, int len) {
+__device__ __forceinline__ GroupKeys group_keys(const Visibility& v, int base, int r0, int live, const Divisor& G, int len) {
   GroupKeys k{};
   k.any = r0 < live;
   if (!k.any) return k;
-  const KeyRanges a = visible_keys(v, base + r0 / G, len);
-  const KeyRanges z = visible_keys(v, base + (min(r0 + 128, live) - 1) / G, len);
+  const KeyRanges a = visible_keys(v, base + G.of(r0), len);
+  const KeyRanges z = visible_keys(v, base + G.of(min(r0 + 128, live) - 1), len);
   k.hi = z.hi;
   k.lo = a.lo;
   k.sink_end = v.window ? min(v.sinks, z.hi) : 0;
@@ -251,38 +267,15 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
   int item = blockIdx.x, split = 0;
   const bool cut = item >= p.whole;
   if (cut) {
-    split = (item - p.whole) / p.cut;
+    split = p.by_cut.of(item - p.whole);
     item -= split * p.cut;
   }
-  const int pair = p.pairs - 1 - item / p.BH;
-  const int bh = item % p.BH, b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  const int from_end = p.by_BH.of(item), pair = p.pairs - 1 - from_end;
+  const int bh = item - from_end * p.BH, b = p.by_Hkv.of(bh), hk = bh - b * p.Hkv;
 
   if (warp == 9) {
     tmem_alloc(&ctl->slot, 512);
     tmem_relinquish();
-  }
-  if (threadIdx.x == 256) {
-    for (int s = 0; s < 4; ++s) {
-      mbar_init(&ctl->k_full[s], kDequant ? 64 : 1);
-      mbar_init(&ctl->step_done[s], 1);
-      mbar_init(&ctl->v_full[s], kDequant ? 64 : 1);
-      if constexpr (kDequant) mbar_init(&ctl->meta_full[s], 128);
-    }
-    if constexpr (kDequant) {
-      for (int s = 0; s < 3; ++s) {
-        mbar_init(&ctl->raw_full[s], 1);
-        mbar_init(&ctl->raw_empty[s], 4);
-      }
-    } else {
-      mbar_init(&ctl->v_fix, 1);
-    }
-    for (int x = 0; x < 2; ++x) {
-      mbar_init(&ctl->q_ready[x], 128);
-      mbar_init(&ctl->s_full[x], 1);
-      mbar_init(&ctl->p_full[x], 128);
-      mbar_init(&ctl->o_final[x], 1);
-    }
-    fence_barrier_init();
   }
   if (p.cut > 0) allow_dependent_launch();
   int len, nq, base;
@@ -295,8 +288,8 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
     base = p.Sk - p.Sq;
   }
   const int live = nq * p.G;
-  const GroupKeys ga = group_keys(p.vis, base, pair * 256, live, p.G, len);
-  const GroupKeys gb = group_keys(p.vis, base, pair * 256 + 128, live, p.G, len);
+  const GroupKeys ga = group_keys(p.vis, base, pair * 256, live, p.by_G, len);
+  const GroupKeys gb = group_keys(p.vis, base, pair * 256 + 128, live, p.by_G, len);
   // the list of tiles: sinks [0, nsink), then [main0, main0 + ...)
   int main0 = 0, nsink = 0, total = 0;
   if (ga.any) {
@@ -319,9 +312,57 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
     return i < nsink ? i : main0 + (i - nsink);
   };
 
+  if (threadIdx.x == 256) {
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&ctl->k_full[s], kDequant ? 64 : 1);
+      mbar_init(&ctl->step_done[s], 1);
+      mbar_init(&ctl->v_full[s], kDequant ? 64 : 1);
+      if constexpr (kDequant) mbar_init(&ctl->meta_full[s], 128);
+    }
+    if constexpr (kDequant) {
+      for (int s = 0; s < 3; ++s) {
+        mbar_init(&ctl->raw_full[s], 1);
+        mbar_init(&ctl->raw_empty[s], 4);
+      }
+    } else {
+      mbar_init(&ctl->v_fix, 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&ctl->q_ready[x], 128);
+      mbar_init(&ctl->s_full[x], 1);
+      mbar_init(&ctl->p_full[x], 128);
+      mbar_init(&ctl->o_final[x], 1);
+    }
+    fence_barrier_init();
+    if constexpr (SRC == kTensors) {   // the first keys are fetched while the rest is set up
+      fence_proxy_async_smem();
+      for (int n = 0; n < C::kKS && n < steps; ++n) {
+        mbar_expect_tx(&ctl->k_full[n], C::kTile);
+        for (int g = 0; g < kSegs; ++g) tma_load_4d(smem + C::kOffK + n * C::kTile + g * kSeg, &tmk, &ctl->k_full[n], g * 64, tile_of(n) * 128, hk, b);
+      }
+    }
+  }
   if constexpr (!kDequant) {
-    if (warp == 8 && lane == 0) tma_prefetch_desc(&tmk);
+    if (SRC != kTensors && warp == 8 && lane == 0) tma_prefetch_desc(&tmk);
     if (warp == 10 && lane == 0) tma_prefetch_desc(&tmv);
+  }
+  // Q and the output move between global memory and the tile of shared memory a warp's 32 rows at a
+  // time, D/8 lanes a row (16 bytes each), so that rows are read and written whole.  A lane has its own
+  // row's offset and gets the others' by shuffles.  Q's loads are all in flight at once, before the
+  // CTA's first barrier: its start counts, the SM has no other CTA.
+  constexpr int kRowLanes = D / 8, kRowsAt = 32 / kRowLanes;
+  const int rl = lane / kRowLanes, ch = lane % kRowLanes;
+  const int row0 = pair * 256 + warp * 32, row = row0 + lane;   // softmax warps: the warp's first row, the lane's
+  const int tok = p.by_G.of(row), head = hk * p.G + (row - tok * p.G);
+  uint4 qv[32 / kRowsAt];
+  if (warp < 8) {
+    const int64_t off = int64_t(b) * p.qsb + head * p.qsh + tok * p.qss;
+#pragma unroll
+    for (int i = 0; i < 32 / kRowsAt; ++i) {
+      const int lr = i * kRowsAt + rl;
+      const QT* src = static_cast<const QT*>(p.q) + __shfl_sync(0xffffffffu, off, lr) + ch * 8;
+      qv[i] = row0 + lr < live ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -395,7 +436,7 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
       auto first_row = [&](int n) -> int { return (SRC == kUnpacked ? un.slot(tile_of(n)) : tile_of(n)) * 128; };
       if (warp == 8 && lane == 0) {
         // ----------------------------------------------------------- K producer
-        for (int n = 0; n < steps; ++n) {
+        for (int n = SRC == kTensors ? C::kKS : 0; n < steps; ++n) {
           const int s = n % C::kKS;
           if (n >= C::kKS && !mbar_wait(&ctl->step_done[(n - C::kKS) & 3], ((n - C::kKS) >> 2) & 1, kErrTimeoutProducer)) break;
           mbar_expect_tx(&ctl->k_full[s], C::kTile);
@@ -578,22 +619,19 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t scol = tmem + lane_base + x * 128, ocol = tmem + lane_base + 256 + x * 128;
     const GroupKeys g = x ? gb : ga;
-    const int row0 = pair * 256 + x * 128 + (warp & 3) * 32;   // this warp's first row
-    const int row = row0 + lane;
-    const int tok = row / p.G;
     float c_row = p.scale_log2;
-    // Q and the output move between global memory and the tile of shared memory a warp's 32 rows at a
-    // time, D/8 lanes a row (16 bytes each), so that rows are read and written whole
-    constexpr int kRowLanes = D / 8, kRowsAt = 32 / kRowLanes;
-    const int rl = lane / kRowLanes, ch = lane % kRowLanes;
     uint8_t* tile_mem = smem + C::kOffQ + x * C::kTile;
     {
-#pragma unroll 4
-      for (int i = 0; i < 32 / kRowsAt; ++i) {
-        const int lr = i * kRowsAt + rl, r = row0 + lr, rt = __shfl_sync(0xffffffffu, tok, lr), rh = hk * p.G + (r - rt * p.G);
-        const QT* src = static_cast<const QT*>(p.q) + int64_t(b) * p.qsb + rh * p.qsh + rt * p.qss + ch * 8;
-        uint4 u = r < live ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
-        if constexpr (KV4) {
+      auto at = [&](int i) -> uint4* {
+        return reinterpret_cast<uint4*>(tile_mem + (ch >> 3) * kSeg + swizzled((warp & 3) * 32 + i * kRowsAt + rl, ch & 7));
+      };
+#pragma unroll
+      for (int i = 0; i < 32 / kRowsAt; ++i) *at(i) = qv[i];
+      if constexpr (KV4) {   // to FP16, in place
+#pragma unroll 2
+        for (int i = 0; i < 32 / kRowsAt; ++i) {
+          const int lr = i * kRowsAt + rl;
+          const uint4 u = *at(i);
           float f[8];
           const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -620,10 +658,9 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
             up = __uint_as_float(uint32_t(127 + e) << 23);
             if (ch == 0) ctl->q_unit[x][(warp & 3) * 32 + lr] = __uint_as_float(uint32_t(127 - e) << 23);
           }
-          u = make_uint4(pack2<__half>(f[0] * up, f[4] * up), pack2<__half>(f[1] * up, f[5] * up),
-                         pack2<__half>(f[2] * up, f[6] * up), pack2<__half>(f[3] * up, f[7] * up));
+          *at(i) = make_uint4(pack2<__half>(f[0] * up, f[4] * up), pack2<__half>(f[1] * up, f[5] * up),
+                              pack2<__half>(f[2] * up, f[6] * up), pack2<__half>(f[3] * up, f[7] * up));
         }
-        *reinterpret_cast<uint4*>(tile_mem + (ch >> 3) * kSeg + swizzled((warp & 3) * 32 + lr, ch & 7)) = u;
       }
       if constexpr (KV4 && std::is_same<QT, __nv_bfloat16>::value) {
         __syncwarp();
@@ -841,11 +878,13 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
       }
       if (!cut) {
         __syncwarp();
-#pragma unroll 2
+        const int64_t off = int64_t(b) * p.osb + head * p.osh + tok * p.oss;
+#pragma unroll 8
         for (int i = 0; i < 32 / kRowsAt; ++i) {
-          const int lr = i * kRowsAt + rl, r = row0 + lr, rt = __shfl_sync(0xffffffffu, tok, lr), rh = hk * p.G + (r - rt * p.G);
+          const int lr = i * kRowsAt + rl;
           const uint4 u = *reinterpret_cast<const uint4*>(tile_mem + (ch >> 3) * kSeg + swizzled((warp & 3) * 32 + lr, ch & 7));
-          if (r < p.rows) *reinterpret_cast<uint4*>(static_cast<QT*>(p.out) + int64_t(b) * p.osb + rh * p.osh + rt * p.oss + ch * 8) = u;
+          QT* dst = static_cast<QT*>(p.out) + __shfl_sync(0xffffffffu, off, lr) + ch * 8;
+          if (row0 + lr < p.rows) *reinterpret_cast<uint4*>(dst) = u;
         }
       }
       if (cut && row < p.rows) p.part_ml[at] = seen ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
@@ -945,6 +984,10 @@ inline void set_plan(TileParams& p, const TilePlan& t, void* partials, int64_t D
   p.cut = static_cast<int>(t.cut);
   p.splits = static_cast<int>(t.splits);
   p.first = static_cast<int>(t.first);
+  p.by_G = divisor(p.G);
+  p.by_Hkv = divisor(p.Hkv);
+  p.by_BH = divisor(p.BH);
+  p.by_cut = divisor(t.cut > 0 ? t.cut : 1);
   p.part_o = static_cast<float*>(partials);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + t.part_rows() * D);
 }
