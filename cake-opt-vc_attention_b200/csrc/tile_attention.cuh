@@ -31,10 +31,11 @@
 // cycles) are 2048 cycles; the step takes about 3400, because a group's chain
 // (scores read, maximum, 128 exponentials a row, probabilities written) is
 // longer than the other group's MMAs.  2 x 4096 tokens, 28/4 heads, BF16, causal:
-// 247 us, 973 TFLOP/s or 59% of the measured GEMM rate, tensor pipe 48% (counters),
+// 238 us, 1010 TFLOP/s or 62% of the measured GEMM rate, tensor pipe 48% (counters),
 // at 1.65 to 1.75 GHz under the power limit.  D 64 has half the MMA work and the
-// same chain: 1 x 4096 107 us against 129.  A CTA's start and end take about
-// 5 us in all, as long as two to three steps.
+// same chain: 1 x 4096 107 us against 129.  A CTA's start takes about 8000 cycles
+// (160 KB of Q, K and V come into the SM before the second tile's scores) and its
+// end 6000, together as long as four steps.
 //
 // K and V stages both hold [64-channel segment][key][128 bytes] with the
 // 128-byte swizzle: K is the K-major B operand of QK^T, V the MN-major B
@@ -68,8 +69,8 @@ struct TileCfg {
   static constexpr int kKS = KV4 ? 2 : D == 128 ? 3 : 4;     // K ring
   static constexpr int kVS = KV4 ? 2 : D == 128 ? 2 : 4;     // V ring
   static constexpr int kRS = KV4 ? 3 : 0;                    // ring of raw half tiles (64 keys)
-  // Of eight pairs of exponentials, on the FMA pipe: 2 x 4096 causal, D 128, 253 us with none, 247 with two, more is
-  // slower.  With the dequantising warps, which use that pipe themselves, none is best.
+  // Of eight pairs of exponentials, on the FMA pipe: 2 x 4096 causal, D 128, none is 2.5% slower than two, and so is
+  // more.  With the dequantising warps, which use that pipe themselves, none is best.
   static constexpr int kPoly = SRC == kRecords ? 0 : 2;
   static constexpr int kRaw = 4 * Kv4Rec<D>::kBytes;
   static constexpr int kOffQ = 0;
@@ -334,11 +335,11 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
       mbar_init(&ctl->o_final[x], 1);
     }
     fence_barrier_init();
-    if constexpr (SRC == kTensors) {   // the first keys are fetched while the rest is set up
+    if constexpr (SRC == kTensors) {   // the first tile of keys is fetched while the rest is set up
       fence_proxy_async_smem();
-      for (int n = 0; n < C::kKS && n < steps; ++n) {
-        mbar_expect_tx(&ctl->k_full[n], C::kTile);
-        for (int g = 0; g < kSegs; ++g) tma_load_4d(smem + C::kOffK + n * C::kTile + g * kSeg, &tmk, &ctl->k_full[n], g * 64, tile_of(n) * 128, hk, b);
+      if (steps > 0) {
+        mbar_expect_tx(&ctl->k_full[0], C::kTile);
+        for (int g = 0; g < kSegs; ++g) tma_load_4d(smem + C::kOffK + g * kSeg, &tmk, &ctl->k_full[0], g * 64, tile_of(0) * 128, hk, b);
       }
     }
   }
@@ -436,7 +437,7 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
       auto first_row = [&](int n) -> int { return (SRC == kUnpacked ? un.slot(tile_of(n)) : tile_of(n)) * 128; };
       if (warp == 8 && lane == 0) {
         // ----------------------------------------------------------- K producer
-        for (int n = SRC == kTensors ? C::kKS : 0; n < steps; ++n) {
+        for (int n = SRC == kTensors ? 1 : 0; n < steps; ++n) {
           const int s = n % C::kKS;
           if (n >= C::kKS && !mbar_wait(&ctl->step_done[(n - C::kKS) & 3], ((n - C::kKS) >> 2) & 1, kErrTimeoutProducer)) break;
           mbar_expect_tx(&ctl->k_full[s], C::kTile);
