@@ -682,6 +682,8 @@ Plan plan_of(const Kv4AttnArgs& a) {
 // (28/4 heads): 28 rows 20 us here, 22 there; 49 rows 30 in two CTAs, 24 there.
 // 16 sequences up to 8192 (32/8 heads): 32 rows 122 and 146, 48 rows 203 and
 // 147.  D 64, 8 up to 4096 (24/24 heads): 32 rows 49 and 75, 48 rows 81 and 75.
+// (FP16 results at D 128, 25 to 32 rows, spill: 155 and 149, 37 and 32; the
+// workspace query does not know the type, so that is left.)
 constexpr int64_t kMostRows = 32;
 bool use_tiles(const Kv4AttnArgs& a) { return a.Sq * (a.Hq / a.cache.Hkv) > kMostRows; }
 

@@ -237,6 +237,10 @@ KV4 = [  # lengths, Sq, Hq, Hkv, D, page, dtype, layout, causal, window, sinks
     ([500, 450], 257, 4, 4, 64, 128, HF, "NHD", False, 200, 30),
     ([900], 300, 2, 1, 128, 32, HF, "HND", True, 70, 10),
     ([40, 1030], 40, 28, 4, 128, 16, BF, "NHD", False, 0, 0),
+    ([600, 90], 7, 8, 2, 128, 64, HF, "HND", True, 0, 0),
+    ([600, 90], 7, 8, 2, 128, 64, BF, "HND", True, 0, 0),
+    ([600, 90], 6, 8, 2, 128, 64, HF, "NHD", True, 200, 7),
+    ([333], 32, 3, 3, 64, 32, HF, "HND", False, 0, 0),
 ]
 
 
