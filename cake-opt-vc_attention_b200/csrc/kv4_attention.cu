@@ -147,6 +147,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, NT>::kThreads, DecodeCfg<D, NT>::
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar) + warp * L::kStages;
   if (lane < L::kStages) mbar_init(&bars[lane], 1);
   fence_barrier_init();
+  wait_for_previous();
   if (p.splits > 1) allow_dependent_launch();
   int len, nq;
   kv4_sequence(p.pages, p.lengths, p.q_lengths, static_cast<int>(p.Sq), b, len, nq);
@@ -695,7 +696,7 @@ int launch_decode(const DecodeParams& p, const Plan& plan, int64_t BH, cudaStrea
   constexpr int bytes = DecodeCfg<D, NT>::kBytes;
   static std::atomic<uint64_t> ready{0};
   if (!allow_smem(reinterpret_cast<const void*>(k), bytes, ready)) return VC_ERR_LAUNCH;
-  k<<<dim3(plan.splits, static_cast<unsigned>(BH)), DecodeCfg<D, NT>::kThreads, bytes, st>>>(p);
+  if (launch_early(k, dim3(plan.splits, static_cast<unsigned>(BH)), DecodeCfg<D, NT>::kThreads, bytes, st, p) != cudaSuccess) return VC_ERR_LAUNCH;
   if (plan.splits > 1) {
     const JoinParams j{p.part_o, p.part_ml, p.out, p.osb, p.osh, p.oss, p.pages.heads, p.rows, p.G, p.splits};
     if (launch_join<D, T>(j, BH * p.rows, st) != cudaSuccess) return VC_ERR_LAUNCH;

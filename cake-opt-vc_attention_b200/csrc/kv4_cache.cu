@@ -15,6 +15,7 @@
 // half-style rotation partner of a lane is R/16 lanes away (one shuffle a
 // channel), the eight codes of a lane are one 32-bit store.
 #include <type_traits>
+#include "join.cuh"
 #include "kernels.h"
 #include "kv4.cuh"
 
@@ -106,6 +107,7 @@ __global__ void __launch_bounds__(kThreads, HEADS > 1 ? 4 : 1) kv4_append_kernel
   const bool live = token < p.B * p.S;
   const int b = live ? sequence_of(token, p.B * p.S, p.S) : 0;
   const int64_t t = live ? token - b * p.S : 0;
+  wait_for_previous();
   const bool write = live && (!p.counts || t < __ldg(p.counts + b));
   const int c0 = l * 8;
   // the block's heads; everything about them is the same in the whole block
@@ -265,6 +267,7 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(ReadParams p) {
   const int l = static_cast<int>(i % L), which = blockIdx.z;
   const int h = blockIdx.y, n = static_cast<int>(p.N);
   const int64_t row = i / L;
+  wait_for_previous();
   if (row >= p.B * p.N) return;
   const int b = sequence_of(row, p.B * n, n), t = static_cast<int>(row - int64_t(b) * n);
   const int64_t at = (p.start ? int64_t(__ldg(p.start + b)) : 0) + t;
@@ -297,7 +300,7 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(ReadParams p) {
   }
 }
 
-int launched() { return cudaGetLastError() == cudaSuccess ? VC_OK : VC_ERR_LAUNCH; }
+int launched(cudaError_t e) { return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? VC_OK : VC_ERR_LAUNCH; }
 
 }  // namespace
 
@@ -315,14 +318,13 @@ int kv4_append(const Kv4AppendArgs& a, cudaStream_t st) {
   auto go = [&](auto tag, auto dim) {
     using T = decltype(tag);
     constexpr int D = decltype(dim)::value;
-    if (many) kv4_append_kernel<D, T, 4><<<grid, kThreads, 0, st>>>(p);
-    else kv4_append_kernel<D, T, 1><<<grid, kThreads, 0, st>>>(p);
+    return many ? launch_early(kv4_append_kernel<D, T, 4>, grid, kThreads, 0, st, p)
+                : launch_early(kv4_append_kernel<D, T, 1>, grid, kThreads, 0, st, p);
   };
   using D128 = std::integral_constant<int, 128>;
   using D64 = std::integral_constant<int, 64>;
-  if (a.dtype == VC_DTYPE_BF16) a.D == 128 ? go(__nv_bfloat16(), D128()) : go(__nv_bfloat16(), D64());
-  else a.D == 128 ? go(__half(), D128()) : go(__half(), D64());
-  return launched();
+  if (a.dtype == VC_DTYPE_BF16) return launched(a.D == 128 ? go(__nv_bfloat16(), D128()) : go(__nv_bfloat16(), D64()));
+  return launched(a.D == 128 ? go(__half(), D128()) : go(__half(), D64()));
 }
 
 int kv4_read(const Kv4ReadArgs& a, cudaStream_t st) {
@@ -331,13 +333,10 @@ int kv4_read(const Kv4ReadArgs& a, cudaStream_t st) {
   const dim3 grid(static_cast<unsigned>((threads + kThreads - 1) / kThreads), static_cast<unsigned>(a.cache.Hkv), 2);
   auto go = [&](auto tag) {
     using T = decltype(tag);
-    if (a.D == 128) kv4_read_kernel<128, T><<<grid, kThreads, 0, st>>>(p);
-    else kv4_read_kernel<64, T><<<grid, kThreads, 0, st>>>(p);
+    return a.D == 128 ? launch_early(kv4_read_kernel<128, T>, grid, kThreads, 0, st, p)
+                      : launch_early(kv4_read_kernel<64, T>, grid, kThreads, 0, st, p);
   };
-  if (a.dtype == VC_DTYPE_BF16) go(__nv_bfloat16());
-  else if (a.dtype == VC_DTYPE_F16) go(__half());
-  else go(float());
-  return launched();
+  return launched(a.dtype == VC_DTYPE_BF16 ? go(__nv_bfloat16()) : a.dtype == VC_DTYPE_F16 ? go(__half()) : go(float()));
 }
 
 cudaError_t kv4_cache_error_word(uint32_t* code, bool clear) { return read_tu_error_word(code, clear); }

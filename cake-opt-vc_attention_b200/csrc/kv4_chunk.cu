@@ -5,7 +5,7 @@
 // Every CTA (256 rows) reads all keys of its head, so with several CTAs a head
 // the dequantising warps of each do the same work again, and they take issue
 // slots from the softmax: the chunk of 1024 tokens over 16384 (28/4 heads,
-// D 128; 28 CTAs a head) takes 396 us that way and 251 us unpacked first,
+// D 128; 28 CTAs a head) takes 396 us that way and 254 us unpacked first,
 // of which the unpacking is about 12.  With one CTA a head it is 32 us fused and
 // 34 unpacked, with two 49 and 45, with four 74 and 63.  So: unpack when a head
 // has two CTAs or more.  The FP16 tiles take 3.6 times the cache's bytes, so
@@ -67,6 +67,7 @@ __global__ void __launch_bounds__(256) kv4_unpack_kernel(UnpackParams p) {
   __shared__ uint2 par[2][D / 64][128];   // scale and minimum twice, FP16
   const int bh = blockIdx.y, b = bh / static_cast<int>(p.pages.heads), hk = bh % static_cast<int>(p.pages.heads);
   int len, nq;
+  wait_for_previous();
   allow_dependent_launch();
   kv4_sequence(p.pages, p.lengths, p.q_lengths, p.Sq, b, len, nq);
   const UnpackedTiles un = unpacked_tiles(p.vis, len, nq);
@@ -182,8 +183,8 @@ int run(const Kv4AttnArgs& a, const ChunkPlan& plan, TileParams& p, cudaStream_t
   uint8_t* v = k + plan.tile_bytes;
   TileMeta* meta = reinterpret_cast<TileMeta*>(v + plan.tile_bytes);
   const UnpackParams u{p.pages, a.lengths, a.q_lengths, p.Sq, static_cast<int>(plan.slots), p.vis, k, v, meta};
-  kv4_unpack_kernel<D><<<dim3(static_cast<unsigned>(plan.slots), static_cast<unsigned>(p.BH)), 256, 0, st>>>(u);
-  if (cudaGetLastError() != cudaSuccess) return VC_ERR_LAUNCH;
+  if (launch_early(kv4_unpack_kernel<D>, dim3(static_cast<unsigned>(plan.slots), static_cast<unsigned>(p.BH)), 256, 0, st, u) != cudaSuccess)
+    return VC_ERR_LAUNCH;
   CUtensorMap mk, mv;
   const int64_t S = plan.slots * 128, H = a.cache.Hkv;
   if (!make_map(&mk, k, VC_DTYPE_F16, a.cache.B, H, S, D, H * S * D, S * D, D) ||

@@ -274,6 +274,8 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
   const int from_end = p.by_BH.of(item), pair = p.pairs - 1 - from_end;
   const int bh = item - from_end * p.BH, b = p.by_Hkv.of(bh), hk = bh - b * p.Hkv;
 
+  // (before tensor memory is taken, which the kernel before may still have to)
+  wait_for_previous();
   if (warp == 9) {
     tmem_alloc(&ctl->slot, 512);
     tmem_relinquish();
@@ -369,9 +371,6 @@ __global__ void __launch_bounds__(TileCfg<D, SRC>::kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ctl->slot;
-  // launched while the cache is still being unpacked; nothing above reads what that kernel writes
-  if constexpr (SRC == kUnpacked) asm volatile("griddepcontrol.wait;" ::: "memory");
-
   if (warp >= 8) {
     if constexpr (kDequant) setmaxnreg_dec<64>();
     else setmaxnreg_dec<88>();
@@ -1001,17 +1000,8 @@ int launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, const TileParams&
   static_assert(bytes <= 227 * 1024, "shared memory");
   static std::atomic<uint64_t> ready{0};
   if (!allow_smem(reinterpret_cast<const void*>(k), bytes, ready)) return VC_ERR_LAUNCH;
-  cudaLaunchConfig_t c{};
-  c.gridDim = dim3(static_cast<unsigned>(p.whole) + static_cast<unsigned>(p.cut) * static_cast<unsigned>(p.splits));
-  c.blockDim = dim3(C::kThreads);
-  c.dynamicSmemBytes = bytes;
-  c.stream = st;
-  cudaLaunchAttribute early{};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  c.attrs = &early;
-  c.numAttrs = SRC == kUnpacked ? 1 : 0;
-  if (cudaLaunchKernelEx(&c, k, mk, mv, p) != cudaSuccess) return VC_ERR_LAUNCH;
+  const dim3 grid(static_cast<unsigned>(p.whole) + static_cast<unsigned>(p.cut) * static_cast<unsigned>(p.splits));
+  if (launch_early(k, grid, C::kThreads, bytes, st, mk, mv, p) != cudaSuccess) return VC_ERR_LAUNCH;
   if (p.cut > 0) {
     const JoinParams j{p.part_o, p.part_ml, p.out, p.osb, p.osh, p.oss, p.Hkv, p.rows, p.G, p.splits, p.whole, p.pairs, p.BH};
     if (launch_join<D, QT>(j, int64_t(p.cut) * 256, st) != cudaSuccess) return VC_ERR_LAUNCH;
